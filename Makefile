@@ -9,8 +9,9 @@ NOPACK   := -Xclang -target-feature -Xclang -packed-fp32-ops
 # wait for the atomic's round trip right where it is issued (k_resident_pipe claims its batches ahead of time)
 HIPFLAGS := -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) $(NOPACK) -mllvm -amdgpu-atomic-optimizer-strategy=None -Wall -Wextra -Wno-unused-parameter -Iinclude
 OBJS     := $(CSRC)/api.o $(CSRC)/kernels_scalar.o $(CSRC)/kernels_engine.o $(CSRC)/kernels_resident.o $(CSRC)/kernels_omega.o $(CSRC)/kernels_local.o $(CSRC)/kernels_long.o $(CSRC)/kernels_direct.o $(CSRC)/kernels_glvq.o \
+            $(CSRC)/kernels_scores.o $(CSRC)/kernels_sample.o $(CSRC)/kernels_lookup.o \
             $(CSRC)/kernels_project.o $(CSRC)/engine_host.o $(CSRC)/synth.o
-HDRS     := $(CSRC)/vq_common.h $(CSRC)/engine.h $(CSRC)/mfma_device.h $(CSRC)/mfma_host.h $(CSRC)/mfma_images.h include/vqhip.h
+HDRS     := $(CSRC)/vq_common.h $(CSRC)/engine.h $(CSRC)/mfma_device.h $(CSRC)/mfma_host.h $(CSRC)/mfma_images.h $(CSRC)/codes_device.h include/vqhip.h
 LIB      := vq_amd/libvqhip.so
 # the same objects as a static archive: what a build.rs links with `cargo:rustc-link-lib=static=vqhip`
 LIBA     := vq_amd/libvqhip.a

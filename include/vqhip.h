@@ -256,6 +256,73 @@ int vqhip_assign_f64(vqhip_ctx *ctx, const double *X, uint64_t N, uint32_t *idx_
 int vqhip_assign_matched_f64(vqhip_ctx *ctx, const double *X, const uint32_t *y, uint64_t N, uint32_t *jpos,
                              double *dpos, uint32_t *jneg, double *dneg);
 
+/* ---- sampled codes and codebook lookup -------------------------------------------------------------------------------
+ * What a program does around the search once prototypes are a codebook: draw a code per sample instead of taking the
+ * nearest, turn codes back into vectors, and train the table from the gradient of those vectors.  No counterpart in the
+ * reference beyond reading `prototypes[idx]` (src/glvq/glvq.rs:231).  All calls take device memory and enqueue on `stream`
+ * without host synchronisation; none allocates, none keeps anything in the context, so they may be captured into a HIP graph,
+ * and calls that overlap are independent as long as their outputs and workspaces are.  Rows of a matrix lie `ld` elements
+ * apart (ld >= its width); what lies between them is neither read nor written.  Outputs must not overlap inputs.  The device
+ * current on the calling thread stays current. */
+typedef enum { VQHIP_F32 = 0, VQHIP_BF16 = 1, VQHIP_F16 = 2 } vqhip_dtype;
+
+/* Scores of N samples against the context's prototypes: S[i][j] = - sum_d (x[i][d] - w[j][d])^2 (src/helpers.rs:18-20
+ * without the root), N x K, rows lds apart.  Euclidean models only (VQHIP_ERR_UNSUPPORTED with an Omega).  A softmax of
+ * S / T is the distribution over codes that vqhip_assign_sampled_device draws from.  Direct form in f32: a sample equal to a
+ * prototype scores 0 exactly. */
+int vqhip_scores_device(vqhip_ctx *ctx, const float *dX, uint64_t N, float *dS, uint64_t lds, void *stream);
+
+/* How to draw: one value for all rows, or, where the pointer is not NULL, one per row (N values on the device).
+ *   temperature  T >= 0, finite; 0 takes the first maximum
+ *   top_k        keep the top_k largest scores (equal ones: lower index first); 0 or >= V keeps all
+ *   top_p        of those, keep the fewest whose probabilities reach top_p, at least one; >= 1 keeps all
+ *   min_p        of those, keep the ones at least min_p times as probable as the most probable; 0 keeps all
+ * Single values outside these ranges (temperature negative or not finite, top_p or min_p outside [0, 1] or NaN) are
+ * VQHIP_ERR_INVALID.  Values read on the device cannot be refused: a temperature that is not finite and positive counts as
+ * 0, a top_p that is not below 1 keeps all and one not above 0 the first maximum, a min_p not above 0 keeps all and one above 1
+ * counts as 1. */
+typedef struct {
+    float temperature, top_p, min_p;
+    uint32_t top_k;
+    const float *dtemperature, *dtop_p, *dmin_p;
+    const uint32_t *dtop_k;
+} vqhip_sampling;
+
+/* One index per row of scores (logits), N x V of `dtype`, drawn with the given random numbers du[i] in [0, 1) (values outside
+ * are moved to the nearest inside, NaN to 0).  With w_j = exp((l_j - max l) / T) over the kept j: idx = the smallest kept j with
+ * sum over kept i <= j of w_i > u * (sum over all kept), prob = w_idx / (sum over all kept), 1 where T = 0.  dprob may be NULL.
+ * NaN and -inf are never drawn; a row of nothing else gives index 0 with probability 0.  A row whose maximum is +inf draws among
+ * its +inf.  V >= 1, below 2^31.  w and its sums are f64, so the index is that of the definition unless u falls within ~1e-15
+ * of a border; the same inputs give the same bits. */
+int vqhip_sample_device(vqhip_ctx *ctx, const void *dS, int dtype, uint64_t N, uint32_t V, uint64_t lds, const vqhip_sampling *how,
+                        const float *du, uint32_t *didx_out, float *dprob_out, void *stream);
+
+/* vqhip_assign_device with the winner drawn instead of nearest: vqhip_scores_device and vqhip_sample_device, a chunk of rows at a
+ * time through dwork (at least K floats, 4-byte aligned; vqhip_assign_sampled_workspace gives the size that keeps the card
+ * busy and the chunk in the last-level cache).  Results are those of the two calls. */
+int vqhip_assign_sampled_workspace(vqhip_ctx *ctx, uint64_t N, size_t *bytes);
+int vqhip_assign_sampled_device(vqhip_ctx *ctx, const float *dX, uint64_t N, const vqhip_sampling *how, const float *du, uint32_t *didx_out,
+                                float *dprob_out, void *dwork, size_t work_bytes, void *stream);
+
+/* Y[i] = scale * T[idx[i]] for N indices: T is K x D of `dtype`, rows ldt apart, Y is N x D of the same type, rows ldy apart.  An
+ * index outside [0, K) (VQHIP_NO_INDEX for padding) gives a row of zeros.  dT == NULL: the context's prototypes (f32; K, D and
+ * ldt must be the model's). The product is formed in f32 and rounded once. */
+#define VQHIP_NO_INDEX 0xFFFFFFFFu
+int vqhip_lookup_device(vqhip_ctx *ctx, const void *dT, int dtype, uint32_t K, uint32_t D, uint64_t ldt, const uint32_t *didx, uint64_t N,
+                        float scale, void *dY, uint64_t ldy, void *stream);
+
+/* The gradient of vqhip_lookup_device with respect to the table: dT[k] = scale * sum over { i : idx[i] == k } dY[i], K x D, rows
+ * ldt apart; accumulate != 0 adds to what dT holds and leaves rows no index names alone, 0 overwrites (zeros there).  dY is
+ * N x D of `dtype`, rows ldy apart; out_dtype is VQHIP_F32 or `dtype`.  dcounts (nullable): how many indices name each row, so
+ * that sums and counts of the samples of every code (the batch update of a codebook) are one call with scale 1.  Indices
+ * outside [0, K) contribute nothing; their rows of dY are not read.  Sums are f32 in an order the inputs alone fix: the same
+ * inputs give the same bits.  N below 2^31, K in [1, 2^31).  dwork: vqhip_lookup_gradient_workspace bytes, 256-byte aligned,
+ * free for other use once the call has run. */
+int vqhip_lookup_gradient_workspace(vqhip_ctx *ctx, uint64_t N, uint32_t K, uint32_t D, size_t *bytes);
+int vqhip_lookup_gradient_device(vqhip_ctx *ctx, const void *dY, int dtype, uint64_t ldy, const uint32_t *didx, uint64_t N, float scale, uint32_t K,
+                                 uint32_t D, void *dT, int out_dtype, uint64_t ldt, int accumulate, uint32_t *dcounts, void *dwork,
+                                 size_t work_bytes, void *stream);
+
 /* ---- introspection / measurement support ------------------------------------------------- */
 
 /* Name of the kernel family the last assign call on this context used ("scalar", "mfma_euclid",

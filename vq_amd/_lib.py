@@ -14,6 +14,16 @@ PROJECT_OMEGA, PROJECT_LAMBDA = 0, 1
 OPT_RANKING, OPT_PROJECTION = 0, 1
 VALUE_DEFAULT, VALUE_F32, VALUE_BF16 = 0, 1, 2
 
+F32, BF16, F16 = 0, 1, 2
+NO_INDEX = 0xFFFFFFFF
+
+
+class Sampling(C.Structure):
+    """vqhip_sampling: one value for all rows, or a device pointer to one per row."""
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", C.c_uint32),
+                ("dtemperature", C.c_void_p), ("dtop_p", C.c_void_p), ("dmin_p", C.c_void_p), ("dtop_k", C.c_void_p)]
+
+
 # name -> (restype, argtypes); the single list the symbol-export test walks too
 _f, _u, _v = C.POINTER(C.c_float), C.POINTER(C.c_uint32), C.c_void_p
 SIGNATURES = {
@@ -44,6 +54,14 @@ SIGNATURES = {
     "vqhip_glvq_batch_gradient": (C.c_int, [_v, _f, _u, C.c_uint64, _f, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]),
     "vqhip_glvq_batch_gradient_device": (C.c_int, [_v, _v, _v, C.c_uint64, _v, _v, _v]),
     "vqhip_multi_glvq_batch_gradient": (C.c_int, [_v, _f, _u, C.c_uint64, _f, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]),
+    "vqhip_scores_device": (C.c_int, [_v, _v, C.c_uint64, _v, C.c_uint64, _v]),
+    "vqhip_sample_device": (C.c_int, [_v, _v, C.c_int, C.c_uint64, C.c_uint32, C.c_uint64, C.POINTER(Sampling), _v, _v, _v, _v]),
+    "vqhip_assign_sampled_workspace": (C.c_int, [_v, C.c_uint64, C.POINTER(C.c_size_t)]),
+    "vqhip_assign_sampled_device": (C.c_int, [_v, _v, C.c_uint64, C.POINTER(Sampling), _v, _v, _v, _v, C.c_size_t, _v]),
+    "vqhip_lookup_device": (C.c_int, [_v, _v, C.c_int, C.c_uint32, C.c_uint32, C.c_uint64, _v, C.c_uint64, C.c_float, _v, C.c_uint64, _v]),
+    "vqhip_lookup_gradient_workspace": (C.c_int, [_v, C.c_uint64, C.c_uint32, C.c_uint32, C.POINTER(C.c_size_t)]),
+    "vqhip_lookup_gradient_device": (C.c_int, [_v, _v, C.c_int, C.c_uint64, _v, C.c_uint64, C.c_float, C.c_uint32, C.c_uint32, _v, C.c_int,
+                                               C.c_uint64, C.c_int, _v, _v, C.c_size_t, _v]),
     "vqhip_last_kernel": (C.c_char_p, [_v]),
     "vqhip_last_ranking": (C.c_char_p, [_v]),
     "vqhip_last_projection": (C.c_char_p, [_v]),

@@ -22,6 +22,29 @@ def _is_torch(x) -> bool:
     return type(x).__module__.startswith("torch")
 
 
+class _Dtypes:
+    """The element types of scores and tables, asked of torch only when a call needs them."""
+
+    def __iter__(self):
+        import torch
+
+        return iter((torch.float32, torch.bfloat16, torch.float16))
+
+    def __contains__(self, d):
+        return any(d == x for x in self)
+
+
+_DTYPES = _Dtypes()
+
+
+def _dtype(d) -> int:
+    """torch dtype -> vqhip_dtype"""
+    for code, x in enumerate(_DTYPES):
+        if d == x:
+            return code
+    raise ValueError(f"unsupported type {d}")
+
+
 class Context:
     """One GPU, one caller at a time (like `predict(&mut self)` in the reference)."""
 
@@ -296,6 +319,169 @@ class Context:
         stream = C.c_void_p(torch.cuda.current_stream(X.device).cuda_stream)
         self._chk(self._L.vqhip_project_device(self._h, C.c_void_p(X.data_ptr()), X.shape[0], int(which),
                                                C.c_void_p(Y_out.data_ptr()), stream))
+
+    # -- sampled codes and codebook lookup (device tensors, enqueued on torch's current stream; nothing is kept between calls)
+    def scores(self, X, out=None):
+        """vqhip_scores_device: -||x_i - w_j||^2 for every row of X and every prototype -> N x K float32 on X's GPU."""
+        import torch
+
+        self._check_torch(X)
+        if not self.K:
+            raise VqhipError(_lib.ERR_STATE, "no prototypes set (vqhip_set_prototypes)")
+        N = X.shape[0]
+        if out is None:
+            out = torch.empty((N, self.K), dtype=torch.float32, device=X.device)
+        else:
+            self._check_rows(out, "out", (N, self.K), (torch.float32,))
+        self._chk(self._L.vqhip_scores_device(self._h, X.data_ptr(), N, out.data_ptr(), self._ld(out), self._stream(X)))
+        return out
+
+    def sample(self, scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """vqhip_sample_device: one index per row of scores (N x V float32, bfloat16 or float16; rows may be strided), drawn from
+        softmax(scores / temperature) cut to top_k, top_p and min_p, with the given numbers u (N float32 in [0, 1))
+        -> (idx int32, prob float32).  Each parameter is a number or a CUDA tensor of N (float32; top_k int32)."""
+        import torch
+
+        N = self._check_rows(scores, "scores", (None, None), _DTYPES)
+        V = scores.shape[1]
+        how = self._sampling(N, u, temperature, top_k, top_p, min_p)
+        idx = torch.empty(N, dtype=torch.int32, device=scores.device)
+        prob = torch.empty(N, dtype=torch.float32, device=scores.device)
+        self._chk(self._L.vqhip_sample_device(self._h, scores.data_ptr(), _dtype(scores.dtype), N, V, self._ld(scores), C.byref(how), u.data_ptr(),
+                                              idx.data_ptr(), prob.data_ptr(), self._stream(scores)))
+        return idx, prob
+
+    def assign_sampled(self, X, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """vqhip_assign_sampled_device: assign with the winner drawn from softmax(-||x - w||^2 / temperature) instead of nearest
+        (temperature 0: the nearest) -> (idx int32, prob float32).  Equals sample(scores(X), u, ...)."""
+        import torch
+
+        self._check_torch(X)
+        N = X.shape[0]
+        how = self._sampling(N, u, temperature, top_k, top_p, min_p)
+        need = C.c_size_t(0)
+        self._chk(self._L.vqhip_assign_sampled_workspace(self._h, N, C.byref(need)))
+        work = torch.empty(need.value, dtype=torch.uint8, device=X.device)
+        idx = torch.empty(N, dtype=torch.int32, device=X.device)
+        prob = torch.empty(N, dtype=torch.float32, device=X.device)
+        self._chk(self._L.vqhip_assign_sampled_device(self._h, X.data_ptr(), N, C.byref(how), u.data_ptr(), idx.data_ptr(), prob.data_ptr(),
+                                                      work.data_ptr(), need.value, self._stream(X)))
+        return idx, prob
+
+    def lookup(self, idx, table=None, scale=1.0, out=None):
+        """vqhip_lookup_device: scale * table[idx] for a CUDA int32 tensor of any shape -> idx.shape + (D,) in the table's type.
+        table: K x D float32, bfloat16 or float16 (rows may be strided); None: the context's prototypes.  An index outside
+        [0, K), -1 for padding, gives zeros."""
+        import torch
+
+        N = self._check_index(idx)
+        if table is None:
+            if not self.K:
+                raise VqhipError(_lib.ERR_STATE, "no prototypes set (vqhip_set_prototypes)")
+            K, D, ldt, dtype, src = self.K, self.D, self.D, torch.float32, None
+        else:
+            K = self._check_rows(table, "table", (None, None), _DTYPES)
+            D, ldt, dtype, src = table.shape[1], self._ld(table), table.dtype, table.data_ptr()
+        if out is None:
+            out = torch.empty((*idx.shape, D), dtype=dtype, device=idx.device)
+            ldy = D
+        else:
+            rows = self._rows_of(out, "out", idx, D)
+            self._check_rows(rows, "out", (N, D), (dtype,))
+            ldy = self._ld(rows)
+        self._chk(self._L.vqhip_lookup_device(self._h, src, _dtype(dtype), K, D, ldt, idx.data_ptr(), N, scale, out.data_ptr(), ldy, self._stream(idx)))
+        return out
+
+    def lookup_gradient(self, grad, idx, K=None, scale=1.0, out=None, accumulate=False, out_dtype=None, want_counts=False):
+        """vqhip_lookup_gradient_device: the gradient of lookup(idx, table, scale) with respect to the table, given that of its
+        result (idx.shape + (D,), float32, bfloat16 or float16) -> K x D (default K: the context's prototypes) in float32 or
+        grad's type (out_dtype or out's; default float32).  accumulate adds to `out`.  want_counts: also how many indices name
+        each row (int32).  The sums are float32 in an order that depends on the inputs alone."""
+        import torch
+
+        N = self._check_index(idx)
+        if grad.dim() == 0:
+            raise ValueError("grad must have the indices' shape and one more dimension")
+        D = grad.shape[-1]
+        rows = self._rows_of(grad, "grad", idx, D)
+        self._check_rows(rows, "grad", (N, D), _DTYPES)
+        K = self.K if K is None else int(K)
+        if K < 1 or D < 1:
+            raise ValueError("the table must have at least one row and one column")
+        if out is None:
+            if accumulate:
+                raise ValueError("accumulate needs out")
+            out = torch.empty((K, D), dtype=out_dtype or torch.float32, device=idx.device)
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+        self._check_rows(out, "out", (K, D), (torch.float32, grad.dtype))
+        need = C.c_size_t(0)
+        self._chk(self._L.vqhip_lookup_gradient_workspace(self._h, N, K, D, C.byref(need)))
+        work = torch.empty(need.value, dtype=torch.uint8, device=idx.device)
+        counts = torch.empty(K, dtype=torch.int32, device=idx.device) if want_counts else None
+        self._chk(self._L.vqhip_lookup_gradient_device(self._h, rows.data_ptr(), _dtype(grad.dtype), self._ld(rows), idx.data_ptr(), N, scale, K, D,
+                                                       out.data_ptr(), _dtype(out.dtype), self._ld(out), bool(accumulate),
+                                                       counts.data_ptr() if want_counts else None, work.data_ptr(), need.value, self._stream(idx)))
+        return (out, counts) if want_counts else out
+
+    def _sampling(self, N, u, temperature, top_k, top_p, min_p):
+        """The vqhip_sampling of a call, and the checks of its device arrays."""
+        import torch
+
+        def column(v, name, dtype):
+            if not _is_torch(v):
+                return None
+            if not (v.is_cuda and v.device.index == self.device and v.dtype == dtype and v.is_contiguous() and tuple(v.shape) == (N,)):
+                raise ValueError(f"{name} must be a number or a contiguous CUDA {dtype} tensor of {N} values on cuda:{self.device}")
+            return v.data_ptr()
+
+        if not _is_torch(u) or column(u, "u", torch.float32) is None:
+            raise ValueError(f"u must be a contiguous CUDA torch.float32 tensor of {N} values on cuda:{self.device}")
+        t, k = column(temperature, "temperature", torch.float32), column(top_k, "top_k", torch.int32)
+        p, m = column(top_p, "top_p", torch.float32), column(min_p, "min_p", torch.float32)
+        if k is None and not 0 <= top_k < 1 << 32:
+            raise ValueError("top_k must not be negative")
+        return _lib.Sampling(1.0 if t else temperature, 1.0 if p else top_p, 0.0 if m else min_p, 0 if k else int(top_k), t, p, m, k)
+
+    @staticmethod
+    def _ld(t):
+        """Elements from one row of a matrix to the next (a single row has none: its width)."""
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    @staticmethod
+    def _stream(t):
+        import torch
+
+        return torch.cuda.current_stream(t.device).cuda_stream
+
+    @staticmethod
+    def _rows_of(t, name, idx, D):
+        """A tensor of shape idx.shape + (D,) as N rows."""
+        if tuple(t.shape) != (*idx.shape, D):
+            raise ValueError(f"{name} must be of shape {(*idx.shape, D)}")
+        if t.dim() == 2:
+            return t
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous unless it is a matrix")
+        return t.view(-1, D) if D else t.reshape(idx.numel(), 0)
+
+    def _check_index(self, idx):
+        import torch
+
+        if not (_is_torch(idx) and idx.is_cuda and idx.device.index == self.device and idx.dtype == torch.int32 and idx.is_contiguous()):
+            raise ValueError(f"idx must be a contiguous CUDA int32 tensor on cuda:{self.device}")
+        return idx.numel()
+
+    def _check_rows(self, t, name, shape, dtypes):
+        """A matrix on the context's GPU whose rows are contiguous and do not overlap -> its number of rows."""
+        if not (_is_torch(t) and t.is_cuda and t.device.index == self.device and t.dtype in dtypes and t.dim() == 2):
+            raise ValueError(f"{name} must be a matrix of {' or '.join(str(d) for d in dtypes)} on cuda:{self.device}")
+        for have, want in zip(t.shape, shape):
+            if want is not None and have != want:
+                raise ValueError(f"{name} must be {shape[0]} x {shape[1]}, not {tuple(t.shape)}")
+        if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"{name} must have contiguous rows that do not overlap")
+        return t.shape[0]
 
     def _assign_torch(self, X, y, want_dist):
         import torch

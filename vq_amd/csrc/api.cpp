@@ -1250,6 +1250,210 @@ try {
 }
 VQHIP_CATCH(c)
 
+// ---- sampled codes and codebook lookup ----------------------------------------------------------------------------------
+namespace {
+
+// Runs a call on the context's device and gives the thread its own back.
+class OnDevice {
+public:
+    explicit OnDevice(int device)
+    {
+        e_ = hipGetDevice(&old_);
+        if (e_ == hipSuccess && old_ != device) {
+            e_ = hipSetDevice(device);
+            moved_ = e_ == hipSuccess;
+        }
+    }
+    ~OnDevice()
+    {
+        if (moved_) (void)hipSetDevice(old_);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+    hipError_t error() const { return e_; }
+
+private:
+    hipError_t e_ = hipSuccess;
+    int old_ = 0;
+    bool moved_ = false;
+};
+
+size_t dtype_bytes(int dtype) { return dtype == VQHIP_F32 ? 4 : dtype == VQHIP_BF16 || dtype == VQHIP_F16 ? 2 : 0; }
+
+// Rows of `width` elements, `ld` apart, at p: aligned for the element type, and their byte offsets inside 63 bits
+const char *check_matrix(const void *p, uint64_t rows, uint64_t width, uint64_t ld, size_t elem)
+{
+    if (ld < width) return "a row stride is smaller than the row";
+    if ((uintptr_t)p & (elem - 1)) return "a matrix is not aligned for its type";
+    if (rows && ld > (uint64_t)INT64_MAX / elem / rows) return "a matrix is too large";
+    return nullptr;
+}
+
+int check_euclidean(vqhip_ctx *c, const char *call)
+{
+    if (c->K == 0) return c->fail(VQHIP_ERR_STATE, "no prototypes set (vqhip_set_prototypes)");
+    if (c->omega_kind != OMEGA_NONE) return c->fail(VQHIP_ERR_UNSUPPORTED, std::string(call) + " serves Euclidean models; clear Omega first");
+    return VQHIP_OK;
+}
+
+int check_sampling(vqhip_ctx *c, const vqhip_sampling *how)
+{
+    if (!how) return c->fail(VQHIP_ERR_INVALID, "sampling: how is NULL");
+    if (!how->dtemperature && !(how->temperature >= 0.0f && how->temperature < INFINITY))
+        return c->fail(VQHIP_ERR_INVALID, "sampling: temperature must be finite and not negative");
+    if (!how->dtop_p && !(how->top_p >= 0.0f && how->top_p <= 1.0f)) return c->fail(VQHIP_ERR_INVALID, "sampling: top_p must lie in [0, 1]");
+    if (!how->dmin_p && !(how->min_p >= 0.0f && how->min_p <= 1.0f)) return c->fail(VQHIP_ERR_INVALID, "sampling: min_p must lie in [0, 1]");
+    if (((uintptr_t)how->dtemperature | (uintptr_t)how->dtop_p | (uintptr_t)how->dmin_p | (uintptr_t)how->dtop_k) & 3)
+        return c->fail(VQHIP_ERR_INVALID, "sampling: device pointers must be 4-byte aligned");
+    return VQHIP_OK;
+}
+
+constexpr uint64_t SAMPLED_CHUNK_BYTES = 128ull << 20;      // scores of one chunk: half the last-level cache
+
+}  // namespace
+
+int vqhip_scores_device(vqhip_ctx *c, const float *dX, uint64_t N, float *dS, uint64_t lds, void *stream)
+try {
+    if (!c) return VQHIP_ERR_INVALID;
+    int rc = check_euclidean(c, "scores");
+    if (rc != VQHIP_OK) return rc;
+    if (N == 0) return VQHIP_OK;
+    if (!dX || !dS) return c->fail(VQHIP_ERR_INVALID, "scores_device: dX or dS is NULL");
+    if (const char *why = check_matrix(dX, N, c->D, c->D, 4)) return c->fail(VQHIP_ERR_INVALID, std::string("scores_device: ") + why);
+    if (const char *why = check_matrix(dS, N, c->K, lds, 4)) return c->fail(VQHIP_ERR_INVALID, std::string("scores_device: ") + why);
+    OnDevice on(c->device);
+    HIPCHK(c, on.error());
+    HIPCHK(c, launch_scores(dX, N, c->D, c->dW, c->K, dS, lds, (hipStream_t)stream));
+    return VQHIP_OK;
+}
+VQHIP_CATCH(c)
+
+int vqhip_sample_device(vqhip_ctx *c, const void *dS, int dtype, uint64_t N, uint32_t V, uint64_t lds, const vqhip_sampling *how, const float *du,
+                        uint32_t *didx_out, float *dprob_out, void *stream)
+try {
+    if (!c) return VQHIP_ERR_INVALID;
+    int rc = check_sampling(c, how);
+    if (rc != VQHIP_OK) return rc;
+    if (!dtype_bytes(dtype)) return c->fail(VQHIP_ERR_INVALID, "sample_device: unknown dtype");
+    if (V == 0 || V >= (1u << 31)) return c->fail(VQHIP_ERR_INVALID, "sample_device: V must lie in [1, 2^31)");
+    if (N == 0) return VQHIP_OK;
+    if (!dS || !du || !didx_out) return c->fail(VQHIP_ERR_INVALID, "sample_device: dS, du or didx_out is NULL");
+    if (const char *why = check_matrix(dS, N, V, lds, dtype_bytes(dtype))) return c->fail(VQHIP_ERR_INVALID, std::string("sample_device: ") + why);
+    if (((uintptr_t)du | (uintptr_t)didx_out | (uintptr_t)dprob_out) & 3) return c->fail(VQHIP_ERR_INVALID, "sample_device: device pointers must be 4-byte aligned");
+    OnDevice on(c->device);
+    HIPCHK(c, on.error());
+    HIPCHK(c, launch_sample(dS, dtype, N, V, lds, *how, du, didx_out, dprob_out, (hipStream_t)stream));
+    return VQHIP_OK;
+}
+VQHIP_CATCH(c)
+
+int vqhip_assign_sampled_workspace(vqhip_ctx *c, uint64_t N, size_t *bytes)
+try {
+    if (!c) return VQHIP_ERR_INVALID;
+    if (!bytes) return c->fail(VQHIP_ERR_INVALID, "assign_sampled_workspace: bytes is NULL");
+    int rc = check_euclidean(c, "assign_sampled");
+    if (rc != VQHIP_OK) return rc;
+    const uint64_t row = (uint64_t)c->K * 4;
+    *bytes = (size_t)(row * std::min<uint64_t>(std::max<uint64_t>(N, 1), std::max<uint64_t>(1, SAMPLED_CHUNK_BYTES / row)));
+    return VQHIP_OK;
+}
+VQHIP_CATCH(c)
+
+int vqhip_assign_sampled_device(vqhip_ctx *c, const float *dX, uint64_t N, const vqhip_sampling *how, const float *du, uint32_t *didx_out,
+                                float *dprob_out, void *dwork, size_t work_bytes, void *stream)
+try {
+    if (!c) return VQHIP_ERR_INVALID;
+    int rc = check_euclidean(c, "assign_sampled");
+    if (rc != VQHIP_OK || (rc = check_sampling(c, how)) != VQHIP_OK) return rc;
+    if (N == 0) return VQHIP_OK;
+    if (!dX || !du || !didx_out || !dwork) return c->fail(VQHIP_ERR_INVALID, "assign_sampled_device: dX, du, didx_out or dwork is NULL");
+    if (const char *why = check_matrix(dX, N, c->D, c->D, 4)) return c->fail(VQHIP_ERR_INVALID, std::string("assign_sampled_device: ") + why);
+    if (((uintptr_t)du | (uintptr_t)didx_out | (uintptr_t)dprob_out | (uintptr_t)dwork) & 3)
+        return c->fail(VQHIP_ERR_INVALID, "assign_sampled_device: device pointers must be 4-byte aligned");
+    const uint64_t chunk = work_bytes / ((uint64_t)c->K * 4);
+    if (chunk == 0) return c->fail(VQHIP_ERR_INVALID, "assign_sampled_device: the workspace holds no row of scores (K floats)");
+    OnDevice on(c->device);
+    HIPCHK(c, on.error());
+    const hipStream_t s = (hipStream_t)stream;
+    for (uint64_t off = 0; off < N; off += chunk) {
+        const uint64_t n = std::min(chunk, N - off);
+        vqhip_sampling h = *how;
+        if (h.dtemperature) h.dtemperature += off;
+        if (h.dtop_p) h.dtop_p += off;
+        if (h.dmin_p) h.dmin_p += off;
+        if (h.dtop_k) h.dtop_k += off;
+        HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->K, (float *)dwork, c->K, s));
+        HIPCHK(c, launch_sample(dwork, VQHIP_F32, n, c->K, c->K, h, du + off, didx_out + off, dprob_out ? dprob_out + off : nullptr, s));
+    }
+    return VQHIP_OK;
+}
+VQHIP_CATCH(c)
+
+int vqhip_lookup_device(vqhip_ctx *c, const void *dT, int dtype, uint32_t K, uint32_t D, uint64_t ldt, const uint32_t *didx, uint64_t N, float scale,
+                        void *dY, uint64_t ldy, void *stream)
+try {
+    if (!c) return VQHIP_ERR_INVALID;
+    if (!dtype_bytes(dtype)) return c->fail(VQHIP_ERR_INVALID, "lookup_device: unknown dtype");
+    if (K == 0 || K >= (1u << 31) || D == 0 || D > (1u << 24)) return c->fail(VQHIP_ERR_INVALID, "lookup_device: K must lie in [1, 2^31), D in [1, 2^24]");
+    if (!dT) {
+        if (c->K == 0) return c->fail(VQHIP_ERR_STATE, "no prototypes set (vqhip_set_prototypes)");
+        if (dtype != VQHIP_F32 || K != c->K || D != c->D || ldt != c->D)
+            return c->fail(VQHIP_ERR_INVALID, "lookup_device: the context's prototypes are K x D of f32, rows D apart");
+        dT = c->dW;
+    }
+    if (N == 0) return VQHIP_OK;
+    if (!didx || !dY) return c->fail(VQHIP_ERR_INVALID, "lookup_device: didx or dY is NULL");
+    if ((uintptr_t)didx & 3) return c->fail(VQHIP_ERR_INVALID, "lookup_device: didx must be 4-byte aligned");
+    if (const char *why = check_matrix(dT, K, D, ldt, dtype_bytes(dtype))) return c->fail(VQHIP_ERR_INVALID, std::string("lookup_device: table: ") + why);
+    if (const char *why = check_matrix(dY, N, D, ldy, dtype_bytes(dtype))) return c->fail(VQHIP_ERR_INVALID, std::string("lookup_device: result: ") + why);
+    OnDevice on(c->device);
+    HIPCHK(c, on.error());
+    HIPCHK(c, launch_lookup(dT, dtype, ldt, K, D, didx, N, scale, dY, ldy, (hipStream_t)stream));
+    return VQHIP_OK;
+}
+VQHIP_CATCH(c)
+
+static int check_gradient_shape(vqhip_ctx *c, uint64_t N, uint32_t K, uint32_t D)
+{
+    if (K == 0 || K >= (1u << 31) || D == 0 || D > (1u << 24)) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient: K must lie in [1, 2^31), D in [1, 2^24]");
+    if (N >= (1ull << 31)) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient: N must be below 2^31");
+    return VQHIP_OK;
+}
+
+int vqhip_lookup_gradient_workspace(vqhip_ctx *c, uint64_t N, uint32_t K, uint32_t D, size_t *bytes)
+try {
+    if (!c) return VQHIP_ERR_INVALID;
+    if (!bytes) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient_workspace: bytes is NULL");
+    const int rc = check_gradient_shape(c, N, K, D);
+    if (rc != VQHIP_OK) return rc;
+    *bytes = lookup_gradient_workspace(N, K, D);
+    return VQHIP_OK;
+}
+VQHIP_CATCH(c)
+
+int vqhip_lookup_gradient_device(vqhip_ctx *c, const void *dY, int dtype, uint64_t ldy, const uint32_t *didx, uint64_t N, float scale, uint32_t K,
+                                 uint32_t D, void *dT, int out_dtype, uint64_t ldt, int accumulate, uint32_t *dcounts, void *dwork, size_t work_bytes,
+                                 void *stream)
+try {
+    if (!c) return VQHIP_ERR_INVALID;
+    const int rc = check_gradient_shape(c, N, K, D);
+    if (rc != VQHIP_OK) return rc;
+    if (!dtype_bytes(dtype)) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient_device: unknown dtype");
+    if (out_dtype != VQHIP_F32 && out_dtype != dtype) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient_device: out_dtype must be VQHIP_F32 or the rows' dtype");
+    if (!dT || !dwork || (N && (!dY || !didx))) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient_device: dY, didx, dT or dwork is NULL");
+    if (((uintptr_t)didx | (uintptr_t)dcounts) & 3) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient_device: didx and dcounts must be 4-byte aligned");
+    if ((uintptr_t)dwork & 255) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient_device: dwork must be 256-byte aligned");
+    if (work_bytes < lookup_gradient_workspace(N, K, D))
+        return c->fail(VQHIP_ERR_INVALID, "lookup_gradient_device: the workspace is smaller than vqhip_lookup_gradient_workspace says");
+    if (const char *why = check_matrix(dY, N, D, ldy, dtype_bytes(dtype))) return c->fail(VQHIP_ERR_INVALID, std::string("lookup_gradient_device: rows: ") + why);
+    if (const char *why = check_matrix(dT, K, D, ldt, dtype_bytes(out_dtype))) return c->fail(VQHIP_ERR_INVALID, std::string("lookup_gradient_device: result: ") + why);
+    OnDevice on(c->device);
+    HIPCHK(c, on.error());
+    HIPCHK(c, launch_lookup_gradient(dY, dtype, ldy, didx, N, scale, K, D, dT, out_dtype, ldt, accumulate != 0, dcounts, dwork, (hipStream_t)stream));
+    return VQHIP_OK;
+}
+VQHIP_CATCH(c)
+
 int vqhip_synth_fill_device(vqhip_ctx *c, float *dout, uint64_t count, uint64_t first, uint64_t seed,
                             uint32_t stream_id, float scale, const float *dbase, uint64_t base_len, void *stream)
 try {

@@ -1,0 +1,33 @@
+// Device helpers shared by the kernels around sampled codes (kernels_sample.hip) and codebook lookup (kernels_lookup.hip):
+// the three element types of their matrices and loads / stores of 2, 4, 8 or 16 bytes of them.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "vq_common.h"
+
+namespace vq {
+
+// Elements are held in their own type and computed with in f32.  The one rounding to 16 bits is the conversion back, to
+// nearest even (a cast of __bf16 / _Float16 is).
+template <class T> __device__ __forceinline__ float widen(T v) { return (float)v; }
+template <class T> __device__ __forceinline__ T narrow(float v) { return (T)v; }
+
+// BYTES of consecutive elements, moved by one load or store (32: by two); the address is a multiple of BYTES, at most 16
+template <class T, int BYTES>
+struct alignas(BYTES > 16 ? 16 : BYTES) Pack {
+    static constexpr int E = BYTES / (int)sizeof(T);
+    T v[E];
+};
+
+// The widest of 16, 8, 4 bytes (or one element) that divides every given address, stride and row length in bytes: what one
+// lane may move at once.  Host side.
+inline int widest_access(size_t elem, uint64_t bits)
+{
+    for (int w : {16, 8, 4})
+        if ((size_t)w >= elem && (bits & (uint64_t)(w - 1)) == 0) return w;
+    return (int)elem;
+}
+
+}  // namespace vq

@@ -1,0 +1,628 @@
+// Codebook lookup and its gradient (vqhip_lookup_device, vqhip_lookup_gradient_device in include/vqhip.h).
+//
+//     lookup     Y[i] = scale * T[idx[i]]                               (a zero row where idx[i] is outside [0, K))
+//     gradient   G[k] (+)= scale * sum over { i : idx[i] = k } dY[i]    and how many rows each sum has
+//
+// The reference keeps its prototypes in a Vec and reads `prototypes[idx].vector` one sample at a time (src/glvq/glvq.rs:231
+// reads the name beside it); these are that read for a batch of indices and the transposed operation, which no part of the
+// reference has.
+//
+// The gradient is a scatter-add.  Atomic additions would make the order of the sums, and so their last bits, differ from run
+// to run, and they serialise on crowded rows.  Instead the rows are put in the order of their indices (a stable radix sort of
+// (index, row) pairs: 8 bytes per row against D values per row) and each run of equal indices is summed in that order, so the
+// same inputs give the same bits on every call:
+//     sort     k_sort_small (one workgroup, all in LDS) or k_sort_count / k_sort_scan / k_sort_move per digit
+//     reduce   k_grad_reduce: the sorted positions are cut into equal chunks whatever the runs are, so one crowded index
+//              costs no more than many rare ones.  A run inside one chunk is finished there; the parts of a run that crosses
+//              chunk borders go to the workspace in f32
+//     join     k_grad_join: adds up the parts of those runs in order, writes the rows no index names, and the counts
+#include <algorithm>
+
+#include "codes_device.h"
+
+namespace vq {
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------- lookup
+struct LookupArgs {
+    const void *T;
+    uint64_t ldt;
+    const uint32_t *idx;
+    uint64_t N;
+    uint32_t K, D;
+    float scale;
+    void *Y;
+    uint64_t ldy;
+    int log2g;              // 2^log2g lanes per row and column step
+};
+
+constexpr int LOOK_THREADS = 256;
+
+// 2^log2g lanes share a row; blockIdx.y picks the column step.  U rows are in flight per lane: index -> row -> store is a
+// chain of two memory latencies, and nothing else hides them.
+template <class T, int BYTES, int U>
+__global__ void __launch_bounds__(LOOK_THREADS) k_lookup(const LookupArgs a)
+{
+    using P = Pack<T, BYTES>;
+    const int g = 1 << a.log2g;
+    const uint32_t col = ((uint32_t)blockIdx.y * g + (threadIdx.x & (g - 1))) * P::E;
+    if (col >= a.D) return;
+    const uint32_t rows = LOOK_THREADS >> a.log2g;                   // rows of one step of the block
+    const T *table = (const T *)a.T + col;
+    T *out = (T *)a.Y + col;
+    for (uint64_t base = (uint64_t)blockIdx.x * rows * U + (threadIdx.x >> a.log2g); base < a.N; base += (uint64_t)gridDim.x * rows * U) {
+        uint32_t k[U];
+        P v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint64_t i = base + (uint64_t)u * rows;
+            k[u] = i < a.N ? a.idx[i] : a.K;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k[u] < a.K) {
+                v[u] = *(const P *)(table + (uint64_t)k[u] * a.ldt);
+            } else {
+#pragma unroll
+                for (int e = 0; e < P::E; ++e) v[u].v[e] = (T)0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint64_t i = base + (uint64_t)u * rows;
+            if (i >= a.N) break;
+            if (k[u] < a.K) {
+#pragma unroll
+                for (int e = 0; e < P::E; ++e) v[u].v[e] = narrow<T>(widen(v[u].v[e]) * a.scale);
+            }
+            *(P *)(out + i * a.ldy) = v[u];
+        }
+    }
+}
+
+template <class T, int BYTES>
+hipError_t run_lookup(LookupArgs a, hipStream_t s)
+{
+    const uint32_t steps = (a.D + BYTES / sizeof(T) - 1) / (uint32_t)(BYTES / sizeof(T));
+    a.log2g = 0;
+    while ((1u << a.log2g) < steps && a.log2g < 8) ++a.log2g;
+    const uint32_t cols = (steps + (1u << a.log2g) - 1) >> a.log2g;
+    const uint64_t rows = LOOK_THREADS >> a.log2g;
+    // four rows in flight per lane once that still leaves every CU several workgroups
+    const bool four = (a.N + 4 * rows - 1) / (4 * rows) * cols >= 2048;
+    const uint64_t per = four ? 4 * rows : rows;
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.N + per - 1) / per, 1u << 20);
+    if (four)
+        hipLaunchKernelGGL((k_lookup<T, BYTES, 4>), dim3(blocks, cols), dim3(LOOK_THREADS), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_lookup<T, BYTES, 1>), dim3(blocks, cols), dim3(LOOK_THREADS), 0, s, a);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------- sort
+// Stable: equal keys stay in the order of their rows.  A workgroup owns a tile of consecutive positions, a wave a consecutive
+// part of the tile, and takes 64 of them at a time, so (wave, step, lane) is the order of the positions.  The place of an
+// element among those with its digit: how many the waves before it hold (a table per wave, summed once), how many the steps
+// before it held (the table's running count), and how many lanes below it hold the same digit (a ballot per digit bit).
+constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_ITEMS = 16;
+constexpr uint32_t SORT_TILE = SORT_THREADS * SORT_ITEMS;
+constexpr int SORT_MAX_BITS = 11;                                   // bins of one pass: 2 bytes x 2048 x 8 waves of LDS
+constexpr uint32_t NONE = 0xFFFFFFFFu;
+
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits)
+{
+    uint64_t m = ~0ull;
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t v = __ballot((d >> b) & 1);
+        m &= (d >> b) & 1 ? v : ~v;
+    }
+    return m;
+}
+
+// Exclusive prefix sum over the n <= 2048 entries of `a` (LDS), by the whole workgroup of THREADS lanes.
+template <int THREADS>
+__device__ void scan_bins(uint32_t *a, uint32_t n, uint32_t *tmp)
+{
+    const uint32_t t = threadIdx.x, per = (n + THREADS - 1) / THREADS;
+    uint32_t sum = 0;
+    for (uint32_t j = 0; j < per; ++j)
+        if (t * per + j < n) sum += a[t * per + j];
+    uint32_t x = sum;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(x, o);
+        if ((int)(t & 63) >= o) x += y;
+    }
+    if ((t & 63) == 63) tmp[t >> 6] = x;
+    __syncthreads();
+    uint32_t before = x - sum;
+    for (uint32_t w = 0; w < t >> 6; ++w) before += tmp[w];
+    for (uint32_t j = 0; j < per; ++j)
+        if (t * per + j < n) {
+            const uint32_t v = a[t * per + j];
+            a[t * per + j] = before;
+            before += v;
+        }
+    __syncthreads();
+}
+
+struct SortArgs {
+    const uint32_t *idx;            // first pass: keys are min(idx, K), rows their positions; null later
+    const uint32_t *keys_in, *rows_in;
+    uint32_t *keys, *rows;          // result of the pass
+    uint32_t *hist;                 // [bins][tiles]
+    uint32_t *total;                // [bins]
+    uint32_t *start;                // K entries to set to NONE in the first pass
+    uint32_t N, K, tiles;
+    int shift, bits;
+};
+
+__device__ __forceinline__ uint32_t load_key(const SortArgs &a, uint32_t i)
+{
+    return a.idx ? min(a.idx[i], a.K) : a.keys_in[i];
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const SortArgs a)
+{
+    __shared__ uint32_t bins[1 << SORT_MAX_BITS];
+    const uint32_t nb = 1u << a.bits, tile = blockIdx.x;
+    for (uint32_t b = threadIdx.x; b < nb; b += SORT_THREADS) bins[b] = 0;
+    if (a.idx)
+        for (uint64_t k = (uint64_t)tile * SORT_THREADS + threadIdx.x; k < a.K; k += (uint64_t)gridDim.x * SORT_THREADS) a.start[k] = NONE;
+    __syncthreads();
+    const uint32_t base = tile * SORT_TILE, end = min(a.N - base, SORT_TILE);
+#pragma unroll 4
+    for (uint32_t j = threadIdx.x; j < end; j += SORT_THREADS) atomicAdd(&bins[(load_key(a, base + j) >> a.shift) & (nb - 1)], 1u);
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < nb; b += SORT_THREADS) a.hist[(size_t)b * a.tiles + tile] = bins[b];
+}
+
+// One workgroup per bin: exclusive prefix sum over the tiles, in place, and the bin's total.
+__global__ void __launch_bounds__(256) k_sort_scan(uint32_t *hist, uint32_t *total, uint32_t tiles)
+{
+    __shared__ uint32_t part[4];
+    uint32_t *h = hist + (size_t)blockIdx.x * tiles;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t carry = 0;
+    for (uint32_t base = 0; base < tiles; base += 256) {
+        const uint32_t i = base + threadIdx.x, v = i < tiles ? h[i] : 0;
+        uint32_t x = v;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 63) part[w] = x;
+        __syncthreads();
+        uint32_t before = carry + x - v;
+        for (int k = 0; k < w; ++k) before += part[k];
+        if (i < tiles) h[i] = before;
+        carry += part[0] + part[1] + part[2] + part[3];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) total[blockIdx.x] = carry;
+}
+
+// Ranks `ITEMS` elements per lane (held in registers, wave-consecutive) by their digit; on return rank[j] is the element's
+// place inside the tile and first[d] the first place of digit d.  `count`: WAVES tables of nb counters.
+template <int WAVES, int ITEMS>
+__device__ __forceinline__ void rank_tile(const uint32_t (&key)[ITEMS], uint32_t valid, int shift, int bits, uint16_t *count, uint32_t *first, uint32_t *tmp,
+                                          uint32_t (&rank)[ITEMS])
+{
+    const uint32_t nb = 1u << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (uint32_t b = threadIdx.x; b < nb * WAVES; b += WAVES * 64) count[b] = 0;
+    __syncthreads();
+    uint16_t *mine = count + w * nb;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+        const bool on = (w * ITEMS + j) * 64 + lane < valid;
+        const uint32_t d = on ? (key[j] >> shift) & (nb - 1) : nb;          // bit `bits` set: never equal to a digit of the tile
+        const uint64_t same = same_digit(d, bits + 1);
+        const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+        uint32_t had = 0;
+        if (on) had = mine[d];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");              // every lane has read before the first of them adds
+        if (on && below == 0) mine[d] = (uint16_t)(had + __popcll(same));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        rank[j] = had + below;
+    }
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < nb; b += WAVES * 64) {
+        uint32_t run = 0;
+        for (int k = 0; k < WAVES; ++k) {
+            const uint32_t c = count[k * nb + b];
+            count[k * nb + b] = (uint16_t)run;
+            run += c;
+        }
+        first[b] = run;
+    }
+    __syncthreads();
+    scan_bins<WAVES * 64>(first, nb, tmp);
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+        if ((w * ITEMS + j) * 64 + lane < valid) {
+            const uint32_t d = (key[j] >> shift) & (nb - 1);
+            rank[j] += first[d] + mine[d];
+        }
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs a)
+{
+    __shared__ uint32_t lkey[SORT_TILE], lrow[SORT_TILE];                   // 64 KiB
+    __shared__ uint16_t count[SORT_WAVES << SORT_MAX_BITS];                 // 32 KiB
+    __shared__ uint32_t first[1 << SORT_MAX_BITS], base[1 << SORT_MAX_BITS], tmp[SORT_WAVES];
+    const uint32_t nb = 1u << a.bits, tile = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint32_t begin = tile * SORT_TILE, valid = min(a.N - begin, SORT_TILE);
+    uint32_t key[SORT_ITEMS], row[SORT_ITEMS], rank[SORT_ITEMS];
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; ++j) {
+        const uint32_t p = (w * SORT_ITEMS + j) * 64 + lane;
+        key[j] = p < valid ? load_key(a, begin + p) : 0;
+        row[j] = p < valid ? (a.idx ? begin + p : a.rows_in[begin + p]) : 0;
+    }
+    for (uint32_t b = threadIdx.x; b < nb; b += SORT_THREADS) base[b] = a.total[b];
+    __syncthreads();
+    scan_bins<SORT_THREADS>(base, nb, tmp);
+    rank_tile<SORT_WAVES, SORT_ITEMS>(key, valid, a.shift, a.bits, count, first, tmp, rank);
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; ++j)
+        if ((w * SORT_ITEMS + j) * 64 + lane < valid) {
+            lkey[rank[j]] = key[j];
+            lrow[rank[j]] = row[j];
+        }
+    __syncthreads();
+    // through LDS in the order of the places, so that the elements of a digit leave as one consecutive piece
+    for (uint32_t p = threadIdx.x; p < valid; p += SORT_THREADS) {
+        const uint32_t k = lkey[p], d = (k >> a.shift) & (nb - 1);
+        const uint32_t to = base[d] + a.hist[(size_t)d * a.tiles + tile] + (p - first[d]);
+        a.keys[to] = k;
+        a.rows[to] = lrow[p];
+    }
+}
+
+// All passes in one workgroup and one launch, for at most SMALL_TILE rows.
+constexpr int SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64, SMALL_ITEMS = 8;
+constexpr uint32_t SMALL_TILE = SMALL_THREADS * SMALL_ITEMS;
+constexpr int SMALL_MAX_BITS = 9;
+
+__global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(const SortArgs a, int key_bits)
+{
+    __shared__ uint32_t lkey[SMALL_TILE], lrow[SMALL_TILE];                 // 64 KiB
+    __shared__ uint16_t count[SMALL_WAVES << SMALL_MAX_BITS];               // 16 KiB
+    __shared__ uint32_t first[1 << SMALL_MAX_BITS], tmp[SMALL_WAVES];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    if (blockIdx.x != 0) {                                                  // the other workgroups only set `start`
+        for (uint64_t k = (uint64_t)(blockIdx.x - 1) * SMALL_THREADS + threadIdx.x; k < a.K; k += (uint64_t)(gridDim.x - 1) * SMALL_THREADS) a.start[k] = NONE;
+        return;
+    }
+    uint32_t key[SMALL_ITEMS], row[SMALL_ITEMS], rank[SMALL_ITEMS];
+#pragma unroll
+    for (int j = 0; j < SMALL_ITEMS; ++j) {
+        const uint32_t p = (w * SMALL_ITEMS + j) * 64 + lane;
+        key[j] = p < a.N ? load_key(a, p) : 0;
+        row[j] = p;
+    }
+    const int passes = (key_bits + SMALL_MAX_BITS - 1) / SMALL_MAX_BITS, bits = (key_bits + passes - 1) / passes;
+    for (int pass = 0; pass < passes; ++pass) {
+        rank_tile<SMALL_WAVES, SMALL_ITEMS>(key, a.N, pass * bits, bits, count, first, tmp, rank);
+#pragma unroll
+        for (int j = 0; j < SMALL_ITEMS; ++j)
+            if ((w * SMALL_ITEMS + j) * 64 + lane < a.N) {
+                lkey[rank[j]] = key[j];
+                lrow[rank[j]] = row[j];
+            }
+        __syncthreads();
+        if (pass + 1 < passes) {
+#pragma unroll
+            for (int j = 0; j < SMALL_ITEMS; ++j) {
+                const uint32_t p = (w * SMALL_ITEMS + j) * 64 + lane;
+                if (p < a.N) {
+                    key[j] = lkey[p];
+                    row[j] = lrow[p];
+                }
+            }
+            __syncthreads();
+        }
+    }
+    for (uint32_t p = threadIdx.x; p < a.N; p += SMALL_THREADS) {
+        a.keys[p] = lkey[p];
+        a.rows[p] = lrow[p];
+    }
+}
+
+__global__ void k_fill_u32(uint32_t *p, uint64_t n, uint32_t v)
+{
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (uint64_t)gridDim.x * blockDim.x) p[i] = v;
+}
+
+// ---------------------------------------------------------------------------------------------- reduce and join
+struct GradArgs {
+    const void *dY;
+    uint64_t ldy;
+    const uint32_t *keys, *rows;    // sorted
+    uint32_t N, K, D;
+    float scale;
+    void *G;
+    uint64_t ldg;
+    int accumulate;
+    uint32_t *start, *end;          // K each: first place and place behind the last of every index that occurs
+    uint32_t *counts;               // nullable
+    float *parts;                   // [chunks][2][dpad]: head (a run that began in an earlier chunk), tail (one that goes on)
+    uint32_t dpad, chunk, chunks, slabs;
+    int log2g;
+};
+
+constexpr int GRAD_THREADS = 256;
+constexpr int GRAD_FLIGHT = 8;      // rows a lane has in flight
+
+// One finished row piece: G (+)= scale * sum, rounded once.
+template <class TO, int E>
+__device__ __forceinline__ void store_grad(const GradArgs &a, uint32_t k, uint32_t col, const float (&acc)[E])
+{
+    TO *g = (TO *)a.G + (uint64_t)k * a.ldg + col;
+    Pack<TO, E * (int)sizeof(TO)> o;
+    if (a.accumulate) {
+        o = *(const Pack<TO, E * (int)sizeof(TO)> *)g;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = narrow<TO>(fmaf(acc[e], a.scale, widen(o.v[e])));
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = narrow<TO>(acc[e] * a.scale);
+    }
+    *(Pack<TO, E * (int)sizeof(TO)> *)g = o;
+}
+
+// 2^log2g lanes own one chunk of sorted places and E * 2^log2g columns of it.
+template <class T, class TO, int E>
+__global__ void __launch_bounds__(GRAD_THREADS) k_grad_reduce(const GradArgs a)
+{
+    const uint64_t group = ((uint64_t)blockIdx.x * GRAD_THREADS + threadIdx.x) >> a.log2g;
+    const uint32_t c = (uint32_t)(group / a.slabs), slab = (uint32_t)(group % a.slabs);
+    if (c >= a.chunks) return;
+    const uint32_t gl = threadIdx.x & ((1u << a.log2g) - 1);
+    const uint32_t col = ((slab << a.log2g) + gl) * E;
+    const bool mine = col < a.D, first = slab == 0 && gl == 0;
+    const uint32_t p0 = c * a.chunk, p1 = min(a.N, p0 + a.chunk);
+    const T *dY = (const T *)a.dY + (mine ? col : 0);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    uint32_t cur = a.keys[p0], from = p0;
+    const bool left = p0 > 0 && a.keys[p0 - 1] == cur;            // the first run began in an earlier chunk
+    const uint32_t behind = p1 < a.N ? a.keys[p1] : NONE;
+
+    auto flush = [&](uint32_t upto) {                              // the run [from, upto) of index cur ends here
+        if (cur >= a.K) return;                                    // the rows without a place in the table
+        const bool l = from == p0 && left, r = upto == p1 && behind == cur;
+        if (first) {
+            if (!l) a.start[cur] = from;
+            if (!r) a.end[cur] = upto;
+        }
+        if (!mine) return;
+        if (!l && !r) {
+            store_grad<TO, E>(a, cur, col, acc);
+        } else {
+            float *part = a.parts + ((size_t)c * 2 + (l ? 0 : 1)) * a.dpad + col;
+#pragma unroll
+            for (int e = 0; e < E; ++e) part[e] = acc[e];
+        }
+    };
+
+    for (uint32_t p = p0; p < p1; p += GRAD_FLIGHT) {
+        uint32_t key[GRAD_FLIGHT], row[GRAD_FLIGHT];
+        Pack<T, E * (int)sizeof(T)> v[GRAD_FLIGHT];
+#pragma unroll
+        for (int j = 0; j < GRAD_FLIGHT; ++j) {
+            const uint32_t q = min(p + j, p1 - 1);
+            key[j] = a.keys[q];
+            row[j] = a.rows[q];
+        }
+        if (key[0] >= a.K) {                                       // sorted: nothing but rows without a place from here on
+            flush(p);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < GRAD_FLIGHT; ++j) v[j] = *(const Pack<T, E * (int)sizeof(T)> *)(dY + (uint64_t)row[j] * a.ldy);
+#pragma unroll
+        for (int j = 0; j < GRAD_FLIGHT; ++j) {
+            if (p + j < p1) {
+                if (key[j] != cur) {
+                    flush(p + j);
+                    cur = key[j];
+                    from = p + j;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += widen(v[j].v[e]);
+            }
+        }
+    }
+    flush(p1);
+}
+
+// Blocks [0, chunks * slabs): the run that begins in the chunk and goes on behind it, if there is one: its parts summed in a
+// fixed order (each group of lanes a consecutive share of them, the shares in order).  The other blocks: rows no index names,
+// and the counts.
+template <class TO, int E>
+__global__ void __launch_bounds__(GRAD_THREADS) k_grad_join(const GradArgs a, uint32_t join_blocks)
+{
+    __shared__ float share[GRAD_THREADS * E];
+    const uint32_t gsize = 1u << a.log2g, gl = threadIdx.x & (gsize - 1), gi = threadIdx.x >> a.log2g, groups = GRAD_THREADS >> a.log2g;
+    if (blockIdx.x < join_blocks) {
+        const uint32_t c = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
+        const uint32_t p1 = min(a.N, c * a.chunk + a.chunk);
+        if (p1 >= a.N) return;
+        const uint32_t k = a.keys[p1 - 1];
+        if (k >= a.K || a.keys[p1] != k || a.start[k] < c * a.chunk) return;
+        const uint32_t more = (a.end[k] - 1) / a.chunk - c;                        // chunks behind this one that the run reaches
+        const uint32_t col = (slab * gsize + gl) * E;
+        const bool mine = col < a.D;
+        const uint32_t per = (more + groups - 1) / groups;
+        float acc[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+        if (mine) {
+            const uint32_t lo = gi * per, hi = min(more, lo + per);
+#pragma unroll 8
+            for (uint32_t j = lo; j < hi; ++j) {
+                const float *part = a.parts + (size_t)(c + 1 + j) * 2 * a.dpad + col;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += part[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) share[(gi * gsize + gl) * E + e] = acc[e];
+        __syncthreads();
+        if (gi != 0 || !mine) return;
+        const float *tail = a.parts + ((size_t)c * 2 + 1) * a.dpad + col;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = tail[e];
+        for (uint32_t g = 0; g < groups && g * per < more; ++g)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += share[(g * gsize + gl) * E + e];
+        store_grad<TO, E>(a, k, col, acc);
+        return;
+    }
+    const uint64_t lanes = (uint64_t)(gridDim.x - join_blocks) * groups;
+    for (uint64_t k = (uint64_t)(blockIdx.x - join_blocks) * groups + gi; k < a.K; k += lanes) {
+        const uint32_t s = a.start[k];
+        if (a.counts && gl == 0) a.counts[k] = s == NONE ? 0 : a.end[k] - s;
+        if (s != NONE || a.accumulate) continue;
+        Pack<TO, E * (int)sizeof(TO)> zero;
+#pragma unroll
+        for (int e = 0; e < E; ++e) zero.v[e] = (TO)0.0f;
+        for (uint32_t col = gl * E; col < a.D; col += gsize * E) *(Pack<TO, E * (int)sizeof(TO)> *)((TO *)a.G + k * a.ldg + col) = zero;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- plan of one gradient call
+struct GradPlan {
+    uint32_t tiles, chunk, chunks, dpad;
+    int key_bits, passes, bits;
+    bool small;
+    size_t keys[2], rows[2], hist, total, start, end, parts, bytes;      // offsets into the workspace
+};
+
+GradPlan plan_gradient(uint64_t N, uint32_t K, uint32_t D)
+{
+    GradPlan p{};
+    p.small = N <= SMALL_TILE;
+    p.key_bits = 32 - __builtin_clz(K);                                   // indices 0 .. K - 1, and K for the rows without a place
+    p.passes = (p.key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
+    p.bits = (p.key_bits + p.passes - 1) / p.passes;
+    p.tiles = (uint32_t)((N + SORT_TILE - 1) / SORT_TILE);
+    // chunks: enough groups of lanes to fill the card (8192 waves) however the runs lie, at least 8 rows each, so that the
+    // parts of runs that cross chunk borders stay a small share of the rows read
+    const uint64_t units = N * ((D + 255) / 256);
+    p.chunk = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((units + 8191) / 8192, 8), 4096);
+    p.chunks = (uint32_t)((N + p.chunk - 1) / p.chunk);
+    p.dpad = (D + 7) / 8 * 8;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at += (bytes + 255) / 256 * 256;
+        return o;
+    };
+    for (int j = 0; j < 2; ++j) {
+        const bool used = j == 0 || (!p.small && p.passes > 1);
+        p.keys[j] = take(used ? N * 4 : 0);
+        p.rows[j] = take(used ? N * 4 : 0);
+    }
+    p.hist = take(p.small ? 0 : ((size_t)p.tiles << p.bits) * 4);
+    p.total = take(p.small ? 0 : (size_t)4 << p.bits);
+    p.start = take((size_t)K * 4);
+    p.end = take((size_t)K * 4);
+    p.parts = take((size_t)p.chunks * 2 * p.dpad * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <class T, class TO, int E>
+hipError_t run_reduce(GradArgs a, hipStream_t s)
+{
+    const uint32_t steps = (a.D + E - 1) / E;
+    a.log2g = 0;
+    while ((1u << a.log2g) < steps && a.log2g < 6) ++a.log2g;
+    a.slabs = (steps + (1u << a.log2g) - 1) >> a.log2g;
+    const uint32_t groups = GRAD_THREADS >> a.log2g;
+    if (a.N) {
+        const uint64_t blocks = ((uint64_t)a.chunks * a.slabs + groups - 1) / groups;
+        hipLaunchKernelGGL((k_grad_reduce<T, TO, E>), dim3((uint32_t)blocks), dim3(GRAD_THREADS), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    const uint32_t join_blocks = a.N ? a.chunks * a.slabs : 0;
+    const uint32_t fill_blocks = std::min<uint32_t>((a.K + groups - 1) / groups, 8192);
+    hipLaunchKernelGGL((k_grad_join<TO, E>), dim3(join_blocks + fill_blocks), dim3(GRAD_THREADS), 0, s, a, join_blocks);
+    return hipGetLastError();
+}
+
+template <class T, class TO>
+hipError_t run_reduce_width(const GradArgs &a, int e, hipStream_t s)
+{
+    if (e >= 8 && sizeof(T) == 2) return run_reduce<T, TO, sizeof(T) == 2 ? 8 : 4>(a, s);
+    if (e >= 4) return run_reduce<T, TO, 4>(a, s);
+    if (e >= 2) return run_reduce<T, TO, 2>(a, s);
+    return run_reduce<T, TO, 1>(a, s);
+}
+
+size_t elem_bytes(int dtype) { return dtype == VQHIP_F32 ? 4 : 2; }
+
+}  // namespace
+
+hipError_t launch_lookup(const void *dT, int dtype, uint64_t ldt, uint32_t K, uint32_t D, const uint32_t *didx, uint64_t N, float scale, void *dY,
+                         uint64_t ldy, hipStream_t s)
+{
+    const size_t b = elem_bytes(dtype);
+    const LookupArgs a{dT, ldt, didx, N, K, D, scale, dY, ldy, 0};
+    const int w = widest_access(b, (uint64_t)(uintptr_t)dT | (uint64_t)(uintptr_t)dY | ldt * b | ldy * b | (uint64_t)D * b);
+    if (dtype == VQHIP_F32)
+        return w == 16 ? run_lookup<float, 16>(a, s) : w == 8 ? run_lookup<float, 8>(a, s) : run_lookup<float, 4>(a, s);
+    if (dtype == VQHIP_BF16)
+        return w == 16 ? run_lookup<__bf16, 16>(a, s) : w == 8 ? run_lookup<__bf16, 8>(a, s) : w == 4 ? run_lookup<__bf16, 4>(a, s) : run_lookup<__bf16, 2>(a, s);
+    return w == 16 ? run_lookup<_Float16, 16>(a, s) : w == 8 ? run_lookup<_Float16, 8>(a, s) : w == 4 ? run_lookup<_Float16, 4>(a, s) : run_lookup<_Float16, 2>(a, s);
+}
+
+size_t lookup_gradient_workspace(uint64_t N, uint32_t K, uint32_t D) { return plan_gradient(N, K, D).bytes; }
+
+hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const uint32_t *didx, uint64_t N, float scale, uint32_t K, uint32_t D, void *dT,
+                                  int out_dtype, uint64_t ldt, bool accumulate, uint32_t *dcounts, void *dwork, hipStream_t s)
+{
+    const GradPlan p = plan_gradient(N, K, D);
+    char *w = (char *)dwork;
+    auto at = [&](size_t o) { return (uint32_t *)(w + o); };
+    SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), (uint32_t)N, K, p.tiles, 0, p.bits};
+    if (N == 0) {
+        hipLaunchKernelGGL(k_fill_u32, dim3(std::min<uint32_t>((K + 255) / 256, 4096)), dim3(256), 0, s, q.start, (uint64_t)K, NONE);
+    } else if (p.small) {
+        const uint32_t fill = std::min<uint32_t>((K + SMALL_THREADS - 1) / SMALL_THREADS, 256);
+        hipLaunchKernelGGL(k_sort_small, dim3(1 + fill), dim3(SMALL_THREADS), 0, s, q, p.key_bits);
+    } else {
+        for (int pass = 0; pass < p.passes; ++pass) {
+            const int to = (p.passes - 1 - pass) & 1;                       // the last pass ends in buffer 0
+            q.idx = pass == 0 ? didx : nullptr;
+            q.keys_in = at(p.keys[to ^ 1]);
+            q.rows_in = at(p.rows[to ^ 1]);
+            q.keys = at(p.keys[to]);
+            q.rows = at(p.rows[to]);
+            q.shift = pass * p.bits;
+            hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(SORT_THREADS), 0, s, q);
+            hipLaunchKernelGGL(k_sort_scan, dim3(1u << p.bits), dim3(256), 0, s, q.hist, q.total, p.tiles);
+            hipLaunchKernelGGL(k_sort_move, dim3(p.tiles), dim3(SORT_THREADS), 0, s, q);
+        }
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const GradArgs a{dG, ldg, at(p.keys[0]), at(p.rows[0]), (uint32_t)N, K, D, scale, dT, ldt, accumulate ? 1 : 0, at(p.start), at(p.end), dcounts,
+                     (float *)(w + p.parts), p.dpad, p.chunk, p.chunks, 0, 0};
+    // elements a lane takes at once: what 16 bytes of the rows hold, if rows, table and strides are aligned for it
+    const size_t bi = elem_bytes(dtype), bo = elem_bytes(out_dtype);
+    const int wi = widest_access(bi, (uint64_t)(uintptr_t)dG | ldg * bi | (uint64_t)D * bi);
+    const int wo = widest_access(bo, (uint64_t)(uintptr_t)dT | ldt * bo | (uint64_t)D * bo);
+    const int n = std::min(wi / (int)bi, wo >= 16 ? 16 : wo / (int)bo);
+    if (dtype == VQHIP_F32) return run_reduce_width<float, float>(a, n, s);
+    if (dtype == VQHIP_BF16) return out_dtype == VQHIP_F32 ? run_reduce_width<__bf16, float>(a, n, s) : run_reduce_width<__bf16, __bf16>(a, n, s);
+    return out_dtype == VQHIP_F32 ? run_reduce_width<_Float16, float>(a, n, s) : run_reduce_width<_Float16, _Float16>(a, n, s);
+}
+
+}  // namespace vq

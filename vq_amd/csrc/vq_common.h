@@ -119,6 +119,19 @@ hipError_t launch_glvq_gradient(const float *dX, uint64_t N, uint32_t D, uint32_
                                 const uint32_t *jn, const float *dn, float *scratch, float *dG, bool accumulate, double *dcost,
                                 unsigned long long *dused, hipStream_t s);
 
+// ---------------------------------------------------------------- sampled codes and codebook lookup
+// kernels_scores.hip: S[i][j] = - sum_d (X[i][d] - W[j][d])^2, rows of S `ld` apart
+hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, uint32_t K, float *dS, uint64_t ld, hipStream_t s);
+// kernels_sample.hip: one index per row of scores (include/vqhip.h vqhip_sample_device); dprob nullable
+hipError_t launch_sample(const void *dS, int dtype, uint64_t N, uint32_t V, uint64_t ld, const vqhip_sampling &how, const float *du,
+                         uint32_t *didx, float *dprob, hipStream_t s);
+// kernels_lookup.hip: Y[i] = scale T[idx[i]]; and its gradient over indices put in order (workspace: lookup_gradient_workspace bytes)
+hipError_t launch_lookup(const void *dT, int dtype, uint64_t ldt, uint32_t K, uint32_t D, const uint32_t *didx, uint64_t N, float scale,
+                         void *dY, uint64_t ldy, hipStream_t s);
+size_t lookup_gradient_workspace(uint64_t N, uint32_t K, uint32_t D);
+hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const uint32_t *didx, uint64_t N, float scale, uint32_t K, uint32_t D,
+                                  void *dT, int out_dtype, uint64_t ldt, bool accumulate, uint32_t *dcounts, void *dwork, hipStream_t s);
+
 // ---------------------------------------------------------------- synth (synth.hip)
 hipError_t launch_synth_fill(float *dout, uint64_t count, uint64_t first, uint64_t seed, uint32_t stream_id,
                              float scale, const float *dbase, uint64_t base_len, hipStream_t s);
