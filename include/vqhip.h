@@ -268,8 +268,9 @@ typedef enum { VQHIP_F32 = 0, VQHIP_BF16 = 1, VQHIP_F16 = 2 } vqhip_dtype;
 
 /* Scores of N samples against the context's prototypes: S[i][j] = - sum_d (x[i][d] - w[j][d])^2 (src/helpers.rs:18-20
  * without the root), N x K, rows lds apart.  Euclidean models only (VQHIP_ERR_UNSUPPORTED with an Omega).  A softmax of
- * S / T is the distribution over codes that vqhip_assign_sampled_device draws from.  Direct form in f32: a sample equal to a
- * prototype scores 0 exactly. */
+ * S / T is the distribution over codes that vqhip_assign_sampled_device draws from.  f32, in the direct form or, for rows of
+ * more than 32 values, on the matrix cores as |x - c|^2 + |w - c|^2 - 2 (x - c).(w - c) with c the mean prototype; distances
+ * small beside those norms are measured in the direct form there too, so a sample equal to a prototype scores 0 exactly. */
 int vqhip_scores_device(vqhip_ctx *ctx, const float *dX, uint64_t N, float *dS, uint64_t lds, void *stream);
 
 /* How to draw: one value for all rows, or, where the pointer is not NULL, one per row (N values on the device).

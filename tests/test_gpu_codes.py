@@ -2,7 +2,7 @@
 vqhip_lookup_gradient_device against their definitions in 64 bits (tests/codes_reference.py).
 
 Tolerances, derived before the first run (a rounding to f32 is off by at most 2^-24, to bf16 by 2^-8 ... relative):
-  scores    every difference x - w rounds once (2^-24), its square and the running sum add a rounding per value: at most
+  scores    (up to 32 values; longer rows have a bound of their own below) every difference x - w rounds once (2^-24), its square and the running sum add a rounding per value: at most
             (D + 3) 2^-24 of the sum (all terms have one sign)
   sample    idx equal; prob one rounding of an f64 value: 2^-24, and 1e-9 for the f64 sums
   lookup    f32 product rounded once, then once to the type: 2^-24 (f32) or 2^-24 + eps/2
@@ -38,8 +38,7 @@ def wide(t):
 
 
 # ---------------------------------------------------------------------------------------------- scores
-@pytest.mark.parametrize("N,D,K", [(150, 4, 3), (1, 1, 1), (7, 5, 2), (130, 16, 129), (257, 17, 300), (64, 128, 256), (33, 784, 100),
-                                   (129, 255, 127), (1000, 2, 1), (2, 1000, 513)])
+@pytest.mark.parametrize("N,D,K", [(150, 4, 3), (1, 1, 1), (7, 5, 2), (130, 16, 129), (257, 17, 300), (1000, 2, 1), (2, 32, 513)])
 def test_scores(ctx, N, D, K):
     g = gen(N + D)
     W = torch.rand(K, D, generator=g) * 2 - 1
@@ -518,3 +517,56 @@ def test_c_refusals(ctx):
         assert L.vqhip_lookup_gradient_device(h, *{**ok, **change}.values()) == bad, change
     assert L.vqhip_lookup_gradient_device(h, *ok.values()) == 0
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------------------- scores on the matrix cores
+@pytest.mark.parametrize("N,D,K", [(1, 33, 1), (64, 128, 256), (33, 784, 100), (129, 255, 127), (2, 1000, 513), (130, 64, 129), (65, 100, 70), (300, 128, 256), (20, 785, 33), (4100, 40, 2100), (2048, 36, 4096)])
+@pytest.mark.parametrize("offset", [0.0, 100.0])
+def test_scores_in_the_expanded_form(ctx, N, D, K, offset):
+    """Rows of more than 32 values: distances not below 1/8 of B = |x - c|^2 + |w - c|^2 come from B - 2 (x - c).(w - c).  Its
+    roundings, with e = 2^-24: each centred value 1 e of itself, which moves the distance by at most 2 sqrt(dist) e (|x - c| + |w - c|)
+    <= 4 e B; each norm a sum of D squares, D e of itself, together D e B; the product a chain of D terms whose absolute
+    values sum to at most B / 2, doubled D e B; the two last additions 2 e B.  (2 D + 6) e B <= 8 (2 D + 6) e dist."""
+    g = gen(N + D)
+    W = torch.rand(K, D, generator=g) * 2 - 1 + offset
+    X = W[torch.randint(K, (N,), generator=g)] + 0.1 * torch.randn(N, D, generator=g)
+    X[:: 3] = torch.rand(len(X[:: 3]), D, generator=g) * 4 - 2 + offset
+    X[0] = W[K - 1]
+    ctx.set_prototypes(W.numpy())
+    S = wide(ctx.scores(X.cuda()))
+    want = -torch.cdist(X.double(), W.double(), compute_mode="donot_use_mm_for_euclid_dist").square().numpy()
+    assert (np.abs(S - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want) + 1e-300).all()
+    assert S[0, K - 1] == 0.0
+
+
+@pytest.mark.parametrize("N", [70, 9000])
+@pytest.mark.parametrize("crowd", [1, 2, 64])
+def test_scores_of_crowded_prototypes(ctx, N, crowd):
+    """Prototypes in `crowd` tight groups, a group's samples among them: from a few close pairs a tile to nothing else.  Close
+    pairs are measured in the direct form: (D + 3) e of the distance; the others as above."""
+    D, K = 48, 900
+    g = gen(crowd)
+    centre = torch.randn(crowd, D, generator=g)
+    W = centre[torch.arange(K) % crowd] + 1e-3 * torch.randn(K, D, generator=g)
+    X = centre[torch.randint(crowd, (N,), generator=g)] + 1e-3 * torch.randn(N, D, generator=g)
+    ctx.set_prototypes(W.numpy())
+    buf = torch.full((N, K + 5), 3.0, device="cuda")
+    S = wide(ctx.scores(X.cuda(), out=buf[:, 2:K + 2]))
+    want = -torch.cdist(X.double(), W.double(), compute_mode="donot_use_mm_for_euclid_dist").square().numpy()
+    assert (np.abs(S - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want)).all()
+    assert (buf[:, :2] == 3).all() and (buf[:, K + 2:] == 3).all()
+
+
+def test_scores_of_long_rows_that_are_not_finite(ctx):
+    W = torch.randn(70, 40)
+    W[3, 5], W[4, 6], W[5, 7] = INF, NAN, 3e38
+    X = torch.randn(80, 40)
+    X[0, 0], X[1, 1], X[2, 2], X[3, 5] = INF, NAN, 1e30, INF
+    ctx.set_prototypes(W.numpy())
+    S = wide(ctx.scores(X.cuda()))
+    with np.errstate(over="ignore", invalid="ignore"):
+        d = (X.numpy()[:, None, :] - W.numpy()[None]).astype(np.float32)
+        want = -(d * d).sum(2).astype(np.float64)
+    bad = ~np.isfinite(want)
+    assert (np.isnan(S) == np.isnan(want)).all() and (S[bad & ~np.isnan(want)] == want[bad & ~np.isnan(want)]).all()
+    assert np.isfinite(S[~bad]).all()

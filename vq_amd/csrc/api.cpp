@@ -75,7 +75,7 @@ struct vqhip_ctx {
     std::vector<float> hW, hOm;
     std::vector<uint32_t> hcls;
 
-    float *dW = nullptr;       // K x D
+    float *dW = nullptr;       // K x D, and one row more: their mean
     double *dW64 = nullptr;    // K x D in the reference's own number type (f64 entry points only)
     uint32_t *dcls = nullptr;  // K
     float *dOm = nullptr;      // M x D  or  K x M x D
@@ -922,7 +922,16 @@ try {
     c->hW.assign(W, W + (size_t)K * D);
     c->K = K;
     c->D = D;
-    return upload(c, &c->dW, W, (size_t)K * D);
+    // their mean behind them: what vqhip_scores_device measures from (0 where it is not finite)
+    std::vector<double> sum(D, 0.0);
+    for (uint32_t k = 0; k < K; ++k)
+        for (uint32_t d = 0; d < D; ++d) sum[d] += (double)W[(size_t)k * D + d];
+    std::vector<float> all(c->hW);
+    for (uint32_t d = 0; d < D; ++d) {
+        const float mean = (float)(sum[d] / K);
+        all.push_back(std::isfinite(mean) ? mean : 0.0f);
+    }
+    return upload(c, &c->dW, all.data(), all.size());
 }
 VQHIP_CATCH(c)
 
@@ -1291,7 +1300,7 @@ const char *check_matrix(const void *p, uint64_t rows, uint64_t width, uint64_t 
 
 int check_euclidean(vqhip_ctx *c, const char *call)
 {
-    if (c->K == 0) return c->fail(VQHIP_ERR_STATE, "no prototypes set (vqhip_set_prototypes)");
+    if (c->K == 0 || !c->dW) return c->fail(VQHIP_ERR_STATE, "no prototypes set (vqhip_set_prototypes)");
     if (c->omega_kind != OMEGA_NONE) return c->fail(VQHIP_ERR_UNSUPPORTED, std::string(call) + " serves Euclidean models; clear Omega first");
     return VQHIP_OK;
 }
@@ -1323,7 +1332,7 @@ try {
     if (const char *why = check_matrix(dS, N, c->K, lds, 4)) return c->fail(VQHIP_ERR_INVALID, std::string("scores_device: ") + why);
     OnDevice on(c->device);
     HIPCHK(c, on.error());
-    HIPCHK(c, launch_scores(dX, N, c->D, c->dW, c->K, dS, lds, (hipStream_t)stream));
+    HIPCHK(c, launch_scores(dX, N, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->K, dS, lds, (hipStream_t)stream));
     return VQHIP_OK;
 }
 VQHIP_CATCH(c)
@@ -1382,7 +1391,7 @@ try {
         if (h.dtop_p) h.dtop_p += off;
         if (h.dmin_p) h.dmin_p += off;
         if (h.dtop_k) h.dtop_k += off;
-        HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->K, (float *)dwork, c->K, s));
+        HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->K, (float *)dwork, c->K, s));
         HIPCHK(c, launch_sample(dwork, VQHIP_F32, n, c->K, c->K, h, du + off, didx_out + off, dprob_out ? dprob_out + off : nullptr, s));
     }
     return VQHIP_OK;
@@ -1396,7 +1405,7 @@ try {
     if (!dtype_bytes(dtype)) return c->fail(VQHIP_ERR_INVALID, "lookup_device: unknown dtype");
     if (K == 0 || K >= (1u << 31) || D == 0 || D > (1u << 24)) return c->fail(VQHIP_ERR_INVALID, "lookup_device: K must lie in [1, 2^31), D in [1, 2^24]");
     if (!dT) {
-        if (c->K == 0) return c->fail(VQHIP_ERR_STATE, "no prototypes set (vqhip_set_prototypes)");
+        if (c->K == 0 || !c->dW) return c->fail(VQHIP_ERR_STATE, "no prototypes set (vqhip_set_prototypes)");
         if (dtype != VQHIP_F32 || K != c->K || D != c->D || ldt != c->D)
             return c->fail(VQHIP_ERR_INVALID, "lookup_device: the context's prototypes are K x D of f32, rows D apart");
         dT = c->dW;
