@@ -3,8 +3,8 @@
 //
 // Two kernels.  Rows of up to DIRECT_D values: k_scores_direct, the formula as it stands on the vector units, a 128 x 128 tile a
 // workgroup, 8 x 8 a lane, so that 16 values read from LDS feed 128 vector instructions.  Longer rows: k_scores_mfma, where the
-// two vector instructions per (sample, prototype, value) of the direct form would bound it, the products run on the f32
-// matrix cores in the expanded form
+// two vector instructions per (sample, prototype, value) of the direct form would bound it, the products run on the bf16
+// matrix cores, six of exact three-piece splits (bf16x6, mfma_device.h), in the expanded form
 //     |x - w|^2 = |x - c|^2 + |w - c|^2 - 2 (x - c).(w - c)
 // with c the mean prototype, so that an offset all values share (pixels) does not cost digits.  Its rounding errors are those
 // of the two norms, so the pairs whose distance is small beside them (below CLOSE of their sum: a sample and the few
@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "mfma_device.h"
 #include "vq_common.h"
 
 namespace vq {
@@ -44,7 +45,7 @@ __device__ __forceinline__ float4 load4(const float *base, uint64_t row, bool on
     return v;
 }
 
-__global__ void __launch_bounds__(SC_THREADS) k_scores_direct(const ScoreArgs a)
+__global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs a)
 {
     __shared__ __attribute__((aligned(16))) float lx[2][SC_K][SC_LD], lw[2][SC_K][SC_LD];
     const uint64_t tile = blockIdx.x;
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(SC_THREADS) k_scores_direct(const ScoreArgs a)
     for (uint32_t d = 0; d < a.D; d += SC_K, b ^= 1) {
         const bool more = d + SC_K < a.D;
         if (more) fetch(d + SC_K);
-#pragma unroll
+#pragma unroll 4
         for (int k = 0; k < SC_K; ++k) {
             float x[8], w[8];
             *(float4 *)&x[0] = *(const float4 *)&lx[b][k][ty * 4];
@@ -128,8 +129,7 @@ __global__ void __launch_bounds__(SC_THREADS) k_scores_direct(const ScoreArgs a)
 // ---------------------------------------------------------------------------------------------- matrix cores
 constexpr uint32_t DIRECT_D = 32;     // rows up to this length: k_scores_direct
 constexpr float CLOSE = 0.125f;       // of |x - c|^2 + |w - c|^2; distances below it are measured directly
-constexpr int MF_THREADS = 256, MF_K = 32, MF_LD = MF_K + 4;       // consecutive LDS rows 4 banks apart (mod 16 of them)
-using f32x16 = __attribute__((ext_vector_type(16))) float;
+constexpr int MF_THREADS = 256, MF_K = 16;
 
 // The sum over 16 consecutive lanes, in the last of them
 __device__ __forceinline__ float row_sum(float v)
@@ -142,14 +142,17 @@ __device__ __forceinline__ float row_sum(float v)
     return v;
 }
 
-// A workgroup: 64 R x 64 R scores, a wave 32 R x 32 R of them in R x R accumulators of v_mfma_f32_32x32x2_f32.  A operand: lane l
-// holds sample l & 31, B operand: prototype l & 31; lanes 0-31 the reduction values 8 q .. + 3 of a step, lanes 32-63
-// 8 q + 4 .. + 7, one of them per instruction.  Result: lane l holds prototype l & 31 and samples 8 g + 4 (l >> 5) + e.
+// A workgroup: 64 R x 64 R scores, a wave 32 R x 32 R of them in R x R accumulators of v_mfma_f32_32x32x16_bf16.  A operand: lane
+// l holds sample l & 31, B operand: prototype l & 31; lanes 0-31 the reduction values 0 .. 7 of a step, lanes 32-63 8 .. 15.
+// Result: lane l holds prototype l & 31 and samples 8 g + 4 (l >> 5) + e.
+// LDS: a piece of a row is 16 bf16 = two 16-byte halves, swapped in every other group of 8 rows, so that 16 lanes reading the same
+// half of 16 rows touch 16 different 16-byte slots of the 64 banks.
 template <int R>
 __global__ void __launch_bounds__(MF_THREADS, 2) k_scores_mfma(const ScoreArgs a)
 {
-    constexpr int TILE = 64 * R, WT = 32 * R, PART = TILE / 32;
-    __shared__ __attribute__((aligned(16))) float lx[2][TILE][MF_LD], lw[2][TILE][MF_LD];
+    constexpr int TILE = 64 * R, WT = 32 * R;
+    __shared__ __attribute__((aligned(16))) uint32_t lds[2][2][3][TILE][8];        // samples, prototypes; two buffers; three pieces
+    auto &lx = lds[0], &lw = lds[1];
     __shared__ __attribute__((aligned(16))) float nx[TILE], nw[TILE];
     // workgroups are dealt to the 8 XCDs in turn: each takes a consecutive share of the tiles, so that the column tiles of the same
     // samples meet in one L2
@@ -158,31 +161,40 @@ __global__ void __launch_bounds__(MF_THREADS, 2) k_scores_mfma(const ScoreArgs a
     const uint32_t col0 = tile % a.colTiles * TILE;
     if (row0 >= a.N) return;
     const int t = threadIdx.x, lane = t & 63, half = lane >> 5, l31 = lane & 31, wr = t >> 7, wc = (t >> 6) & 1;
-    const int sr = t >> 3, sd = (t & 7) * 4;          // staging: values sd .. + 3 of rows sr, sr + 32, ...
+    const int sr = t >> 2, sd = (t & 3) * 4;          // staging: values sd .. + 3 of rows sr, sr + 64
+    const int slot = ((((t & 3) >> 1) ^ (sr >> 3)) & 1) * 4 + (t & 1) * 2;       // ... and where they go, in dwords of the row's piece
+    const int swap = (half ^ (l31 >> 3)) & 1;         // which slot this lane reads
 
-    float4 px[PART], pw[PART], pc;
-    float sx[PART], sw[PART];
+    float4 px[R], pw[R], pc;
+    float sx[R], sw[R];
 #pragma unroll
-    for (int i = 0; i < PART; ++i) sx[i] = sw[i] = 0.0f;
+    for (int i = 0; i < R; ++i) sx[i] = sw[i] = 0.0f;
     auto fetch = [&](uint32_t d) {
         pc = load4(a.C, 0, true, a.D, d + sd, a.vecC);
 #pragma unroll
-        for (int i = 0; i < PART; ++i) {
-            const uint64_t r = row0 + sr + 32 * i;
-            const uint32_t c = col0 + sr + 32 * i;
+        for (int i = 0; i < R; ++i) {
+            const uint64_t r = row0 + sr + 64 * i;
+            const uint32_t c = col0 + sr + 64 * i;
             px[i] = load4(a.X, r, r < a.N, a.D, d + sd, a.vecX);
             pw[i] = load4(a.W, c, c < a.K, a.D, d + sd, a.vecW);
         }
     };
+    auto put = [&](uint32_t (&to)[3][TILE][8], int row, const float4 &v) {
+        uint32_t p[3], q[3];
+        split3(v.x, v.y, p[0], p[1], p[2]);
+        split3(v.z, v.w, q[0], q[1], q[2]);
+#pragma unroll
+        for (int c = 0; c < 3; ++c) *(uint2 *)&to[c][row][slot] = make_uint2(p[c], q[c]);
+    };
     auto stage = [&](int b) {
 #pragma unroll
-        for (int i = 0; i < PART; ++i) {
+        for (int i = 0; i < R; ++i) {
             const float4 x = make_float4(px[i].x - pc.x, px[i].y - pc.y, px[i].z - pc.z, px[i].w - pc.w);
             const float4 w = make_float4(pw[i].x - pc.x, pw[i].y - pc.y, pw[i].z - pc.z, pw[i].w - pc.w);
             sx[i] = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, fmaf(x.w, x.w, sx[i]))));
             sw[i] = fmaf(w.x, w.x, fmaf(w.y, w.y, fmaf(w.z, w.z, fmaf(w.w, w.w, sw[i]))));
-            *(float4 *)&lx[b][sr + 32 * i][sd] = x;
-            *(float4 *)&lw[b][sr + 32 * i][sd] = w;
+            put(lx[b], sr + 64 * i, x);
+            put(lw[b], sr + 64 * i, w);
         }
     };
     f32x16 acc[R][R];
@@ -200,61 +212,70 @@ __global__ void __launch_bounds__(MF_THREADS, 2) k_scores_mfma(const ScoreArgs a
     for (uint32_t d = 0; d < a.D; d += MF_K, b ^= 1) {
         const bool more = d + MF_K < a.D;
         if (more) fetch(d + MF_K);
+        u32x4 fx[R][3], fw[R][3];
 #pragma unroll
-        for (int q = 0; q < MF_K / 8; ++q) {
-            float fx[R][4], fw[R][4];
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                *(float4 *)fx[i] = *(const float4 *)&lx[b][wr * WT + i * 32 + l31][8 * q + 4 * half];
-                *(float4 *)fw[i] = *(const float4 *)&lw[b][wc * WT + i * 32 + l31][8 * q + 4 * half];
+            for (int c = 0; c < 3; ++c) {
+                fx[i][c] = *(const u32x4 *)&lx[b][c][wr * WT + i * 32 + l31][swap * 4];
+                fw[i][c] = *(const u32x4 *)&lw[b][c][wc * WT + i * 32 + l31][swap * 4];
             }
+        // the six products that matter, the smallest first
+        constexpr int PX[6] = {2, 0, 1, 1, 0, 0}, PW[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+        for (int p = 0; p < 6; ++p)
 #pragma unroll
-                for (int i = 0; i < R; ++i)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-                    for (int j = 0; j < R; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fx[i][e], fw[j][e], acc[i][j], 0, 0, 0);
-        }
+                for (int j = 0; j < R; ++j) acc[i][j] = mma_bf(fx[i][PX[p]], fw[j][PW[p]], acc[i][j]);
         if (more) stage(b ^ 1);
         __syncthreads();
     }
-    // the norms: 8 lanes hold the parts of a row
+    // the norms: 4 lanes hold the parts of a row
 #pragma unroll
-    for (int i = 0; i < PART; ++i) {
+    for (int i = 0; i < R; ++i) {
         float x = sx[i], w = sw[i];
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
+        for (int o = 1; o < 4; o <<= 1) {
             x += __shfl_xor(x, o);
             w += __shfl_xor(w, o);
         }
-        if ((t & 7) == 0) {
-            nx[sr + 32 * i] = x;
-            nw[sr + 32 * i] = w;
+        if ((t & 3) == 0) {
+            nx[sr + 64 * i] = x;
+            nw[sr + 64 * i] = w;
         }
     }
     __syncthreads();
 
     // scores, and this wave's list of close pairs (sample << 8 | prototype, inside its tile) in the staging memory
-    uint16_t *list = (uint16_t *)&lx[0][0][0] + (t >> 6) * (WT * WT);
-    static_assert(sizeof lx >= 4 * WT * WT * sizeof(uint16_t), "a list of all pairs of the four waves fits");
+    uint16_t *list = (uint16_t *)&lds[0][0][0][0][0] + (t >> 6) * (WT * WT);
+    static_assert(sizeof lds >= 4 * WT * WT * sizeof(uint16_t), "a list of all pairs of the four waves fits");
     uint32_t n = 0;
+    const bool inside = row0 + TILE <= a.N && col0 + TILE <= a.K;
+    float *const out = a.S + (row0 + wr * WT) * a.ld + col0 + wc * WT;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-        const uint32_t lc = j * 32 + l31, c = col0 + wc * WT + lc;
+        const uint32_t lc = j * 32 + l31;
         const float w2 = nw[wc * WT + lc];
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const uint32_t lr = i * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-                const uint64_t r = row0 + wr * WT + lr;
-                const float both = nx[wr * WT + lr] + w2, s = fmaf(2.0f, acc[i][j][v], -both);
-                const bool on = r < a.N && c < a.K, close = on && !(-s >= CLOSE * both);       // (also where anything is not finite)
-                if (on && !close) a.S[r * a.ld + c] = s;
-                const uint64_t m = __ballot(close);
-                if (m) {
-                    if (close) list[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(lr << 8 | lc);
-                    n += __popcll(m);
+            for (int g = 0; g < 4; ++g) {
+                const uint32_t lr0 = i * 32 + 8 * g + 4 * half;
+                const float4 x2 = *(const float4 *)&nx[wr * WT + lr0];
+                const float fx2[4] = {x2.x, x2.y, x2.z, x2.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t lr = lr0 + e;
+                    const float both = fx2[e] + w2, s = fmaf(2.0f, acc[i][j][4 * g + e], -both);
+                    const bool on = inside || (row0 + wr * WT + lr < a.N && col0 + wc * WT + lc < a.K);
+                    const bool close = on && !(-s >= CLOSE * both);               // (also where anything is not finite)
+                    if (on && !close) out[lr * a.ld + lc] = s;
+                    const uint64_t m = __ballot(close);
+                    if (m) {
+                        if (close) list[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(lr << 8 | lc);
+                        n += __popcll(m);
+                    }
                 }
             }
     }
