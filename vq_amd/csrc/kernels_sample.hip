@@ -16,6 +16,7 @@
 // k_sample_block, a workgroup per row, which first cuts the row down to the few hundred scores the filters are decided
 // among and hands those to the same code as a wave's row.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "codes_device.h"
@@ -38,6 +39,8 @@ struct SampleArgs {
     float *prob;
 };
 
+using u32x4s = uint32_t __attribute__((ext_vector_type(4)));
+
 // ---------------------------------------------------------------------------------------------- keys, weights, wave sums
 constexpr uint32_t KEY_LEAST = 0x007FFFFFu;            // key of -inf: masked scores and NaN
 
@@ -50,37 +53,32 @@ __device__ __forceinline__ uint32_t key_of(float l)
 }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 
-// exp(x) for x <= 0 (0 for -inf and NaN), relative error below 4e-16: x = n ln 2 + r, |r| <= ln 2 / 2, and the exponential series of
-// r to r^12 / 12! (the next term is 1.7e-16)
-__device__ __forceinline__ double exp_down(double x)
-{
-    x = fmax(x, -800.0);
-    const double n = rint(x * 1.4426950408889634);
-    double r = fma(n, -0.693147180369123816490, x);
-    r = fma(n, -1.90821492927058770002e-10, r);
-    double p = 1.0 / 479001600.0;
-    p = fma(p, r, 1.0 / 39916800.0);
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return ldexp(p, (int)n);
-}
-
+// w = exp((l - top) / T) = 2^z, z = (l - top) log2(e) / T <= 0: 2^n by the exponent, 2^f, |f| <= 1/2, by the exponential series of
+// f ln 2 to its 12th power (the next term is 1.7e-16); 0 for -inf and NaN, 1 for the maximum itself, also where that is +inf.
 struct Weigh {
-    uint32_t top_key;
-    double top, inv_t;
-    __device__ __forceinline__ double operator()(uint32_t k) const
+    float top;
+    double scale;                       // log2(e) / T
+    __device__ Weigh() {}
+    __device__ Weigh(float maximum, float temperature) : top(maximum), scale(1.4426950408889634 / (double)temperature) {}
+    __device__ __forceinline__ double operator()(float l) const
     {
-        const double w = exp_down(((double)value_of(k) - top) * inv_t);
-        return k == top_key ? 1.0 : w;                 // (also where the maximum is +inf)
+        const double z = fmax(((double)l - (double)top) * scale, -1100.0), n = rint(z), f = z - n;
+        double p = 2.5678435993488206e-11;              // ln2^k / k!
+        p = fma(p, f, 4.4455382718708116e-10);
+        p = fma(p, f, 7.0549116208011233e-09);
+        p = fma(p, f, 1.0178086009239700e-07);
+        p = fma(p, f, 1.3215486790144309e-06);
+        p = fma(p, f, 1.5252733804059840e-05);
+        p = fma(p, f, 1.5403530393381609e-04);
+        p = fma(p, f, 1.3333558146428443e-03);
+        p = fma(p, f, 9.6181291076284772e-03);
+        p = fma(p, f, 5.5504108664821580e-02);
+        p = fma(p, f, 2.4022650695910071e-01);
+        p = fma(p, f, 6.9314718055994531e-01);
+        p = fma(p, f, 1.0);
+        const uint64_t w = (uint64_t)__double_as_longlong(ldexp(p, (int)n));
+        const uint32_t hi = l == top ? 0x3FF00000u : (uint32_t)(w >> 32);      // (the low half is 0 for the maximum either way)
+        return __longlong_as_double((long long)((uint64_t)hi << 32 | (uint32_t)w));
     }
 };
 
@@ -132,116 +130,170 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v)
 }
 __device__ __forceinline__ double wave_total(double v) { return last_lane(wave_scan(v)); }
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63); }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+// (-inf is what a lane without a source sees)
+__device__ __forceinline__ float wave_max(float v)
 {
-    v = max(v, dpp<0x111, 0xf>(0u, v));
-    v = max(v, dpp<0x112, 0xf>(0u, v));
-    v = max(v, dpp<0x114, 0xf>(0u, v));
-    v = max(v, dpp<0x118, 0xf>(0u, v));
-    v = max(v, dpp<0x142, 0xa>(0u, v));
-    v = max(v, dpp<0x143, 0xc>(0u, v));
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    auto f = [](uint32_t x) { return __uint_as_float(x); };
+    constexpr uint32_t NONE = 0xFF800000u;
+    v = fmaxf(v, f(dpp<0x111, 0xf>(NONE, __float_as_uint(v))));
+    v = fmaxf(v, f(dpp<0x112, 0xf>(NONE, __float_as_uint(v))));
+    v = fmaxf(v, f(dpp<0x114, 0xf>(NONE, __float_as_uint(v))));
+    v = fmaxf(v, f(dpp<0x118, 0xf>(NONE, __float_as_uint(v))));
+    v = fmaxf(v, f(dpp<0x142, 0xa>(NONE, __float_as_uint(v))));
+    v = fmaxf(v, f(dpp<0x143, 0xc>(NONE, __float_as_uint(v))));
+    return f((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
 }
-__device__ __forceinline__ uint32_t wave_min(uint32_t v) { return ~wave_max(~v); }
+__device__ __forceinline__ float wave_min(float v) { return -wave_max(-v); }
 
 // ---------------------------------------------------------------------------------------------- a wave's set of scores
-// 64 E scores in the order of their index, lane i holding E consecutive ones, weights beside them: a weight of 0 is a score
-// that is out (masked, filtered, or padding).  All members are called by the whole wave; what they return is uniform.
+// 64 E scores in the order of their index, lane i holding E consecutive ones, weights beside them.  A score that is out (masked,
+// filtered, of no weight, or padding) is -inf and weighs 0.  All members are called by the whole wave; what they return is uniform.
+constexpr int SET_BINS = 256;
+
 template <int E>
 struct WaveSet {
-    uint32_t key[E];
+    float l[E];
     double w[E];
 
-    // A step of the search for a threshold inside [lo, hi], lo < hi: the middle of the values, which splits an even spread of
-    // scores in half; after `many` steps the middle of the keys, which ends after 32 more however the scores lie.
-    __device__ static uint32_t middle(uint32_t lo, uint32_t hi, int step)
+    __device__ __forceinline__ void weigh_all(const Weigh &weigh)
     {
-        const uint32_t half = lo + (hi - lo) / 2;
-        if (step >= 24) return half;
-        const uint32_t m = key_of(0.5f * value_of(lo) + 0.5f * value_of(hi));
-        return m >= lo && m < hi ? m : half;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            w[e] = weigh(l[e]);
+            l[e] = w[e] > 0.0 ? l[e] : -INFINITY;
+        }
     }
-    __device__ uint32_t count_above(uint32_t k) const
+    __device__ uint32_t count_above(float x) const
     {
         uint32_t n = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) n += __popcll(__ballot(w[e] > 0.0 && key[e] > k));
+        for (int e = 0; e < E; ++e) n += __popcll(__ballot(l[e] > x));
         return n;
     }
-    __device__ double mass_above(uint32_t k) const
+    __device__ uint32_t count_equal(float x) const
+    {
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) n += __popcll(__ballot(l[e] == x));
+        return n;
+    }
+    __device__ double mass_above(float x) const
     {
         double s = 0.0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += key[e] > k ? w[e] : 0.0;
+        for (int e = 0; e < E; ++e) s += l[e] > x ? w[e] : 0.0;
         return wave_total(s);
     }
-    __device__ uint32_t least_key() const
+    // the largest score not above x, the least one above x
+    __device__ float snap_down(float x) const
     {
-        uint32_t m = 0xFFFFFFFFu;
+        float m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = min(m, w[e] > 0.0 ? key[e] : 0xFFFFFFFFu);
+        for (int e = 0; e < E; ++e) m = fmaxf(m, l[e] <= x ? l[e] : -INFINITY);
+        return wave_max(m);
+    }
+    __device__ float snap_up(float x) const
+    {
+        float m = INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fminf(m, l[e] > x ? l[e] : INFINITY);
         return wave_min(m);
     }
-    __device__ uint32_t count_equal(uint32_t k) const
-    {
-        uint32_t n = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) n += __popcll(__ballot(w[e] > 0.0 && key[e] == k));
-        return n;
-    }
 
-    // The threshold of the first k in the order; more than k scores are in.
-    __device__ void cut_count(uint32_t k, uint32_t top_key, uint32_t &t, uint32_t &r) const
+    // The first k in the order end with the score t, of which r of `ties` are among them; more than k scores are in.
+    __device__ void cut_count(uint32_t k, float &t, uint32_t &r, uint32_t &ties) const
     {
-        uint32_t lo = least_key(), hi = top_key;       // fewer than k above hi, k or more above lo - 1
-        for (int step = 0; lo < hi; ++step) {
-            const uint32_t m = middle(lo, hi, step), n = count_above(m);
+        // fewer than k above hi, k or more above lo; hi is one of the scores.  Every step takes at least one value out of the bracket
+        // and, where scores are spread evenly, half of them.
+        float lo = -INFINITY, hi = snap_down(INFINITY);
+        for (;;) {
+            const float least = snap_up(lo);
+            if (least >= hi) break;
+            float m = 0.5f * least + 0.5f * hi;
+            if (!(m >= least && m < hi)) m = least;
+            const uint32_t n = count_above(m);
             if (n == k) {
-                t = m;
-                r = 0;
+                t = snap_up(m);
+                r = ties = count_equal(t);
                 return;
             }
             if (n < k)
-                hi = m;
+                hi = snap_down(m);
             else
-                lo = m + 1;
+                lo = m;
         }
-        t = lo;
+        t = hi;
+        ties = count_equal(t);
         r = k - count_above(t);
     }
 
-    // The threshold of those whose mass before them in the order is below `border` (> 0): the first always.
-    __device__ void cut_mass(double border, uint32_t top_key, uint32_t &t, uint32_t &r, uint32_t &ties) const
+    // A bracket for cut_mass by a histogram over even steps of the score, `span` of it in all, from the maximum `high` down.  Its
+    // masses are integers, w 2^21 rounded, which at most 1024 of them put at most 512 off: with 600 to spare on either side
+    // the border lies in the bins found, whatever their order of addition.
+    __device__ __forceinline__ void narrow(double border, float high, float span, float &lo, float &hi, uint32_t *bins) const
     {
-        uint32_t lo = least_key(), hi = top_key;       // mass above hi is below the border
-        for (int step = 0; lo < hi; ++step) {
-            const uint32_t m = middle(lo, hi, step);
-            if (mass_above(m) < border)
-                hi = m;
-            else
-                lo = m + 1;
-            uint32_t n = 0, some = 0;                  // a single score left inside: it is the threshold
+        static_assert(E <= 16, "at most 1024 scores");
+        const float per = (float)SET_BINS / span;
+        const uint32_t lane = threadIdx.x & 63;
+        *(uint4 *)&bins[4 * lane] = make_uint4(0, 0, 0, 0);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        uint32_t bin[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const bool in = w[e] > 0.0 && key[e] >= lo && key[e] <= hi;
-                n += __popcll(__ballot(in));
-                some = max(some, in ? key[e] : 0u);
-            }
-            if (n == 1) {
-                lo = hi = wave_max(some);
-                break;
-            }
+        for (int e = 0; e < E; ++e) {
+            // (a maximum or a step beyond all bounds: 0 * inf and the like go to the last bin, but for the maximum itself)
+            const float at = fminf((high - l[e]) * per, (float)(SET_BINS - 1));
+            bin[e] = l[e] == high ? 0u : (uint32_t)at;
+            const uint32_t f = (uint32_t)fma(w[e], 0x1p21, 0.5);
+            if (f) atomicAdd(&bins[bin[e]], f);
         }
-        t = lo;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint4 c = *(const uint4 *)&bins[4 * lane];
+        const uint32_t p0 = c.x, p1 = p0 + c.y, p2 = p1 + c.z, p3 = p2 + c.w, base = wave_scan(p3) - p3;
+        auto first = [&](uint32_t x) -> uint32_t {                      // the first bin that brings the total to x
+            const uint64_t hit = __ballot(base + p3 >= x);
+            if (!hit) return SET_BINS - 1;
+            const int q = __ffsll((unsigned long long)hit) - 1;
+            const uint32_t in = (base + p0 < x) + (base + p1 < x) + (base + p2 < x);
+            return 4 * q + (uint32_t)__builtin_amdgcn_readlane((int)in, q);
+        };
+        const double units = border * 0x1p21;
+        const uint32_t b0 = first(units > 600.0 ? (uint32_t)(units - 600.0) : 0u), b1 = first((uint32_t)fmin(units + 600.0, 4294967295.0));
+        float top = -INFINITY, below = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            top = fmaxf(top, bin[e] >= b0 ? l[e] : -INFINITY);
+            below = fmaxf(below, bin[e] > b1 ? l[e] : -INFINITY);
+        }
+        hi = wave_max(top);
+        lo = wave_max(below);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+
+    // Those whose mass before them in the order is below `border` (> 0), the first always: they end with the score t, of which r of
+    // `ties` are among them.  high: the largest score that is in.
+    __device__ __forceinline__ void cut_mass(double border, float high, float span, float &t, uint32_t &r, uint32_t &ties, uint32_t *bins) const
+    {
+        float lo = -INFINITY, hi = high;               // mass above hi below the border, mass above lo not
+        narrow(border, high, span, lo, hi, bins);
+        for (;;) {
+            const float least = snap_up(lo);
+            if (least >= hi) break;
+            float m = 0.5f * least + 0.5f * hi;
+            if (!(m >= least && m < hi)) m = least;
+            if (mass_above(m) < border)
+                hi = snap_down(m);
+            else
+                lo = m;
+        }
+        t = hi;
         ties = count_equal(t);
         double wt = 0.0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) wt = key[e] == t ? fmax(wt, w[e]) : wt;
+        for (int e = 0; e < E; ++e) wt = l[e] == t ? w[e] : wt;
         const uint64_t has = __ballot(wt > 0.0);
         wt = lane_of(wt, __ffsll((unsigned long long)has) - 1);
-        const double above = mass_above(t);
-        // the j-th of the equal ones (from 0) is kept while above + j wt < border
-        r = equal_kept(border - above, wt, ties);
+        // the j-th of the equal ones (from 0) is kept while (mass above) + j wt < border
+        r = ties == 1 ? 1u : equal_kept(border - mass_above(t), wt, ties);
     }
     // The least r in [1, ties] with r wt >= room.
     __device__ static uint32_t equal_kept(double room, double wt, uint32_t ties)
@@ -250,38 +302,50 @@ struct WaveSet {
         uint32_t r = q < 1.0 ? 1u : q > (double)ties ? ties : (uint32_t)q;
         if (r > 1 && (double)(r - 1) * wt >= room) --r;
         if (r < ties && (double)r * wt < room) ++r;
-        return r;
+        return (uint32_t)__builtin_amdgcn_readfirstlane((int)r);
     }
 
-    // Weights of scores behind the threshold become 0.
-    __device__ void apply(uint32_t t, uint32_t r)
+    // Scores behind the threshold go out.
+    __device__ __forceinline__ void apply(float t, uint32_t r, uint32_t ties)
     {
-        uint32_t mine = 0;
+        if (r < ties) {                                // by index, of the equal ones
+            uint32_t mine = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) mine += w[e] > 0.0 && key[e] == t;
-        uint32_t before = 0;
-        const bool all = wave_total(mine) <= r;
-        if (!all) before = wave_scan(mine) - mine;
+            for (int e = 0; e < E; ++e) mine += l[e] == t;
+            uint32_t before = wave_scan(mine) - mine;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const bool eq = l[e] == t;
+                if (eq && before >= r) {
+                    l[e] = -INFINITY;
+                    w[e] = 0.0;
+                }
+                before += eq;
+            }
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const bool eq = w[e] > 0.0 && key[e] == t;
-            if (key[e] < t || (eq && !all && before >= r)) w[e] = 0.0;
-            before += eq;
+            const bool in = l[e] >= t;
+            l[e] = in ? l[e] : -INFINITY;
+            w[e] = in ? w[e] : 0.0;
         }
     }
 
     // The filters, then the draw.  -> place of the index drawn in the set, its weight, the sum of the weights.
-    __device__ uint32_t draw(uint32_t top_key, uint32_t top_k, float top_p, float min_p, float u, double &drawn, double &total)
+    __device__ __forceinline__ uint32_t draw(float top, uint32_t top_k, float top_p, float min_p, float u, float reach, uint32_t *bins, double &drawn,
+                                             double &total)
     {
-        if (top_k > 0 && count_above(KEY_LEAST) > top_k) {
-            uint32_t t, r;
-            cut_count(top_k, top_key, t, r);
-            apply(t, r);
+        if (top_k > 0 && count_above(-INFINITY) > top_k) {
+            float t;
+            uint32_t r, ties;
+            cut_count(top_k, t, r, ties);
+            apply(t, r, ties);
         }
         if (top_p < 1.0f) {
-            uint32_t t, r, ties;
-            cut_mass((double)top_p * mass_above(KEY_LEAST), top_key, t, r, ties);
-            apply(t, r);
+            float t;
+            uint32_t r, ties;
+            cut_mass((double)top_p * mass_above(-INFINITY), top, reach, t, r, ties, bins);
+            apply(t, r, ties);
         }
         if (min_p > 0.0f) {
             const double least = (double)fminf(min_p, 1.0f);
@@ -296,25 +360,24 @@ struct WaveSet {
         const double target = (double)u * total;
         // the first lane past the target; should rounding leave the target at the very end, the last lane that holds anything
         const uint64_t some = __ballot(mine > 0.0), hit = __ballot(mine > 0.0 && upto > target);
-        const int l = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(some);
-        double before = lane_of(upto - mine, l);
+        const int q = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(some);
+        double run = upto - mine;
         uint32_t at = 0;
         bool done = false;
         drawn = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const double x = w[e];
-            before += x;
+            run += x;
             if (!done && x > 0.0) {
                 at = e;
                 drawn = x;
-                done = before > target;
+                done = run > target;
             }
         }
-        // (only lane l's walk counts: it started from that lane's own sum)
-        at = (uint32_t)__builtin_amdgcn_readlane((int)at, l);
-        drawn = lane_of(drawn, l);
-        return (uint32_t)l * E + at;
+        at = (uint32_t)__builtin_amdgcn_readlane((int)at, q);
+        drawn = lane_of(drawn, q);
+        return (uint32_t)q * E + at;
     }
 };
 
@@ -334,6 +397,9 @@ struct RowParams {
         if (!(top_p < 1.0f)) top_p = 1.0f;
         if (!(min_p > 0.0f)) min_p = 0.0f;
     }
+    // How far below the maximum the border of a nucleus among V scores lies at most: all scores more than ln(V / (1 - p)) below
+    // it (in units of T) together weigh less than 1 - p.
+    __device__ float reach(uint32_t V) const { return (__logf((float)V) - __logf(fmaxf(1.0f - top_p, 0x1p-24f)) + 1.0f) * temperature; }
 };
 
 // ---------------------------------------------------------------------------------------------- a wave per row
@@ -343,6 +409,7 @@ constexpr int WAVE_THREADS = 256;
 template <class T, int E, bool VEC>
 __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a)
 {
+    __shared__ __attribute__((aligned(16))) uint32_t bins[WAVE_THREADS / 64][SET_BINS];
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t waves = (uint64_t)gridDim.x * (WAVE_THREADS / 64);
     for (uint64_t i = (uint64_t)blockIdx.x * (WAVE_THREADS / 64) + (threadIdx.x >> 6); i < a.N; i += waves) {
@@ -355,34 +422,32 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
             if (VEC && j0 + c + LOAD <= a.V) {
                 const Pack<T, LOAD * (int)sizeof(T)> v = *(const Pack<T, LOAD * (int)sizeof(T)> *)(row + j0 + c);
 #pragma unroll
-                for (int e = 0; e < LOAD; ++e) set.key[c + e] = key_of(widen(v.v[e]));
+                for (int e = 0; e < LOAD; ++e) set.l[c + e] = fmaxf(widen(v.v[e]), -INFINITY);      // (NaN: -inf)
             } else {
 #pragma unroll
-                for (int e = 0; e < LOAD; ++e) set.key[c + e] = j0 + c + e < a.V ? key_of(widen(row[j0 + c + e])) : KEY_LEAST;
+                for (int e = 0; e < LOAD; ++e) set.l[c + e] = j0 + c + e < a.V ? fmaxf(widen(row[j0 + c + e]), -INFINITY) : -INFINITY;
             }
         }
         const RowParams p(a, i);
-        uint32_t most = 0;
+        float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) most = max(most, set.key[e]);
-        most = wave_max(most);
+        for (int e = 0; e < E; ++e) top = fmaxf(top, set.l[e]);
+        top = wave_max(top);
         uint32_t at = 0;
         float prob = 0.0f;
-        if (most > KEY_LEAST) {
+        if (top > -INFINITY) {
             if (p.greedy) {
                 uint32_t e1 = E;
 #pragma unroll
                 for (int e = E - 1; e >= 0; --e)
-                    if (set.key[e] == most) e1 = e;
-                const int l = __ffsll((unsigned long long)__ballot(e1 < E)) - 1;
-                at = (uint32_t)l * E + (uint32_t)__builtin_amdgcn_readlane((int)e1, l);
+                    if (set.l[e] == top) e1 = e;
+                const int q = __ffsll((unsigned long long)__ballot(e1 < E)) - 1;
+                at = (uint32_t)q * E + (uint32_t)__builtin_amdgcn_readlane((int)e1, q);
                 prob = 1.0f;
             } else {
-                const Weigh weigh{most, (double)value_of(most), 1.0 / (double)p.temperature};
-#pragma unroll
-                for (int e = 0; e < E; ++e) set.w[e] = weigh(set.key[e]);
+                set.weigh_all(Weigh(top, p.temperature));
                 double drawn, total;
-                at = set.draw(most, p.top_k, p.top_p, p.min_p, p.u, drawn, total);
+                at = set.draw(top, p.top_k, p.top_p, p.min_p, p.u, p.reach(a.V), bins[threadIdx.x >> 6], drawn, total);
                 prob = (float)(drawn / total);
             }
         }
@@ -404,17 +469,42 @@ struct BlockShared {
     union {
         unsigned long long mass[BINS];
         struct {
-            uint32_t key[WAVES * SEGMENT], at[WAVES * SEGMENT];
+            float l[WAVES * SEGMENT];
+            uint32_t at[WAVES * SEGMENT];
         } segment;
     };
-    uint32_t list_key[LIST], list_at[LIST];
-    unsigned long long wide[WAVES];
+    float list_l[LIST];
+    uint32_t list_at[LIST];
+    unsigned long long wide[WAVES], hist_mass[256], above;
     double sums[WAVES];
-    uint32_t words[WAVES];
-    uint32_t hist[256];
-    unsigned long long hist_mass[256];
-    uint32_t n, t, r, ties;
-    unsigned long long above;
+    float queue[WAVES][128];            // scores of the draw on their way to a full wave
+    uint32_t words[WAVES], hist[256];
+    __attribute__((aligned(16))) uint32_t bins[SET_BINS];
+    uint32_t n, pick, found;
+    float t;
+};
+// One per workgroup, the same for the kernel and the functions it calls.
+template <class T, int THREADS>
+__device__ __forceinline__ BlockShared<THREADS> &block_shared()
+{
+    __shared__ BlockShared<THREADS> sh;
+    return sh;
+}
+
+// Scalars that are the same in all lanes, told to the compiler (arguments of a called function are not).
+__device__ __forceinline__ uint32_t same(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ float same(float v) { return __uint_as_float(same(__float_as_uint(v))); }
+__device__ __forceinline__ uint64_t same(uint64_t v) { return (uint64_t)same((uint32_t)(v >> 32)) << 32 | same((uint32_t)v); }
+__device__ __forceinline__ double same(double v) { return __longlong_as_double((long long)same((uint64_t)__double_as_longlong(v))); }
+
+// A cut of the order: it ends with the score t, of which r of `ties` are kept.  t = -inf: not cut.
+struct Cut {
+    float t;
+    uint32_t r, ties;
+};
+struct Drawn {
+    uint32_t at;
+    float prob;
 };
 
 // One row, worked on by a workgroup: all members are called by all its lanes.  The row is dealt to the waves in consecutive
@@ -424,18 +514,30 @@ struct BlockRow {
     static constexpr int WAVES = THREADS / 64;
     static constexpr int PER = VEC ? 16 / (int)sizeof(T) : 1;
     static constexpr uint32_t STEP = 64 * PER;
-    using Shared = BlockShared<THREADS>;
+    using Piece = Pack<T, PER * (int)sizeof(T)>;
+    using GlobalT = const __attribute__((address_space(1))) T;
+    using Global16 = const __attribute__((address_space(1))) u32x4s;
 
-    Shared &sh;
-    const T *row;
+    uint64_t row;                       // address of the row in global memory
     uint32_t V;
     int s;
     Weigh weigh;
 
-    __device__ static uint32_t wave() { return threadIdx.x >> 6; }
-    __device__ static uint32_t lane() { return threadIdx.x & 63; }
+    __device__ __forceinline__ static BlockShared<THREADS> &shared() { return block_shared<T, THREADS>(); }
+    __device__ __forceinline__ BlockRow uniform() const
+    {
+        BlockRow b;
+        b.row = same(row);
+        b.V = same(V);
+        b.s = (int)same((uint32_t)s);
+        b.weigh.top = same(weigh.top);
+        b.weigh.scale = same(weigh.scale);
+        return b;
+    }
+    __device__ __forceinline__ static uint32_t wave() { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+    __device__ __forceinline__ static uint32_t lane() { return threadIdx.x & 63; }
     // this wave's part of [lo, hi)
-    __device__ static void part(uint32_t &lo, uint32_t &hi)
+    __device__ __forceinline__ static void part(uint32_t &lo, uint32_t &hi)
     {
         const uint32_t steps = (hi - lo + STEP - 1) / STEP, len = (steps + WAVES - 1) / WAVES * STEP;
         const uint64_t from = (uint64_t)lo + (uint64_t)wave() * len;
@@ -443,28 +545,34 @@ struct BlockRow {
         lo = (uint32_t)min(from, (uint64_t)end);
         hi = (uint32_t)min(from + len, (uint64_t)end);
     }
+    __device__ __forceinline__ Piece load_whole(uint32_t j) const
+    {
+        if constexpr (VEC) {
+            return __builtin_bit_cast(Piece, *(Global16 *)(row + (uint64_t)j * sizeof(T)));
+        } else {
+            Piece v;
+            v.v[0] = ((GlobalT *)row)[j];
+            return v;
+        }
+    }
     // This lane's scores of one step; what lies behind `hi` is a masked score.
-    using Piece = Pack<T, PER * (int)sizeof(T)>;
     __device__ __forceinline__ Piece load(uint32_t base, uint32_t hi) const
     {
         const uint32_t j = base + lane() * PER;
+        if (j + PER <= hi) return load_whole(j);
         Piece v;
-        if (j + PER <= hi) {
-            v = *(const Piece *)(row + j);
-        } else {
 #pragma unroll
-            for (int e = 0; e < PER; ++e) v.v[e] = j + e < hi ? row[j + e] : (T)-INFINITY;
-        }
+        for (int e = 0; e < PER; ++e) v.v[e] = j + e < hi ? ((GlobalT *)row)[j + e] : (T)-INFINITY;
         return v;
     }
-    // f(index of the first, keys) for this lane's scores of one step
+    // f(index of the first, scores) for this lane's scores of one step
     template <class F>
     __device__ __forceinline__ void step_of(uint32_t base, const Piece &v, F &&f) const
     {
-        uint32_t key[PER];
+        float l[PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) key[e] = key_of(widen(v.v[e]));
-        f(base + lane() * PER, key);
+        for (int e = 0; e < PER; ++e) l[e] = widen(v.v[e]);
+        f(base + lane() * PER, l);
     }
     // ... and of all steps of [lo, hi).  FLIGHT steps are on their way at a time: 4 where f is a few instructions; where it
     // computes weights, the one next is, which its hundreds of instructions cover.
@@ -487,7 +595,7 @@ struct BlockRow {
         for (; base < hi && hi - base >= FLIGHT * STEP; base += FLIGHT * STEP) {
             Piece v[FLIGHT];
 #pragma unroll
-            for (uint32_t q = 0; q < FLIGHT; ++q) v[q] = *(const Piece *)(row + base + q * STEP + lane() * PER);
+            for (uint32_t q = 0; q < FLIGHT; ++q) v[q] = load_whole(base + q * STEP + lane() * PER);
 #pragma unroll
             for (uint32_t q = 0; q < FLIGHT; ++q) step_of(base + q * STEP, v[q], f);
         }
@@ -495,35 +603,39 @@ struct BlockRow {
         for (; base < hi; base += STEP) step_of(base, load(base, hi), f);
     }
 
-    __device__ unsigned long long fixed(double w) const
+    __device__ __forceinline__ unsigned long long fixed(double w) const
     {
         // w 2^s + 2^52 has the rounded integer in its mantissa (s <= 51, w <= 1)
         const double d = fma(w, __longlong_as_double((long long)(1023 + s) << 52), 0x1p52);
         return (unsigned long long)__double_as_longlong(d) & 0xFFFFFFFFFFFFFull;
     }
 
-    // Maximum of the row; mine: of what this lane has seen.
-    __device__ uint32_t find_top(uint32_t &mine)
+    // Maximum of the row; mine: of what this lane has seen.  (fmaxf passes NaN over.)
+    __device__ __forceinline__ float find_top(float &mine) const
     {
-        uint32_t lo = 0, hi = V, m = 0;
+        auto &sh = shared();
+        uint32_t lo = 0, hi = V;
         part(lo, hi);
-        each<4>(lo, hi, [&](uint32_t, const uint32_t (&k)[PER]) {
+        float high = -INFINITY;
+        each<4>(lo, hi, [&](uint32_t, const float (&l)[PER]) {
 #pragma unroll
-            for (int e = 0; e < PER; ++e) m = max(m, k[e]);
+            for (int e = 0; e < PER; ++e) high = fmaxf(high, l[e]);
         });
-        mine = m;
-        m = wave_max(m);
-        if (lane() == 0) sh.words[wave()] = m;
+        mine = high;
+        high = wave_max(high);
+        if (lane() == 0) sh.words[wave()] = __float_as_uint(high);
         __syncthreads();
-        for (int k = 0; k < WAVES; ++k) m = max(m, sh.words[k]);
+        for (int k = 0; k < WAVES; ++k) high = fmaxf(high, __uint_as_float(sh.words[k]));
         __syncthreads();
-        return m;
+        return same(high + 0.0f);
     }
 
     // The k-th largest (1 <= k <= THREADS) of one key per lane, by 8 bits at a time.
-    __device__ uint32_t kth_largest(uint32_t key, uint32_t k)
+    __device__ __forceinline__ uint32_t kth_largest(uint32_t key, uint32_t k) const
     {
+        auto &sh = shared();
         uint32_t prefix = 0;
+#pragma unroll 1
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
             __syncthreads();
@@ -538,8 +650,9 @@ struct BlockRow {
         return prefix;
     }
     // Over sh.hist: the bin that holds the k-th from the top, and how many lie in the bins above it.  Every wave for itself.
-    __device__ uint32_t border_bin(uint32_t k, uint32_t &above) const
+    __device__ __forceinline__ uint32_t border_bin(uint32_t k, uint32_t &above) const
     {
+        auto &sh = shared();
         uint32_t c[4], mine = 0;                       // lane l: bins 255 - 4 l down to 252 - 4 l
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -548,7 +661,7 @@ struct BlockRow {
         }
         const uint32_t upto = wave_scan(mine);
         const uint64_t hit = __ballot(upto >= k);
-        const int l = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
+        const int q = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
         uint32_t run = upto - mine, at = 3, before = run;
         bool done = false;
 #pragma unroll
@@ -560,30 +673,34 @@ struct BlockRow {
                 done = run >= k;
             }
         }
-        at = (uint32_t)__builtin_amdgcn_readlane((int)at, l);
-        above = (uint32_t)__builtin_amdgcn_readlane((int)before, l);
-        return 255 - 4 * l - at;
+        at = (uint32_t)__builtin_amdgcn_readlane((int)at, q);
+        above = (uint32_t)__builtin_amdgcn_readlane((int)before, q);
+        return 255 - 4 * q - at;
     }
 
-    // The scores `in` says, in the order of their index, into the list.  False if they do not fit.
+    // The scores in [least, most] that `in` says, in the order of their index, into the list.  False if they do not fit.
     template <class P>
-    __device__ bool collect(P &&in)
+    __device__ __forceinline__ bool collect(float least, float most, P &&in) const
     {
+        auto &sh = shared();
         uint32_t lo = 0, hi = V, n = 0;
         part(lo, hi);
         const uint32_t w = wave();
-        each<4>(lo, hi, [&](uint32_t j, const uint32_t (&k)[PER]) {
+        each<4>(lo, hi, [&](uint32_t j, const float (&l)[PER]) {
+            bool some = false;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) some |= l[e] >= least && l[e] <= most;
+            if (__ballot(some) == 0) return;
             uint32_t mask = 0;
 #pragma unroll
-            for (int e = 0; e < PER; ++e) mask |= in(k[e]) ? 1u << e : 0u;
-            if (__ballot(mask != 0) == 0) return;
+            for (int e = 0; e < PER; ++e) mask |= l[e] >= least && l[e] <= most && in(l[e]) ? 1u << e : 0u;
             const uint32_t c = __popc(mask), upto = wave_scan(c);
             uint32_t to = n + upto - c;
 #pragma unroll
             for (int e = 0; e < PER; ++e)
                 if ((mask >> e) & 1) {
                     if (to < SEGMENT) {
-                        sh.segment.key[w * SEGMENT + to] = k[e];
+                        sh.segment.l[w * SEGMENT + to] = l[e];
                         sh.segment.at[w * SEGMENT + to] = j + e;
                     }
                     ++to;
@@ -602,343 +719,399 @@ struct BlockRow {
         fits = fits && all <= LIST;
         if (fits)
             for (uint32_t q = lane(); q < n; q += 64) {
-                sh.list_key[before + q] = sh.segment.key[w * SEGMENT + q];
+                sh.list_l[before + q] = sh.segment.l[w * SEGMENT + q];
                 sh.list_at[before + q] = sh.segment.at[w * SEGMENT + q];
             }
         if (threadIdx.x == 0) sh.n = all;
         __syncthreads();
-        return fits;
+        return same((uint32_t)fits) != 0;
     }
 
     // The list as a wave's set.
     template <int E>
-    __device__ void load_list(WaveSet<E> &set) const
+    __device__ __forceinline__ void load_list(WaveSet<E> &set) const
     {
+        auto &sh = shared();
+        const uint32_t n = same(sh.n);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const uint32_t q = lane() * E + e;
-            set.key[e] = q < sh.n ? sh.list_key[q] : KEY_LEAST;
-            set.w[e] = weigh(set.key[e]);
+            set.l[e] = q < n ? sh.list_l[q] : -INFINITY;
         }
-    }
-    template <int E>
-    __device__ void draw_from_list(const RowParams &p, uint32_t &at, float &prob)
-    {
-        WaveSet<E> set;
-        load_list(set);
-        double drawn, total;
-        at = sh.list_at[set.draw(weigh.top_key, p.top_k, p.top_p, p.min_p, p.u, drawn, total)];
-        prob = (float)(drawn / total);
-    }
-    template <int E>
-    __device__ void cut_list(double border, uint32_t &t, uint32_t &r, uint32_t &ties)
-    {
-        WaveSet<E> set;
-        load_list(set);
-        set.cut_mass(border, weigh.top_key, t, r, ties);
-    }
-
-    // Radix selection over the whole row, 8 bits of the key at a time, for the rows the list does not serve (top_k beyond it,
-    // a border among more equal or nearly equal scores than it holds).  Kept so far: keys above t and r of those equal to t;
-    // on return the shorter beginning.  By count: the first `border`.  By mass: those whose mass before them is below it.
-    template <bool MASS>
-    __device__ void cut(unsigned long long border, uint32_t &t, uint32_t &r, uint32_t &ties)
-    {
-        uint32_t prefix = 0, found = 0;
-        bool first = true;
-        unsigned long long before = 0;
-        // the low bits of a widened 16-bit score follow from its sign: 16 of them for bf16, 13 for f16
-        constexpr int LAST = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 16 : 8;
-        for (int shift = 24; shift >= LAST; shift -= 8) {
-            if (threadIdx.x < 256) {
-                sh.hist[threadIdx.x] = 0;
-                sh.hist_mass[threadIdx.x] = 0;
-            }
-            __syncthreads();
-            uint32_t lo = 0, hi = V;
-            part(lo, hi);
-            each<1>(lo, hi, [&](uint32_t, const uint32_t (&k)[PER]) {
-#pragma unroll
-                for (int e = 0; e < PER; ++e) {
-                    if (k[e] < t || k[e] <= KEY_LEAST || (!first && (k[e] >> (shift + 8)) != prefix)) continue;
-                    const uint32_t b = (k[e] >> shift) & 255;
-                    atomicAdd(&sh.hist[b], 1u);
-                    if (MASS && k[e] > t) atomicAdd(&sh.hist_mass[b], fixed(weigh(k[e])));
-                }
-            });
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                // of the keys equal to t only r are left
-                if (MASS && r != 0 && t > KEY_LEAST && (first || (t >> (shift + 8)) == prefix)) sh.hist_mass[(t >> shift) & 255] += (unsigned long long)r * fixed(weigh(t));
-                // the bin of the last element kept: the lowest whose total above it is below the border
-                unsigned long long run = before, above = before;
-                uint32_t pick = 0;
-                bool any = false;
-                for (int b = 255; b >= 0; --b) {
-                    if (sh.hist[b] == 0) continue;
-                    if (run >= border && any) break;
-                    any = true;
-                    pick = b;
-                    above = run;
-                    run += MASS ? sh.hist_mass[b] : sh.hist[b];
-                }
-                sh.n = pick;
-                sh.above = above;
-                sh.ties = any ? sh.hist[pick] : 0;
-            }
-            __syncthreads();
-            prefix = (prefix << 8) | sh.n;
-            before = sh.above;
-            found = sh.ties;
-            first = false;
-            __syncthreads();
-        }
-        if (found == 0) return;
-        uint32_t nt = prefix << LAST;
-        if (!(nt >> 31)) nt |= (1u << LAST) - 1u;        // a negative score: the folded bits are ones
-        ties = found;
-        const uint32_t most = nt == t ? min(found, r) : found;               // the border of an earlier cut
-        uint32_t nr;
-        if (MASS) {
-            const unsigned long long w = fixed(weigh(nt));
-            nr = border <= before ? 1 : w == 0 ? most : (uint32_t)min((unsigned long long)most, (border - before + w - 1) / w);
-            nr = max(nr, 1u);
-        } else {
-            nr = (uint32_t)min((unsigned long long)most, border - before);
-        }
-        t = nt;
-        r = nr;
-    }
-
-    // Index of the r-th (r >= 1) score equal to t.
-    __device__ uint32_t nth_equal(uint32_t t, uint32_t r)
-    {
-        uint32_t lo = 0, hi = V, n = 0;
-        part(lo, hi);
-        each<4>(lo, hi, [&](uint32_t, const uint32_t (&k)[PER]) {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) n += k[e] == t;
-        });
-        n = wave_total(n);
-        if (lane() == 0) sh.words[wave()] = n;
-        __syncthreads();
-        uint32_t before = 0;
-        for (uint32_t k = 0; k < wave(); ++k) before += sh.words[k];
-        if (before < r && before + n >= r) {              // this wave's part holds it
-            for (uint32_t base = lo; base < hi; base += STEP) {
-                bool done = false;
-                step_of(base, load(base, hi), [&](uint32_t j, const uint32_t (&k)[PER]) {
-                    uint32_t c = 0;
-#pragma unroll
-                    for (int e = 0; e < PER; ++e) c += k[e] == t;
-                    const uint32_t upto = wave_scan(c), here = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-                    if (before + here >= r) {
-                        uint32_t at = before + upto - c;
-#pragma unroll
-                        for (int e = 0; e < PER; ++e) {
-                            at += k[e] == t;
-                            if (k[e] == t && at == r) sh.n = j + e;
-                        }
-                        done = true;
-                    }
-                    before += here;
-                });
-                if (done) break;
-            }
-        }
-        __syncthreads();
-        const uint32_t at = sh.n;
-        __syncthreads();
-        return at;
-    }
-
-    // The draw among keys above t and those equal to t up to index last_equal, with weights of at least `least`.
-    __device__ void draw(uint32_t t, uint32_t last_equal, double least, float u, uint32_t &at, float &prob)
-    {
-        const uint32_t floor_key = max(t, KEY_LEAST + 1);
-        auto kept = [&](uint32_t k, uint32_t j) -> double {
-            if (k < floor_key || (k == t && j > last_equal)) return 0.0;
-            const double x = weigh(k);
-            return x >= least ? x : 0.0;
-        };
-        uint32_t lo = 0, hi = V;
-        double before = 0.0, target = 0.0, total = 0.0;
-        // sums of the waves' parts, the part the target falls in, its parts, ... down to one step
-        for (bool whole = true; whole || hi - lo > STEP; whole = false) {
-            uint32_t a = lo, b = hi;
-            part(a, b);
-            double mine = 0.0;
-            each<1>(a, b, [&](uint32_t j, const uint32_t (&k)[PER]) {
-#pragma unroll
-                for (int e = 0; e < PER; ++e) mine += kept(k[e], j + e);
-            });
-            mine = wave_total(mine);
-            if (lane() == 0) sh.sums[wave()] = mine;
-            __syncthreads();
-            if (whole) {
-                for (int k = 0; k < WAVES; ++k) total += sh.sums[k];
-                target = (double)u * total;
-            }
-            int pick = -1;
-            for (int k = 0; k < WAVES; ++k) {
-                if (sh.sums[k] == 0.0) continue;
-                if (pick >= 0) before += sh.sums[pick];
-                pick = k;
-                if (before + sh.sums[k] > target) break;
-            }
-            const uint32_t steps = (hi - lo + STEP - 1) / STEP, len = (steps + WAVES - 1) / WAVES * STEP;
-            lo += (uint32_t)pick * len;
-            hi = (uint32_t)min((uint64_t)lo + len, (uint64_t)hi);
-            __syncthreads();
-        }
-        step_of(lo, load(lo, hi), [&](uint32_t j, const uint32_t (&k)[PER]) {
-            double x[PER], mine = 0.0;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                x[e] = kept(k[e], j + e);
-                mine += x[e];
-            }
-            const double upto = before + wave_scan(mine);
-            const uint64_t some = __ballot(mine > 0.0), hit = __ballot(mine > 0.0 && upto > target);
-            const int l = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(some);
-            double run = upto - mine, drawn = 0.0;
-            uint32_t place = 0;
-            bool done = false;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                run += x[e];
-                if (!done && x[e] > 0.0) {
-                    place = e;
-                    drawn = x[e];
-                    done = run > target;
-                }
-            }
-            at = (uint32_t)__builtin_amdgcn_readlane((int)(j + place), l);
-            prob = (float)(lane_of(drawn, l) / total);
-        });
+        set.weigh_all(weigh);
     }
 };
+
+// The parts of a row's work that a row needs once at most, as functions of their own: one kernel with all of them in line does not
+// fit its registers.
+template <class Row, int E>
+__device__ __attribute__((noinline)) Drawn list_draw(const Row r, const RowParams p)
+{
+    const Row row = r.uniform();
+    WaveSet<E> set;
+    row.load_list(set);
+    double drawn, total;
+    const uint32_t q = set.draw(row.weigh.top, same(p.top_k), same(p.top_p), same(p.min_p), same(p.u), same(p.reach(row.V)), Row::shared().bins, drawn, total);
+    return {Row::shared().list_at[q], (float)(drawn / total)};
+}
+
+template <class Row, int E>
+__device__ __attribute__((noinline)) Cut list_cut(const Row r, double border)
+{
+    const Row row = r.uniform();
+    WaveSet<E> set;
+    row.load_list(set);
+    const float high = set.snap_down(INFINITY), low = set.snap_up(-INFINITY);
+    Cut c;
+    set.cut_mass(same(border), high, high > low ? high - low : 1.0f, c.t, c.r, c.ties, Row::shared().bins);
+    return c;
+}
+
+// Radix selection over the whole row, 8 bits of the ordered key at a time, for the rows the list does not serve (top_k beyond it,
+// a border among more equal or nearly equal scores than it holds).  `old`: an earlier cut.  By count: the first `border`.  By
+// mass: those whose mass before them is below it.
+template <class Row, class T, int THREADS, bool MASS>
+__device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long long border, const Cut o)
+{
+    const Row row = r0.uniform();
+    auto &sh = Row::shared();
+    border = same((uint64_t)border);
+    const Cut old{same(o.t), same(o.r), same(o.ties)};
+    const uint32_t t = key_of(old.t);
+    uint32_t prefix = 0, found = 0;
+    bool first = true;
+    unsigned long long before = 0;
+    // the low bits of a widened 16-bit score follow from its sign: 16 of them for bf16, 13 for f16
+    constexpr int LAST = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 16 : 8;
+#pragma unroll 1
+    for (int shift = 24; shift >= LAST; shift -= 8) {
+        if (threadIdx.x < 256) {
+            sh.hist[threadIdx.x] = 0;
+            sh.hist_mass[threadIdx.x] = 0;
+        }
+        __syncthreads();
+        uint32_t lo = 0, hi = row.V;
+        Row::part(lo, hi);
+        row.template each<1>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
+#pragma unroll
+            for (int e = 0; e < Row::PER; ++e) {
+                const uint32_t k = key_of(l[e]);
+                if (k < t || k <= KEY_LEAST || (!first && (k >> (shift + 8)) != prefix)) continue;
+                const uint32_t b = (k >> shift) & 255;
+                atomicAdd(&sh.hist[b], 1u);
+                if (MASS && k > t) atomicAdd(&sh.hist_mass[b], row.fixed(row.weigh(l[e])));
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            // of the scores equal to t only r are left
+            if (MASS && old.r != 0 && (first || (t >> (shift + 8)) == prefix)) sh.hist_mass[(t >> shift) & 255] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
+            // the bin of the last score kept: the lowest whose total above it is below the border
+            unsigned long long run = before, above = before;
+            uint32_t pick = 0;
+            bool any = false;
+            for (int b = 255; b >= 0; --b) {
+                if (sh.hist[b] == 0) continue;
+                if (run >= border && any) break;
+                any = true;
+                pick = b;
+                above = run;
+                run += MASS ? sh.hist_mass[b] : sh.hist[b];
+            }
+            sh.pick = pick;
+            sh.above = above;
+            sh.found = any ? sh.hist[pick] : 0;
+        }
+        __syncthreads();
+        prefix = (prefix << 8) | same(sh.pick);
+        before = same((uint64_t)sh.above);
+        found = same(sh.found);
+        first = false;
+        __syncthreads();
+    }
+    if (found == 0) return old;
+    uint32_t nt = prefix << LAST;
+    if (!(nt >> 31)) nt |= (1u << LAST) - 1u;          // a negative score: the folded bits are ones
+    Cut c{value_of(nt), 0, found};
+    const uint32_t most = nt == t ? min(found, old.r) : found;               // the border of an earlier cut
+    if (MASS) {
+        const unsigned long long w = row.fixed(row.weigh(c.t));
+        c.r = border <= before ? 1 : w == 0 ? most : (uint32_t)min((unsigned long long)most, (border - before + w - 1) / w);
+        c.r = max(c.r, 1u);
+    } else {
+        c.r = (uint32_t)min((unsigned long long)most, border - before);
+    }
+    return c;
+}
+
+// Index of the r-th (r >= 1) score equal to v.
+template <class Row>
+__device__ __attribute__((noinline)) uint32_t nth_equal(const Row r0, float v, uint32_t r)
+{
+    const Row row = r0.uniform();
+    auto &sh = Row::shared();
+    v = same(v);
+    r = same(r);
+    uint32_t lo = 0, hi = row.V, n = 0;
+    Row::part(lo, hi);
+    row.template each<4>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
+#pragma unroll
+        for (int e = 0; e < Row::PER; ++e) n += l[e] == v;
+    });
+    n = wave_total(n);
+    if (Row::lane() == 0) sh.words[Row::wave()] = n;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t k = 0; k < Row::wave(); ++k) before += sh.words[k];
+    before = same(before);
+    if (before < r && before + n >= r) {                  // this wave's part holds it
+        for (uint32_t base = lo; base < hi; base += Row::STEP) {
+            bool done = false;
+            row.step_of(base, row.load(base, hi), [&](uint32_t j, const float (&l)[Row::PER]) {
+                uint32_t c = 0;
+#pragma unroll
+                for (int e = 0; e < Row::PER; ++e) c += l[e] == v;
+                const uint32_t upto = wave_scan(c), here = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+                if (before + here >= r) {
+                    uint32_t at = before + upto - c;
+#pragma unroll
+                    for (int e = 0; e < Row::PER; ++e) {
+                        at += l[e] == v;
+                        if (l[e] == v && at == r) sh.n = j + e;
+                    }
+                    done = true;
+                }
+                before += here;
+            });
+            if (done) break;
+        }
+    }
+    __syncthreads();
+    const uint32_t at = same(sh.n);
+    __syncthreads();
+    return at;
+}
+
+// The draw among scores above `edge` and those equal to it up to index last_equal (edge = -inf: all), with weights of at least
+// `least`, which scores below `from` do not have.
+template <class Row, int THREADS>
+__device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, uint32_t last_equal, double least, float from, float u)
+{
+    constexpr int WAVES = THREADS / 64, PER = Row::PER;
+    const Row row = r0.uniform();
+    auto &sh = Row::shared();
+    edge = same(edge);
+    last_equal = same(last_equal);
+    least = same(least);
+    u = same(u);
+    const bool all = edge == -INFINITY && least == 0.0;
+    const float floor = fmaxf(fmaxf(edge, -FLT_MAX), same(from));
+    auto in = [&](float l, uint32_t j) { return l >= floor && !(l == edge && j > last_equal); };
+    auto weight = [&](float l) {
+        const double x = row.weigh(l);
+        return x >= least ? x : 0.0;
+    };
+    uint32_t lo = 0, hi = row.V;
+    double before = 0.0, target = 0.0, total = 0.0;
+    // sums of the waves' parts, the part the target falls in, its parts, ... down to one step
+    for (bool whole = true; whole || hi - lo > Row::STEP; whole = false) {
+        uint32_t a = lo, b = hi;
+        Row::part(a, b);
+        double mine = 0.0;
+        if (all) {
+            row.template each<1>(a, b, [&](uint32_t, const float (&l)[PER]) {
+#pragma unroll
+                for (int e = 0; e < PER; ++e) mine += row.weigh(l[e]);
+            });
+        } else {
+            // few scores are in: they queue up until a whole wave of them can be weighed at once
+            float *queue = sh.queue[Row::wave()];
+            uint32_t n = 0;
+            row.template each<2>(a, b, [&](uint32_t j, const float (&l)[PER]) {
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const bool is = in(l[e], j + e);
+                    const uint64_t m = __ballot(is);
+                    if (is) queue[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = l[e];
+                    n += __popcll(m);
+                    if (n >= 64) {
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        mine += weight(queue[Row::lane()]);
+                        const float rest = queue[64 + Row::lane()];
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        queue[Row::lane()] = rest;
+                        n -= 64;
+                    }
+                }
+            });
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (Row::lane() < n) mine += weight(queue[Row::lane()]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        mine = wave_total(mine);
+        if (Row::lane() == 0) sh.sums[Row::wave()] = mine;
+        __syncthreads();
+        if (whole) {
+            for (int k = 0; k < WAVES; ++k) total += sh.sums[k];
+            target = (double)u * total;
+        }
+        int pick = -1;
+        for (int k = 0; k < WAVES; ++k) {
+            if (sh.sums[k] == 0.0) continue;
+            if (pick >= 0) before += sh.sums[pick];
+            pick = k;
+            if (before + sh.sums[k] > target) break;
+        }
+        const uint32_t steps = (hi - lo + Row::STEP - 1) / Row::STEP, len = (steps + WAVES - 1) / WAVES * Row::STEP;
+        lo = same(lo + (uint32_t)pick * len);
+        hi = same((uint32_t)min((uint64_t)lo + len, (uint64_t)hi));
+        __syncthreads();
+    }
+    Drawn d;
+    row.step_of(lo, row.load(lo, hi), [&](uint32_t j, const float (&l)[PER]) {
+        double x[PER], mine = 0.0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            x[e] = in(l[e], j + e) ? weight(l[e]) : 0.0;
+            mine += x[e];
+        }
+        const double upto = before + wave_scan(mine);
+        const uint64_t some = __ballot(mine > 0.0), hit = __ballot(mine > 0.0 && upto > target);
+        const int q = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(some);
+        double run = upto - mine, drawn = 0.0;
+        uint32_t place = 0;
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            run += x[e];
+            if (!done && x[e] > 0.0) {
+                place = e;
+                drawn = x[e];
+                done = run > target;
+            }
+        }
+        d.at = (uint32_t)__builtin_amdgcn_readlane((int)(j + place), q);
+        d.prob = (float)(lane_of(drawn, q) / total);
+    });
+    return d;
+}
+
+// The nucleus of a row with none or a count cut: masses by even steps of the score, from the maximum down to where the border
+// can be; then the scores of the step it falls in.
+template <class Row, class T, int THREADS>
+__device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, float reach, const Cut o)
+{
+    constexpr int WAVES = THREADS / 64;
+    const Row row = r0.uniform();
+    auto &sh = Row::shared();
+    const Cut old{same(o.t), same(o.r), same(o.ties)};
+    top_p = same(top_p);
+    const float high = row.weigh.top, per = (float)BINS / same(reach);
+    auto bin = [&](float l) {
+        const float below = high - l;
+        return below > 0.0f ? (uint32_t)fminf(below * per, (float)(BINS - 1)) : 0u;
+    };
+    for (uint32_t b = threadIdx.x; b < BINS; b += THREADS) sh.mass[b] = 0;
+    __syncthreads();
+    uint32_t lo = 0, hi = row.V;
+    Row::part(lo, hi);
+    row.template each<1>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
+#pragma unroll
+        for (int e = 0; e < Row::PER; ++e) {
+            const unsigned long long f = row.fixed(row.weigh(l[e]));
+            if (l[e] > old.t && f) atomicAdd(&sh.mass[bin(l[e])], f);          // (of the scores equal to old.t, r are left: added below)
+        }
+    });
+    __syncthreads();
+    if (old.r != 0 && threadIdx.x == 0) sh.mass[bin(old.t)] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
+    __syncthreads();
+    // running totals of the bins
+    constexpr uint32_t EACH = BINS / THREADS;
+    unsigned long long sum = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < EACH; ++e) sum += sh.mass[threadIdx.x * EACH + e];
+    unsigned long long upto = sum;
+    for (int o1 = 1; o1 < 64; o1 <<= 1) {
+        const unsigned long long y = __shfl_up(upto, o1);
+        if ((int)Row::lane() >= o1) upto += y;
+    }
+    if (Row::lane() == 63) sh.wide[Row::wave()] = upto;
+    __syncthreads();
+    unsigned long long before = upto - sum, z = 0;
+    for (int k = 0; k < WAVES; ++k) {
+        before += k < (int)Row::wave() ? sh.wide[k] : 0;
+        z += sh.wide[k];
+    }
+    const unsigned long long border = same((uint64_t)ceil((double)top_p * (double)z));
+    if (before < border && border <= before + sum) {
+        uint32_t b = threadIdx.x * EACH;
+        while (before + sh.mass[b] < border) before += sh.mass[b++];
+        sh.pick = b;
+        sh.above = before;
+    }
+    __syncthreads();
+    const uint32_t at_bin = same(sh.pick);
+    const unsigned long long above = same((uint64_t)sh.above);
+    // (half a bin to spare on either side: the exact answer is bin()'s)
+    const float step = 1.0f / per, most = high - ((float)at_bin - 0.5f) * step;
+    const float least = at_bin + 1 < BINS ? high - ((float)at_bin + 1.5f) * step : -FLT_MAX;
+    if (old.r != 0 || !row.collect(least, most, [&](float l) { return bin(l) == at_bin; })) return radix_cut<Row, T, THREADS, true>(row, border, old);
+    if (threadIdx.x < 64) {
+        const double room = (double)(border - above) * __longlong_as_double((long long)(1023 - row.s) << 52);
+        const Cut c = sh.n <= 256 ? list_cut<Row, 4>(row, room) : list_cut<Row, 8>(row, room);
+        if (threadIdx.x == 0) {
+            sh.t = c.t;
+            sh.pick = c.r;
+            sh.found = c.ties;
+        }
+    }
+    __syncthreads();
+    const Cut c{same(sh.t), same(sh.pick), same(sh.found)};
+    __syncthreads();
+    return c;
+}
 
 template <class T, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
 {
     using Row = BlockRow<T, THREADS, VEC>;
-    constexpr int WAVES = THREADS / 64;
-    __shared__ typename Row::Shared sh;
+    auto &sh = Row::shared();
     for (uint64_t i = blockIdx.x; i < a.N; i += gridDim.x) {
-        Row row{sh, (const T *)a.S + i * a.ld, a.V, a.mass_bits, {}};
+        Row row{(uint64_t)((const T *)a.S + i * a.ld), a.V, a.mass_bits, Weigh()};
         const RowParams p(a, i);
-        uint32_t at = 0, mine;
-        float prob = 0.0f;
-        const uint32_t top = row.find_top(mine);
-        row.weigh = Weigh{top, (double)value_of(top), 1.0 / (double)p.temperature};
-        if (top > KEY_LEAST && p.greedy) {
-            at = row.nth_equal(top, 1);
-            prob = 1.0f;
-        } else if (top > KEY_LEAST) {
-            uint32_t t = KEY_LEAST, r = 0, ties = 0;
+        Drawn d{0, 0.0f};
+        float mine;
+        const float top = row.find_top(mine);
+        row.weigh = Weigh(top, p.temperature);
+        if (top > -INFINITY && p.greedy) {
+            d = Drawn{nth_equal(row, top, 1), 1.0f};
+        } else if (top > -INFINITY) {
+            Cut c{-INFINITY, 0, 0};
             bool done = false;
             if (p.top_k > 0 && p.top_k < a.V) {
                 // The k-th largest of the lanes' own maxima: at least k scores reach it, and few more do, since the largest
                 // scores rarely share a lane.
                 if (p.top_k <= (THREADS < 1024 ? THREADS / 2 : 256)) {
-                    const uint32_t least = max(row.kth_largest(mine, p.top_k), KEY_LEAST + 1);
-                    if (row.collect([&](uint32_t k) { return k >= least; })) {
-                        if (threadIdx.x < 64) {
-                            if (sh.n <= 256)
-                                row.template draw_from_list<4>(p, at, prob);
-                            else
-                                row.template draw_from_list<8>(p, at, prob);
-                        }
+                    const uint32_t least = max(row.kth_largest(key_of(mine), p.top_k), KEY_LEAST + 1);
+                    if (row.collect(value_of(least), INFINITY, [](float) { return true; })) {
+                        if (threadIdx.x < 64) d = sh.n <= 256 ? list_draw<Row, 4>(row, p) : list_draw<Row, 8>(row, p);
                         done = true;
                     }
                 }
-                if (!done) row.template cut<false>(p.top_k, t, r, ties);
+                if (!done) c = radix_cut<Row, T, THREADS, false>(row, p.top_k, c);
             }
             if (!done) {
-                if (p.top_p < 1.0f) {
-                    // masses by even steps of the score from the maximum down.  All scores more than ln(V / (1 - p)) below it (in
-                    // units of T) together weigh less than 1 - p, so the border lies above: that is where the steps are.
-                    const float reach = (logf((float)a.V) - logf(fmaxf(1.0f - p.top_p, 0x1p-24f)) + 1.0f) * p.temperature;
-                    const float per = (float)BINS / reach, high = value_of(top);
-                    auto bin = [&](uint32_t k) {
-                        const float below = high - value_of(k);
-                        return below > 0.0f ? (uint32_t)fminf(below * per, (float)(BINS - 1)) : 0u;
-                    };
-                    for (uint32_t b = threadIdx.x; b < BINS; b += THREADS) sh.mass[b] = 0;
-                    __syncthreads();
-                    uint32_t lo = 0, hi = a.V;
-                    row.part(lo, hi);
-                    row.template each<1>(lo, hi, [&](uint32_t, const uint32_t (&k)[Row::PER]) {
-#pragma unroll
-                        for (int e = 0; e < Row::PER; ++e) {
-                            if (k[e] <= t) continue;                       // (of the scores equal to t, r are left: added below)
-                            const unsigned long long f = row.fixed(row.weigh(k[e]));
-                            if (f) atomicAdd(&sh.mass[bin(k[e])], f);
-                        }
-                    });
-                    __syncthreads();
-                    if (r != 0 && threadIdx.x == 0) sh.mass[bin(t)] += (unsigned long long)r * row.fixed(row.weigh(t));
-                    __syncthreads();
-                    // running totals of the bins
-                    constexpr uint32_t EACH = BINS / THREADS;
-                    unsigned long long sum = 0;
-#pragma unroll
-                    for (uint32_t e = 0; e < EACH; ++e) sum += sh.mass[threadIdx.x * EACH + e];
-                    unsigned long long upto = sum;
-                    for (int o = 1; o < 64; o <<= 1) {
-                        const unsigned long long y = __shfl_up(upto, o);
-                        if ((int)row.lane() >= o) upto += y;
-                    }
-                    if (row.lane() == 63) sh.wide[row.wave()] = upto;
-                    __syncthreads();
-                    unsigned long long before = upto - sum, z = 0;
-                    for (int k = 0; k < WAVES; ++k) {
-                        before += k < (int)row.wave() ? sh.wide[k] : 0;
-                        z += sh.wide[k];
-                    }
-                    const unsigned long long border = (unsigned long long)ceil((double)p.top_p * (double)z);
-                    if (before < border && border <= before + sum) {
-                        uint32_t b = threadIdx.x * EACH;
-                        while (before + sh.mass[b] < border) before += sh.mass[b++];
-                        sh.t = b;
-                        sh.above = before;
-                    }
-                    __syncthreads();
-                    const uint32_t at_bin = sh.t;
-                    const unsigned long long above = sh.above;
-                    const bool listed = r == 0 && row.collect([&](uint32_t k) { return k > KEY_LEAST && bin(k) == at_bin; });
-                    if (listed) {
-                        if (threadIdx.x < 64) {
-                            const double room = (double)(border - above) * __longlong_as_double((long long)(1023 - a.mass_bits) << 52);
-                            uint32_t t1, r1, n1;
-                            if (sh.n <= 256)
-                                row.template cut_list<4>(room, t1, r1, n1);
-                            else
-                                row.template cut_list<8>(room, t1, r1, n1);
-                            if (threadIdx.x == 0) {
-                                sh.t = t1;
-                                sh.r = r1;
-                                sh.ties = n1;
-                            }
-                        }
-                        __syncthreads();
-                        t = sh.t;
-                        r = sh.r;
-                        ties = sh.ties;
-                    } else {
-                        row.template cut<true>(border, t, r, ties);
-                    }
-                }
-                uint32_t last_equal = a.V;
-                if (t > KEY_LEAST && r < ties) last_equal = row.nth_equal(t, r);
-                __syncthreads();
-                row.draw(t, last_equal, p.min_p > 0.0f ? (double)fminf(p.min_p, 1.0f) : 0.0, p.u, at, prob);
+                if (p.top_p < 1.0f) c = mass_cut<Row, T, THREADS>(row, p.top_p, p.reach(a.V), c);
+                const uint32_t last_equal = c.r < c.ties ? nth_equal(row, c.t, c.r) : a.V;
+                // scores this far below the maximum miss min_p whatever the rounding
+                const double least = p.min_p > 0.0f ? (double)fminf(p.min_p, 1.0f) : 0.0;
+                const float from = p.min_p > 0.0f && top < INFINITY ? top + p.temperature * (__logf((float)least) * 1.001f - 0.001f) : -INFINITY;
+                d = row_draw<Row, THREADS>(row, c.t, last_equal, least, from, p.u);
             }
         }
         if (threadIdx.x == 0) {
-            a.idx[i] = at;
-            if (a.prob) a.prob[i] = prob;
+            a.idx[i] = d.at;
+            if (a.prob) a.prob[i] = d.prob;
         }
         __syncthreads();
     }
