@@ -260,8 +260,11 @@ int vqhip_assign_matched_f64(vqhip_ctx *ctx, const double *X, const uint32_t *y,
  * What a program does around the search once prototypes are a codebook: draw a code per sample instead of taking the
  * nearest, turn codes back into vectors, and train the table from the gradient of those vectors.  No counterpart in the
  * reference beyond reading `prototypes[idx]` (src/glvq/glvq.rs:231).  All calls take device memory and enqueue on `stream`
- * without host synchronisation; none allocates, none keeps anything in the context, so they may be captured into a HIP graph,
- * and calls that overlap are independent as long as their outputs and workspaces are.  Rows of a matrix lie `ld` elements
+ * without host synchronisation; none allocates or keeps anything between calls, so they may be captured into a HIP graph, and
+ * calls that overlap are independent as long as their outputs and workspaces are.  The one exception: with prototypes of more
+ * than 32 values the first vqhip_scores_device or vqhip_assign_sampled_device call after vqhip_set_prototypes lays them out for
+ * the matrix cores (6 bytes per value) and waits for that; under capture that first call is VQHIP_ERR_STATE.  A captured call
+ * reads the model where it lay: no vqhip_set_* between capture and replay.  Rows of a matrix lie `ld` elements
  * apart (ld >= its width); what lies between them is neither read nor written.  Outputs must not overlap inputs.  The device
  * current on the calling thread stays current. */
 typedef enum { VQHIP_F32 = 0, VQHIP_BF16 = 1, VQHIP_F16 = 2 } vqhip_dtype;

@@ -523,10 +523,11 @@ def test_c_refusals(ctx):
 @pytest.mark.parametrize("N,D,K", [(1, 33, 1), (64, 128, 256), (33, 784, 100), (129, 255, 127), (2, 1000, 513), (130, 64, 129), (65, 100, 70), (300, 128, 256), (20, 785, 33), (4100, 40, 2100), (2048, 36, 4096)])
 @pytest.mark.parametrize("offset", [0.0, 100.0])
 def test_scores_in_the_expanded_form(ctx, N, D, K, offset):
-    """Rows of more than 32 values: distances not below 1/8 of B = |x - c|^2 + |w - c|^2 come from B - 2 (x - c).(w - c).  Its
+    """Rows of more than 32 values: distances not below 1/16 of B = |x - c|^2 + |w - c|^2 come from B - 2 (x - c).(w - c).  Its
     roundings, with e = 2^-24: each centred value 1 e of itself, which moves the distance by at most 2 sqrt(dist) e (|x - c| + |w - c|)
     <= 4 e B; each norm a sum of D squares, D e of itself, together D e B; the product a chain of D terms whose absolute
-    values sum to at most B / 2, doubled D e B; the two last additions 2 e B.  (2 D + 6) e B <= 8 (2 D + 6) e dist."""
+    values sum to at most B / 2, doubled D e B; the two last additions 2 e B.  (2 D + 6) e B <= 16 (2 D + 6) e dist;
+    the tests hold it to half of that."""
     g = gen(N + D)
     W = torch.rand(K, D, generator=g) * 2 - 1 + offset
     X = W[torch.randint(K, (N,), generator=g)] + 0.1 * torch.randn(N, D, generator=g)

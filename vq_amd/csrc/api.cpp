@@ -76,6 +76,7 @@ struct vqhip_ctx {
     std::vector<uint32_t> hcls;
 
     float *dW = nullptr;       // K x D, and one row more: their mean
+    void *dScoreImg = nullptr; // the prototypes laid out for vqhip_scores_device (rows above 32 values), made by its first call
     double *dW64 = nullptr;    // K x D in the reference's own number type (f64 entry points only)
     uint32_t *dcls = nullptr;  // K
     float *dOm = nullptr;      // M x D  or  K x M x D
@@ -887,6 +888,7 @@ try {
     drop_engine(c);
     free_omega(c);
     (void)hipFree(c->dW);
+    (void)hipFree(c->dScoreImg);
     (void)hipFree(c->dW64);
     free_f64(c);
     (void)hipFree(c->dcls);
@@ -919,6 +921,8 @@ try {
     c->hcls.clear();
     (void)hipFree(c->dW64);
     c->dW64 = nullptr;
+    (void)hipFree(c->dScoreImg);
+    c->dScoreImg = nullptr;
     c->hW.assign(W, W + (size_t)K * D);
     c->K = K;
     c->D = D;
@@ -1317,6 +1321,27 @@ int check_sampling(vqhip_ctx *c, const vqhip_sampling *how)
     return VQHIP_OK;
 }
 
+// The layout of the prototypes that scores of longer rows read: made (and waited for) by the first call that needs it.
+int prepare_scores(vqhip_ctx *c, hipStream_t s)
+{
+    const size_t bytes = scores_image_bytes(c->K, c->D);
+    if (bytes == 0 || c->dScoreImg) return VQHIP_OK;
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    HIPCHK(c, hipStreamIsCapturing(s, &capture));
+    if (capture != hipStreamCaptureStatusNone)
+        return c->fail(VQHIP_ERR_STATE, "scores: call once after vqhip_set_prototypes and before the capture");
+    void *img = nullptr;
+    HIPCHK(c, hipMalloc(&img, bytes));
+    hipError_t e = launch_scores_image(c->dW, c->dW + (size_t)c->K * c->D, c->K, c->D, img, s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    if (e != hipSuccess) {
+        (void)hipFree(img);
+        return c->fail_hip(e, "scores image");
+    }
+    c->dScoreImg = img;
+    return VQHIP_OK;
+}
+
 constexpr uint64_t SAMPLED_CHUNK_BYTES = 128ull << 20;      // scores of one chunk: half the last-level cache
 
 }  // namespace
@@ -1332,7 +1357,8 @@ try {
     if (const char *why = check_matrix(dS, N, c->K, lds, 4)) return c->fail(VQHIP_ERR_INVALID, std::string("scores_device: ") + why);
     OnDevice on(c->device);
     HIPCHK(c, on.error());
-    HIPCHK(c, launch_scores(dX, N, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->K, dS, lds, (hipStream_t)stream));
+    if ((rc = prepare_scores(c, (hipStream_t)stream)) != VQHIP_OK) return rc;
+    HIPCHK(c, launch_scores(dX, N, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->dScoreImg, c->K, dS, lds, (hipStream_t)stream));
     return VQHIP_OK;
 }
 VQHIP_CATCH(c)
@@ -1384,6 +1410,7 @@ try {
     OnDevice on(c->device);
     HIPCHK(c, on.error());
     const hipStream_t s = (hipStream_t)stream;
+    if ((rc = prepare_scores(c, s)) != VQHIP_OK) return rc;
     for (uint64_t off = 0; off < N; off += chunk) {
         const uint64_t n = std::min(chunk, N - off);
         vqhip_sampling h = *how;
@@ -1391,7 +1418,7 @@ try {
         if (h.dtop_p) h.dtop_p += off;
         if (h.dmin_p) h.dmin_p += off;
         if (h.dtop_k) h.dtop_k += off;
-        HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->K, (float *)dwork, c->K, s));
+        HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->dScoreImg, c->K, (float *)dwork, c->K, s));
         HIPCHK(c, launch_sample(dwork, VQHIP_F32, n, c->K, c->K, h, du + off, didx_out + off, dprob_out ? dprob_out + off : nullptr, s));
     }
     return VQHIP_OK;

@@ -27,6 +27,9 @@ struct ScoreArgs {
     float *S;
     uint64_t N, ld;
     uint32_t K, D;
+    const uint32_t *img;              // k_scores_image: the prototypes' pieces, then their norms
+    const float *norms;
+    uint32_t blocks;                  // of 64 prototypes
     uint32_t colTiles;
     int vecX, vecW, vecS, vecC;       // rows may be moved 16 bytes at a time
 };
@@ -128,8 +131,11 @@ __global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs
 
 // ---------------------------------------------------------------------------------------------- matrix cores
 constexpr uint32_t DIRECT_D = 32;     // rows up to this length: k_scores_direct
-constexpr float CLOSE = 0.125f;       // of |x - c|^2 + |w - c|^2; distances below it are measured directly
-constexpr int MF_THREADS = 256, MF_K = 16;
+// Of |x - c|^2 + |w - c|^2; distances below it are measured directly.  The products' error is a few 2^-24 of the norms, so at 1/16
+// a distance is within a few 1e-6 of itself (the bar of this library is 1e-5); at 1/8 the samples of a codebook would take
+// their own prototype's way through the direct form too, 45 us more on 500k x 128 against 256.
+constexpr float CLOSE = 0.0625f;
+constexpr int MF_K = 16;
 
 // The sum over 16 consecutive lanes, in the last of them
 __device__ __forceinline__ float row_sum(float v)
@@ -142,148 +148,231 @@ __device__ __forceinline__ float row_sum(float v)
     return v;
 }
 
-// A workgroup: 64 R x 64 R scores, a wave 32 R x 32 R of them in R x R accumulators of v_mfma_f32_32x32x16_bf16.  A operand: lane
-// l holds sample l & 31, B operand: prototype l & 31; lanes 0-31 the reduction values 0 .. 7 of a step, lanes 32-63 8 .. 15.
-// Result: lane l holds prototype l & 31 and samples 8 g + 4 (l >> 5) + e.
-// LDS: a piece of a row is 16 bf16 = two 16-byte halves, swapped in every other group of 8 rows, so that 16 lanes reading the same
-// half of 16 rows touch 16 different 16-byte slots of the 64 banks.
-template <int R>
-__global__ void __launch_bounds__(MF_THREADS, 2) k_scores_mfma(const ScoreArgs a)
+// The prototypes as the matrix cores read them, made once per model: per step of 16 reduction values and block of 64 prototypes
+// three pieces of 64 rows of 16 bf16 (6 KiB, what a workgroup copies to LDS as it is), zero behind the last prototype and
+// value.  A row of a piece is two 16-byte halves, swapped in every other group of 8 rows, so that 16 lanes reading the same half
+// of 16 rows touch 16 different 16-byte slots of the 64 banks.
+constexpr uint32_t IMG_BLOCK = 3 * 64 * 8;             // dwords
+constexpr uint32_t IMG_PAD = 256;                      // prototypes the image is filled up to a multiple of: the widest tile
+
+__device__ __forceinline__ int piece_slot(int row, int quad) { return (((quad >> 1) ^ (row >> 3)) & 1) * 4 + (quad & 1) * 2; }
+inline uint32_t image_blocks(uint32_t K) { return (uint32_t)(((uint64_t)K + IMG_PAD - 1) / IMG_PAD * (IMG_PAD / 64)); }
+
+__global__ void __launch_bounds__(256) k_scores_image(const float *W, const float *C, uint32_t K, uint32_t D, uint32_t blocks, uint32_t *img)
 {
-    constexpr int TILE = 64 * R, WT = 32 * R;
-    __shared__ __attribute__((aligned(16))) uint32_t lds[2][2][3][TILE][8];        // samples, prototypes; two buffers; three pieces
-    auto &lx = lds[0], &lw = lds[1];
-    __shared__ __attribute__((aligned(16))) float nx[TILE], nw[TILE];
+    const uint32_t block = blockIdx.x % blocks, step = blockIdx.x / blocks;
+    const int row = threadIdx.x >> 2, quad = threadIdx.x & 3;
+    const uint32_t k = block * 64 + row, d = step * MF_K + quad * 4;
+    const float4 w = load4(W, k, k < K, D, d, 0), c = load4(C, 0, k < K, D, d, 0);
+    uint32_t p[3], q[3];
+    split3(w.x - c.x, w.y - c.y, p[0], p[1], p[2]);
+    split3(w.z - c.z, w.w - c.w, q[0], q[1], q[2]);
+    uint32_t *to = img + ((size_t)step * blocks + block) * IMG_BLOCK + row * 8 + piece_slot(row, quad);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *(uint2 *)(to + i * 64 * 8) = make_uint2(p[i], q[i]);
+}
+
+// |w - c|^2, a wave per prototype; 0 behind the last
+__global__ void __launch_bounds__(64) k_scores_norms(const float *W, const float *C, uint32_t K, uint32_t D, float *norms)
+{
+    const uint32_t k = blockIdx.x;
+    float s = 0.0f;
+    if (k < K)
+        for (uint32_t d = threadIdx.x; d < D; d += 64) {
+            const float e = W[(size_t)k * D + d] - C[d];
+            s = fmaf(e, e, s);
+        }
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (threadIdx.x == 0) norms[k] = s;
+}
+
+// A workgroup of WR x WC waves, a wave 32 RW x 32 CW scores in RW x CW accumulators of v_mfma_f32_32x32x16_bf16.  A operand: lane l
+// holds sample l & 31, B operand: prototype l & 31; lanes 0-31 the reduction values 0 .. 7 of a step, lanes 32-63 8 .. 15.
+// Result: lane l holds prototype l & 31 and samples 8 g + 4 (l >> 5) + e.  The samples are centred and split on their way to LDS;
+// both operands are double buffered there.
+constexpr uint32_t CLOSE_LIST = 512;                   // close pairs a wave measures one by one at most; more: its whole tile
+
+template <int RW, int CW, int WR, int WC, int PER_SIMD, bool VEC>
+__global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const ScoreArgs a)
+{
+    constexpr int THREADS = WR * WC * 64, TM = 32 * RW * WR, TN = 32 * CW * WC, MT = 32 * RW, NT = 32 * CW;
+    constexpr int XROWS = THREADS / 4, XPARTS = TM / XROWS;                         // staging: 4 lanes a sample
+    constexpr int COPY = TN / 64 * (int)IMG_BLOCK / 4, COPIES = (COPY + THREADS - 1) / THREADS;     // 16-byte pieces of the image
+    static_assert(TM % XROWS == 0 && TM % 64 == 0 && TN % 64 == 0, "whole blocks of 64 rows");
+    constexpr int XSTAGE = TM * 3 * 8, WSTAGE = TN * 3 * 8;
+    __shared__ __attribute__((aligned(16))) uint32_t lx[2][XSTAGE], lw[2][WSTAGE];
+    __shared__ __attribute__((aligned(16))) float nx[TM], nw[TN];
+    __shared__ uint16_t lists[WR * WC][CLOSE_LIST];
     // workgroups are dealt to the 8 XCDs in turn: each takes a consecutive share of the tiles, so that the column tiles of the same
     // samples meet in one L2
     const uint32_t share = (gridDim.x + 7) / 8, tile = blockIdx.x % 8 * share + blockIdx.x / 8;
-    const uint64_t row0 = (uint64_t)(tile / a.colTiles) * TILE;
-    const uint32_t col0 = tile % a.colTiles * TILE;
+    const uint64_t row0 = (uint64_t)(tile / a.colTiles) * TM;
+    const uint32_t col0 = tile % a.colTiles * TN;
     if (row0 >= a.N) return;
-    const int t = threadIdx.x, lane = t & 63, half = lane >> 5, l31 = lane & 31, wr = t >> 7, wc = (t >> 6) & 1;
-    const int sr = t >> 2, sd = (t & 3) * 4;          // staging: values sd .. + 3 of rows sr, sr + 64
-    const int slot = ((((t & 3) >> 1) ^ (sr >> 3)) & 1) * 4 + (t & 1) * 2;       // ... and where they go, in dwords of the row's piece
-    const int swap = (half ^ (l31 >> 3)) & 1;         // which slot this lane reads
+    const int t = threadIdx.x, lane = t & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave / WC, wc = wave % WC;
+    const int sr = t >> 2, sd = (t & 3) * 4;          // staging: values sd .. + 3 of rows sr, sr + XROWS, ...
+    const int slot = piece_slot(sr, t & 3);           // ... and where they go, in dwords of the row's piece
+    const int swap = ((half ^ (l31 >> 3)) & 1) * 4;   // which half of a row's piece this lane reads
+    const u32x4 *img = (const u32x4 *)(a.img + (size_t)(col0 / 64) * IMG_BLOCK);
+    const size_t imgStep = (size_t)a.blocks * (IMG_BLOCK / 4);
 
-    float4 px[R], pw[R], pc;
-    float sx[R], sw[R];
+    const uint32_t steps = (a.D + MF_K - 1) / MF_K;
+
+    // Samples are requested PREFETCH steps ahead of their use (HBM), the image one (L2), and the image first: loads are waited for
+    // in the order of their issue.  None of them is conditional (a count of loads on their way that depends on a branch is
+    // waited for as a whole): what lies behind the last sample or value is read inside instead, and dropped.
+    constexpr int PREFETCH = 2;
+    float4 px[PREFETCH][XPARTS], pc;
+    u32x4 pw[COPIES];
+    float sx[XPARTS];
+    const float *xrow[XPARTS];
 #pragma unroll
-    for (int i = 0; i < R; ++i) sx[i] = sw[i] = 0.0f;
-    auto fetch = [&](uint32_t d) {
-        pc = load4(a.C, 0, true, a.D, d + sd, a.vecC);
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const uint64_t r = row0 + sr + 64 * i;
-            const uint32_t c = col0 + sr + 64 * i;
-            px[i] = load4(a.X, r, r < a.N, a.D, d + sd, a.vecX);
-            pw[i] = load4(a.W, c, c < a.K, a.D, d + sd, a.vecW);
-        }
+    for (int i = 0; i < XPARTS; ++i) {
+        sx[i] = 0.0f;
+        xrow[i] = a.X + min(row0 + sr + XROWS * i, a.N - 1) * a.D;
+    }
+    auto values = [&](const float *row, uint32_t step) -> float4 {
+        const uint32_t d = step * MF_K + sd;
+        if constexpr (VEC) return *(const float4 *)(row + min(d, a.D - 4));
+        return make_float4(row[min(d, a.D - 1)], row[min(d + 1, a.D - 1)], row[min(d + 2, a.D - 1)], row[min(d + 3, a.D - 1)]);
     };
-    auto put = [&](uint32_t (&to)[3][TILE][8], int row, const float4 &v) {
-        uint32_t p[3], q[3];
-        split3(v.x, v.y, p[0], p[1], p[2]);
-        split3(v.z, v.w, q[0], q[1], q[2]);
+    auto samples = [&](int u, uint32_t step) {
 #pragma unroll
-        for (int c = 0; c < 3; ++c) *(uint2 *)&to[c][row][slot] = make_uint2(p[c], q[c]);
+        for (int i = 0; i < XPARTS; ++i) px[u][i] = values(xrow[i], step);
     };
-    auto stage = [&](int b) {
+    auto fetch = [&](uint32_t step) {
+        pc = values(a.C, step);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const float4 x = make_float4(px[i].x - pc.x, px[i].y - pc.y, px[i].z - pc.z, px[i].w - pc.w);
-            const float4 w = make_float4(pw[i].x - pc.x, pw[i].y - pc.y, pw[i].z - pc.z, pw[i].w - pc.w);
+        for (int i = 0; i < COPIES; ++i) pw[i] = img[COPY % THREADS == 0 ? t + i * THREADS : min(t + i * THREADS, COPY - 1)];
+        if (step + 1 < steps) img += imgStep;
+    };
+    auto stage = [&](int b, int u, uint32_t step) {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i)
+            if (COPY % THREADS == 0 || t + i * THREADS < COPY) *(u32x4 *)&lw[b][4 * (t + i * THREADS)] = pw[i];
+#pragma unroll
+        for (int i = 0; i < XPARTS; ++i) {
+            const float4 v = px[u][i];
+            float4 x = make_float4(v.x - pc.x, v.y - pc.y, v.z - pc.z, v.w - pc.w);
+            if ((step + 1) * MF_K > a.D) {
+                const uint32_t d = step * MF_K + sd;
+                x = make_float4(d < a.D ? x.x : 0.0f, d + 1 < a.D ? x.y : 0.0f, d + 2 < a.D ? x.z : 0.0f, d + 3 < a.D ? x.w : 0.0f);
+            }
             sx[i] = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, fmaf(x.w, x.w, sx[i]))));
-            sw[i] = fmaf(w.x, w.x, fmaf(w.y, w.y, fmaf(w.z, w.z, fmaf(w.w, w.w, sw[i]))));
-            put(lx[b], sr + 64 * i, x);
-            put(lw[b], sr + 64 * i, w);
+            uint32_t p[3], q[3];
+            split3(x.x, x.y, p[0], p[1], p[2]);
+            split3(x.z, x.w, q[0], q[1], q[2]);
+            const int row = sr + XROWS * i;
+#pragma unroll
+            for (int c = 0; c < 3; ++c) *(uint2 *)&lx[b][((row / 64 * 3 + c) * 64 + row % 64) * 8 + slot] = make_uint2(p[c], q[c]);
         }
     };
-    f32x16 acc[R][R];
+    // (both operands lie as blocks of 64 rows, three pieces each)
+    auto piece = [&](const uint32_t *l, int row, int c) { return *(const u32x4 *)&l[((row / 64 * 3 + c) * 64 + row % 64) * 8 + swap]; };
+    f32x16 acc[RW][CW];
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < RW; ++i)
 #pragma unroll
-        for (int j = 0; j < R; ++j)
+        for (int j = 0; j < CW; ++j)
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
 
     fetch(0);
-    stage(0);
+#pragma unroll
+    for (int u = 0; u < PREFETCH; ++u) samples(u, u);
+    stage(0, 0, 0);
+    fetch(min(1u, steps - 1));
+    samples(0, PREFETCH);
     __syncthreads();
-    int b = 0;
-    for (uint32_t d = 0; d < a.D; d += MF_K, b ^= 1) {
-        const bool more = d + MF_K < a.D;
-        if (more) fetch(d + MF_K);
-        u32x4 fx[R][3], fw[R][3];
+    for (uint32_t k0 = 0; k0 < steps; k0 += PREFETCH) {
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int u = 0; u < PREFETCH; ++u) {
+            const uint32_t k = k0 + u;
+            if (k >= steps) break;
+            const int b = u & 1, next = (u + 1) % PREFETCH;
+            u32x4 fx[RW][3];
 #pragma unroll
-            for (int c = 0; c < 3; ++c) {
-                fx[i][c] = *(const u32x4 *)&lx[b][c][wr * WT + i * 32 + l31][swap * 4];
-                fw[i][c] = *(const u32x4 *)&lw[b][c][wc * WT + i * 32 + l31][swap * 4];
+            for (int i = 0; i < RW; ++i)
+#pragma unroll
+                for (int c = 0; c < 3; ++c) fx[i][c] = piece(lx[b], wr * MT + i * 32 + l31, c);
+#pragma unroll
+            for (int j = 0; j < CW; ++j) {
+                u32x4 fw[3];
+#pragma unroll
+                for (int c = 0; c < 3; ++c) fw[c] = piece(lw[b], wc * NT + j * 32 + l31, c);
+                // the six products that matter, the smallest first
+                constexpr int PX[6] = {2, 0, 1, 1, 0, 0}, PW[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+                for (int p = 0; p < 6; ++p)
+#pragma unroll
+                    for (int i = 0; i < RW; ++i) acc[i][j] = mma_bf(fx[i][PX[p]], fw[PW[p]], acc[i][j]);
             }
-        // the six products that matter, the smallest first
-        constexpr int PX[6] = {2, 0, 1, 1, 0, 0}, PW[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-        for (int p = 0; p < 6; ++p)
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-#pragma unroll
-                for (int j = 0; j < R; ++j) acc[i][j] = mma_bf(fx[i][PX[p]], fw[j][PW[p]], acc[i][j]);
-        if (more) stage(b ^ 1);
-        __syncthreads();
-    }
-    // the norms: 4 lanes hold the parts of a row
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        float x = sx[i], w = sw[i];
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            x += __shfl_xor(x, o);
-            w += __shfl_xor(w, o);
-        }
-        if ((t & 3) == 0) {
-            nx[sr + 64 * i] = x;
-            nw[sr + 64 * i] = w;
+            if (k + 1 < steps) {
+                stage(b ^ 1, next, k + 1);
+                fetch(k + 2);
+                samples(next, k + 1 + PREFETCH);
+            }
+            __syncthreads();
         }
     }
+    // the samples' norms: 4 lanes hold the parts of a row
+#pragma unroll
+    for (int i = 0; i < XPARTS; ++i) {
+        float x = sx[i];
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) x += __shfl_xor(x, o);
+        if ((t & 3) == 0) nx[sr + XROWS * i] = x;
+    }
+    for (int q = t; q < TN; q += THREADS) nw[q] = a.norms[col0 + q];
     __syncthreads();
 
-    // scores, and this wave's list of close pairs (sample << 8 | prototype, inside its tile) in the staging memory
-    uint16_t *list = (uint16_t *)&lds[0][0][0][0][0] + (t >> 6) * (WT * WT);
-    static_assert(sizeof lds >= 4 * WT * WT * sizeof(uint16_t), "a list of all pairs of the four waves fits");
+    // scores, and this wave's list of close pairs (sample << 8 | prototype, inside its tile)
+    uint16_t *list = lists[wave];
+    const uint64_t wrow = row0 + wr * MT;
+    const uint32_t wcol = col0 + wc * NT;
     uint32_t n = 0;
-    const bool inside = row0 + TILE <= a.N && col0 + TILE <= a.K;
-    float *const out = a.S + (row0 + wr * WT) * a.ld + col0 + wc * WT;
+    auto finish = [&](auto bounded) {
+        float *const out = a.S + wrow * a.ld + wcol;
+        const uint32_t at = (uint32_t)(4 * half * a.ld) + l31;
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-        const uint32_t lc = j * 32 + l31;
-        const float w2 = nw[wc * WT + lc];
+        for (int j = 0; j < CW; ++j) {
+            const float w2 = nw[wc * NT + j * 32 + l31];
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+            for (int i = 0; i < RW; ++i)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const uint32_t lr0 = i * 32 + 8 * g + 4 * half;
-                const float4 x2 = *(const float4 *)&nx[wr * WT + lr0];
-                const float fx2[4] = {x2.x, x2.y, x2.z, x2.w};
+                for (int g = 0; g < 4; ++g) {
+                    const float4 x2 = *(const float4 *)&nx[wr * MT + i * 32 + 8 * g + 4 * half];
+                    const float fx2[4] = {x2.x, x2.y, x2.z, x2.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t lr = lr0 + e;
-                    const float both = fx2[e] + w2, s = fmaf(2.0f, acc[i][j][4 * g + e], -both);
-                    const bool on = inside || (row0 + wr * WT + lr < a.N && col0 + wc * WT + lc < a.K);
-                    const bool close = on && !(-s >= CLOSE * both);               // (also where anything is not finite)
-                    if (on && !close) out[lr * a.ld + lc] = s;
-                    const uint64_t m = __ballot(close);
-                    if (m) {
-                        if (close) list[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(lr << 8 | lc);
-                        n += __popcll(m);
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t lr = i * 32 + 8 * g + 4 * half + e, lc = j * 32 + l31;
+                        const float both = fx2[e] + w2, s = fmaf(2.0f, acc[i][j][4 * g + e], -both);
+                        float *const to = out + (size_t)(i * 32 + 8 * g + e) * a.ld + j * 32;
+                        const bool on = !decltype(bounded)::value || (wrow + lr < a.N && wcol + lc < a.K);
+                        const bool far = s <= -CLOSE * both;                          // (not so where anything is not finite)
+                        const uint64_t m = __ballot(!far);
+                        if (m == 0) {
+                            if (on) to[at] = s;
+                        } else {
+                            if (on && far) to[at] = s;
+                            const uint64_t c = __ballot(on && !far);
+                            const uint32_t q = n + __popcll(c & ((1ull << lane) - 1));
+                            if (on && !far && q < CLOSE_LIST) list[q] = (uint16_t)(lr << 8 | lc);
+                            n += __popcll(c);
+                        }
                     }
                 }
-            }
-    }
+        }
+    };
+    if (row0 + TM <= a.N && col0 + TN <= a.K)
+        finish(std::false_type());
+    else
+        finish(std::true_type());
     if (n == 0) return;
-    const uint64_t wrow = row0 + wr * WT;
-    const uint32_t wcol = col0 + wc * WT;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (n <= WT * WT / 32) {
+    if (n <= MT * NT / 32) {
+        static_assert(MT * NT / 32 <= (int)CLOSE_LIST, "the pairs measured one by one are all in the list");
         // 16 lanes a pair, two pairs at a time
         const uint32_t g = lane >> 4, gl = lane & 15;
         for (uint32_t p = g; p < n; p += 8) {
@@ -292,13 +381,22 @@ __global__ void __launch_bounds__(MF_THREADS, 2) k_scores_mfma(const ScoreArgs a
             const float *x0 = a.X + (wrow + (q0 >> 8)) * a.D, *w0 = a.W + (uint64_t)(wcol + (q0 & 255)) * a.D;
             const float *x1 = a.X + (wrow + (q1 >> 8)) * a.D, *w1 = a.W + (uint64_t)(wcol + (q1 & 255)) * a.D;
             float s0 = 0.0f, s1 = 0.0f;
-            for (uint32_t d = gl * 4; d < a.D; d += 64) {
-                const float4 u0 = load4(x0, 0, true, a.D, d, a.vecX), v0 = load4(w0, 0, true, a.D, d, a.vecW);
-                const float4 u1 = load4(x1, 0, true, a.D, d, a.vecX), v1 = load4(w1, 0, true, a.D, d, a.vecW);
-                const float e0 = u0.x - v0.x, e1 = u0.y - v0.y, e2 = u0.z - v0.z, e3 = u0.w - v0.w;
-                const float f0 = u1.x - v1.x, f1 = u1.y - v1.y, f2 = u1.z - v1.z, f3 = u1.w - v1.w;
-                s0 = fmaf(e0, e0, fmaf(e1, e1, fmaf(e2, e2, fmaf(e3, e3, s0))));
-                s1 = fmaf(f0, f0, fmaf(f1, f1, fmaf(f2, f2, fmaf(f3, f3, s1))));
+            for (uint32_t d = gl * 4; d < a.D; d += 128) {
+                // (both halves of 128 values on their way at once; what lies behind the row is 0 - 0)
+                float4 u[4], v[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    u[h] = load4(x0, 0, true, a.D, d + 64 * h, a.vecX);
+                    v[h] = load4(w0, 0, true, a.D, d + 64 * h, a.vecW);
+                    u[2 + h] = load4(x1, 0, true, a.D, d + 64 * h, a.vecX);
+                    v[2 + h] = load4(w1, 0, true, a.D, d + 64 * h, a.vecW);
+                }
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const float e0 = u[h].x - v[h].x, e1 = u[h].y - v[h].y, e2 = u[h].z - v[h].z, e3 = u[h].w - v[h].w;
+                    float &s = h < 2 ? s0 : s1;
+                    s = fmaf(e0, e0, fmaf(e1, e1, fmaf(e2, e2, fmaf(e3, e3, s))));
+                }
             }
             s0 = row_sum(s0);
             s1 = row_sum(s1);
@@ -309,73 +407,108 @@ __global__ void __launch_bounds__(MF_THREADS, 2) k_scores_mfma(const ScoreArgs a
         }
         return;
     }
-    // the wave's whole tile, 4 R x 4 R scores a lane
-    __threadfence();                                   // (its scores so far are written, before others lanes write some of them again)
+    // the wave's whole tile, a square of it at a time, Q x Q scores a lane
+    __threadfence();                                   // (its scores so far are written, before other lanes write some of them again)
+    constexpr int Q = 4 * RW;
     const int ty = lane >> 3, tx = lane & 7;
-    float sum[4 * R][4 * R];
+#pragma unroll 1
+    for (uint32_t c0 = 0; c0 < NT; c0 += MT) {
+        float sum[Q][Q];
 #pragma unroll
-    for (int i = 0; i < 4 * R; ++i)
+        for (int i = 0; i < Q; ++i)
 #pragma unroll
-        for (int j = 0; j < 4 * R; ++j) sum[i][j] = 0.0f;
-    for (uint32_t d = 0; d < a.D; d += 4) {
-        float4 x[4 * R], w[4 * R];
+            for (int j = 0; j < Q; ++j) sum[i][j] = 0.0f;
+        for (uint32_t d = 0; d < a.D; d += 4) {
+            float4 x[Q], w[Q];
 #pragma unroll
-        for (int i = 0; i < 4 * R; ++i) {
-            x[i] = load4(a.X, wrow + ty + 8 * i, wrow + ty + 8 * i < a.N, a.D, d, a.vecX);
-            w[i] = load4(a.W, wcol + tx + 8 * i, wcol + tx + 8 * i < a.K, a.D, d, a.vecW);
+            for (int i = 0; i < Q; ++i) {
+                x[i] = load4(a.X, wrow + ty + 8 * i, wrow + ty + 8 * i < a.N, a.D, d, a.vecX);
+                w[i] = load4(a.W, wcol + c0 + tx + 8 * i, wcol + c0 + tx + 8 * i < a.K, a.D, d, a.vecW);
+            }
+#pragma unroll
+            for (int i = 0; i < Q; ++i)
+#pragma unroll
+                for (int j = 0; j < Q; ++j) {
+                    const float e0 = x[i].x - w[j].x, e1 = x[i].y - w[j].y, e2 = x[i].z - w[j].z, e3 = x[i].w - w[j].w;
+                    sum[i][j] = fmaf(e3, e3, fmaf(e2, e2, fmaf(e1, e1, fmaf(e0, e0, sum[i][j]))));
+                }
         }
 #pragma unroll
-        for (int i = 0; i < 4 * R; ++i)
+        for (int i = 0; i < Q; ++i)
 #pragma unroll
-            for (int j = 0; j < 4 * R; ++j) {
-                const float e0 = x[i].x - w[j].x, e1 = x[i].y - w[j].y, e2 = x[i].z - w[j].z, e3 = x[i].w - w[j].w;
-                sum[i][j] = fmaf(e3, e3, fmaf(e2, e2, fmaf(e1, e1, fmaf(e0, e0, sum[i][j]))));
+            for (int j = 0; j < Q; ++j) {
+                const uint64_t r = wrow + ty + 8 * i;
+                const uint32_t c = wcol + c0 + tx + 8 * j;
+                if (r < a.N && c < a.K) a.S[r * a.ld + c] = -sum[i][j];
             }
     }
-#pragma unroll
-    for (int i = 0; i < 4 * R; ++i)
-#pragma unroll
-        for (int j = 0; j < 4 * R; ++j) {
-            const uint64_t r = wrow + ty + 8 * i;
-            const uint32_t c = wcol + tx + 8 * j;
-            if (r < a.N && c < a.K) a.S[r * a.ld + c] = -sum[i][j];
-        }
 }
 
-template <int R>
-hipError_t run_mfma(ScoreArgs a, hipStream_t s)
+template <int RW, int CW, int WR, int WC, int PER_SIMD, bool VEC>
+hipError_t run_mfma_as(ScoreArgs a, hipStream_t s)
 {
-    constexpr uint32_t TILE = 64 * R;
-    a.colTiles = (a.K + TILE - 1) / TILE;
-    const uint64_t N = a.N, most = std::max<uint64_t>(1, (1u << 30) / a.colTiles) * TILE;        // a grid holds fewer than 2^31 workgroups
+    constexpr uint32_t TM = 32 * RW * WR, TN = 32 * CW * WC;
+    static_assert(IMG_PAD % TN == 0, "the image covers every tile");
+    a.colTiles = (a.K + TN - 1) / TN;
+    const uint64_t N = a.N, most = std::max<uint64_t>(1, (1u << 30) / a.colTiles) * TM;          // a grid holds fewer than 2^31 workgroups
     const float *X = a.X;
     float *S = a.S;
     for (uint64_t off = 0; off < N; off += most) {
         a.X = X + off * a.D;
         a.S = S + off * a.ld;
         a.N = std::min(N - off, most);
-        const uint64_t tiles = (a.N + TILE - 1) / TILE * a.colTiles;
-        hipLaunchKernelGGL((k_scores_mfma<R>), dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(MF_THREADS), 0, s, a);
+        const uint64_t tiles = (a.N + TM - 1) / TM * a.colTiles;
+        hipLaunchKernelGGL((k_scores_mfma<RW, CW, WR, WC, PER_SIMD, VEC>), dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(WR * WC * 64), 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
 
+template <int RW, int CW, int WR, int WC, int PER_SIMD>
+hipError_t run_mfma(const ScoreArgs &a, hipStream_t s)
+{
+    return a.vecX && a.vecC ? run_mfma_as<RW, CW, WR, WC, PER_SIMD, true>(a, s) : run_mfma_as<RW, CW, WR, WC, PER_SIMD, false>(a, s);
+}
+
 }  // namespace
 
-hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const float *dC, uint32_t K, float *dS, uint64_t ld, hipStream_t s)
+size_t scores_image_bytes(uint32_t K, uint32_t D)
 {
-    ScoreArgs a{dX, dW, dC, dS, N, ld, K, D, (K + SC_N - 1) / SC_N, 0, 0, 0, 0};
+    if (D <= DIRECT_D) return 0;
+    const size_t blocks = image_blocks(K), steps = (D + MF_K - 1) / MF_K;
+    return steps * blocks * IMG_BLOCK * 4 + blocks * 64 * 4;
+}
+
+hipError_t launch_scores_image(const float *dW, const float *dC, uint32_t K, uint32_t D, void *dImg, hipStream_t s)
+{
+    const uint32_t blocks = image_blocks(K), steps = (D + MF_K - 1) / MF_K;
+    hipLaunchKernelGGL(k_scores_image, dim3((uint32_t)((size_t)blocks * steps)), dim3(256), 0, s, dW, dC, K, D, blocks, (uint32_t *)dImg);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k_scores_norms, dim3(blocks * 64), dim3(64), 0, s, dW, dC, K, D, (float *)((uint32_t *)dImg + (size_t)steps * blocks * IMG_BLOCK));
+    return hipGetLastError();
+}
+
+hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const float *dC, const void *dImg, uint32_t K, float *dS, uint64_t ld,
+                         hipStream_t s)
+{
+    ScoreArgs a{dX, dW, dC, dS, N, ld, K, D, nullptr, nullptr, image_blocks(K), (K + SC_N - 1) / SC_N, 0, 0, 0, 0};
+    a.img = (const uint32_t *)dImg;
+    a.norms = (const float *)(a.img + (size_t)((D + MF_K - 1) / MF_K) * a.blocks * IMG_BLOCK);
     const bool rows = D % 4 == 0;
     a.vecX = rows && ((uintptr_t)dX & 15) == 0;
     a.vecW = rows && ((uintptr_t)dW & 15) == 0;
     a.vecC = rows && ((uintptr_t)dC & 15) == 0;
     a.vecS = ld % 4 == 0 && ((uintptr_t)dS & 15) == 0;
     if (D > DIRECT_D) {
-        // the large tile reads every operand half as often; the small one fills the card with fewer scores
-        const uint64_t large = (N + 127) / 128 * ((K + 127) / 128);
-        return large >= 512 ? run_mfma<2>(a, s) : run_mfma<1>(a, s);
+        // Larger tiles read both operands less often, smaller ones leave fewer of the 512 places (two workgroups a CU) empty in the last
+        // round.  us, 128 x 256 / 128 x 128 / 64 x 64 tiles: 500k x 128 against 256 (3907 wide tiles) 270 / 295 / 399, 20011 x 784
+        // against 1000 (628) 209 / 203 / 278
+        const uint64_t rows = (N + 127) / 128;
+        if (rows * ((K + 255) / 256) >= 2048) return run_mfma<2, 4, 2, 2, 2>(a, s);
+        if (rows * ((K + 127) / 128) >= 512) return run_mfma<2, 2, 2, 2, 2>(a, s);
+        return run_mfma<1, 1, 2, 2, 4>(a, s);
     }
     // one grid holds fewer than 2^31 workgroups
     const uint64_t most = ((1ull << 30) / a.colTiles) * SC_M;
