@@ -105,19 +105,24 @@ hipError_t run_lookup(LookupArgs a, hipStream_t s)
 // part of the tile, and takes 64 of them at a time, so (wave, step, lane) is the order of the positions.  The place of an
 // element among those with its digit: how many the waves before it hold (a table per wave, summed once), how many the steps
 // before it held (the table's running count), and how many lanes below it hold the same digit (a ballot per digit bit).
-constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_ITEMS = 16;
-constexpr uint32_t SORT_TILE = SORT_THREADS * SORT_ITEMS;
-constexpr int SORT_MAX_BITS = 11;                                   // bins of one pass: 2 bytes x 2048 x 8 waves of LDS
+constexpr int SORT_MAX_BITS = 11;                                   // bits of one pass
 constexpr uint32_t NONE = 0xFFFFFFFFu;
 
+// The lanes whose digit of `bits` <= MAX bits is this lane's
+template <int MAX>
 __device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits)
 {
-    uint64_t m = ~0ull;
-    for (int b = 0; b < bits; ++b) {
-        const uint64_t v = __ballot((d >> b) & 1);
-        m &= (d >> b) & 1 ? v : ~v;
+    uint32_t lo = ~0u, hi = ~0u;
+#pragma unroll
+    for (int b = 0; b < MAX; ++b) {
+        if (b < bits) {                                                     // (the same in all lanes)
+            const uint64_t v = __ballot((d >> b) & 1);
+            const uint32_t mine = (uint32_t)((int32_t)(d << (31 - b)) >> 31);
+            lo &= ~((uint32_t)v ^ mine);
+            hi &= ~((uint32_t)(v >> 32) ^ mine);
+        }
     }
-    return m;
+    return (uint64_t)hi << 32 | lo;
 }
 
 // Exclusive prefix sum over the n <= 2048 entries of `a` (LDS), by the whole workgroup of THREADS lanes.
@@ -146,42 +151,91 @@ __device__ void scan_bins(uint32_t *a, uint32_t n, uint32_t *tmp)
     __syncthreads();
 }
 
+// Rows of zeros where start[k] is NONE, 2^log2g lanes a row, `width` bytes a lane and store
+struct ZeroArgs {
+    char *G;
+    uint64_t pitch, bytes;          // of a row, in bytes
+    uint32_t width;
+    int log2g;
+    uint32_t blocks;                // workgroups that do it, behind the others; 0: none
+};
+
+template <class V>
+__device__ __forceinline__ void zero_rows_by(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
+{
+    const uint32_t gl = threadIdx.x & ((1u << z.log2g) - 1), groups = threads >> z.log2g;
+    const V zero{};
+    for (uint64_t k = (uint64_t)block * groups + (threadIdx.x >> z.log2g); k < K; k += (uint64_t)z.blocks * groups) {
+        if (start[k] != NONE) continue;
+        char *row = z.G + k * z.pitch;
+        for (uint64_t at = gl * sizeof(V); at < z.bytes; at += sizeof(V) << z.log2g) *(V *)(row + at) = zero;
+    }
+}
+__device__ __forceinline__ void zero_rows(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
+{
+    switch (z.width) {
+    case 16: return zero_rows_by<uint4>(z, start, K, block, threads);
+    case 8: return zero_rows_by<uint2>(z, start, K, block, threads);
+    case 4: return zero_rows_by<uint32_t>(z, start, K, block, threads);
+    default: return zero_rows_by<uint16_t>(z, start, K, block, threads);
+    }
+}
+
 struct SortArgs {
     const uint32_t *idx;            // first pass: keys are min(idx, K), rows their positions; null later
     const uint32_t *keys_in, *rows_in;
     uint32_t *keys, *rows;          // result of the pass
     uint32_t *hist;                 // [bins][tiles]
     uint32_t *total;                // [bins]
-    uint32_t *start;                // K entries to set to NONE in the first pass
+    uint32_t *start;                // K entries: NONE in the first pass, then (with `mark`) 0 where an index occurs
+    const uint32_t *mark;           // the indices, or null
     uint32_t N, K, tiles;
     int shift, bits;
+    ZeroArgs zero;                  // rows to clear beside the first move
 };
 
 __device__ __forceinline__ uint32_t load_key(const SortArgs &a, uint32_t i)
 {
     return a.idx ? min(a.idx[i], a.K) : a.keys_in[i];
 }
+__device__ __forceinline__ void mark_present(const SortArgs &a, uint64_t from, uint64_t step)
+{
+    for (uint64_t i = from; i < a.N; i += step) {
+        const uint32_t k = a.mark[i];
+        if (k < a.K) a.start[k] = 0;
+    }
+}
 
-__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const SortArgs a)
+// THREADS x ITEMS positions a workgroup
+template <int THREADS, int ITEMS>
+__global__ void __launch_bounds__(THREADS) k_sort_count(const SortArgs a)
 {
     __shared__ uint32_t bins[1 << SORT_MAX_BITS];
+    constexpr uint32_t TILE = THREADS * ITEMS;
     const uint32_t nb = 1u << a.bits, tile = blockIdx.x;
-    for (uint32_t b = threadIdx.x; b < nb; b += SORT_THREADS) bins[b] = 0;
+    for (uint32_t b = threadIdx.x; b < nb; b += THREADS) bins[b] = 0;
     if (a.idx)
-        for (uint64_t k = (uint64_t)tile * SORT_THREADS + threadIdx.x; k < a.K; k += (uint64_t)gridDim.x * SORT_THREADS) a.start[k] = NONE;
+        for (uint64_t k = (uint64_t)tile * THREADS + threadIdx.x; k < a.K; k += (uint64_t)gridDim.x * THREADS) a.start[k] = NONE;
     __syncthreads();
-    const uint32_t base = tile * SORT_TILE, end = min(a.N - base, SORT_TILE);
-#pragma unroll 4
-    for (uint32_t j = threadIdx.x; j < end; j += SORT_THREADS) atomicAdd(&bins[(load_key(a, base + j) >> a.shift) & (nb - 1)], 1u);
+    const uint32_t base = tile * TILE, end = min(a.N - base, TILE);
+    uint32_t key[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) key[j] = threadIdx.x + j * THREADS < end ? load_key(a, base + threadIdx.x + j * THREADS) : 0;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+        if (threadIdx.x + j * THREADS < end) atomicAdd(&bins[(key[j] >> a.shift) & (nb - 1)], 1u);
     __syncthreads();
-    for (uint32_t b = threadIdx.x; b < nb; b += SORT_THREADS) a.hist[(size_t)b * a.tiles + tile] = bins[b];
+    for (uint32_t b = threadIdx.x; b < nb; b += THREADS) a.hist[(size_t)b * a.tiles + tile] = bins[b];
 }
 
 // One workgroup per bin: exclusive prefix sum over the tiles, in place, and the bin's total.
-__global__ void __launch_bounds__(256) k_sort_scan(uint32_t *hist, uint32_t *total, uint32_t tiles)
+// Workgroups behind the bins': which indices occur.
+__global__ void __launch_bounds__(256) k_sort_scan(const SortArgs a)
 {
     __shared__ uint32_t part[4];
-    uint32_t *h = hist + (size_t)blockIdx.x * tiles;
+    const uint32_t nb = 1u << a.bits, tiles = a.tiles;
+    if (blockIdx.x >= nb) return mark_present(a, (uint64_t)(blockIdx.x - nb) * 256 + threadIdx.x, (uint64_t)(gridDim.x - nb) * 256);
+    uint32_t *h = a.hist + (size_t)blockIdx.x * tiles, *total = a.total;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     uint32_t carry = 0;
     for (uint32_t base = 0; base < tiles; base += 256) {
@@ -204,34 +258,41 @@ __global__ void __launch_bounds__(256) k_sort_scan(uint32_t *hist, uint32_t *tot
 
 // Ranks `ITEMS` elements per lane (held in registers, wave-consecutive) by their digit; on return rank[j] is the element's
 // place inside the tile and first[d] the first place of digit d.  `count`: WAVES tables of nb counters.
-template <int WAVES, int ITEMS>
+template <int WAVES, int ITEMS, int MAX>
 __device__ __forceinline__ void rank_tile(const uint32_t (&key)[ITEMS], uint32_t valid, int shift, int bits, uint16_t *count, uint32_t *first, uint32_t *tmp,
                                           uint32_t (&rank)[ITEMS])
 {
     const uint32_t nb = 1u << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (uint32_t b = threadIdx.x; b < nb * WAVES; b += WAVES * 64) count[b] = 0;
+    for (uint32_t b = threadIdx.x; b < nb * WAVES / 2; b += WAVES * 64) ((uint32_t *)count)[b] = 0;
     __syncthreads();
     uint16_t *mine = count + w * nb;
+    uint64_t same[ITEMS];
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
         const bool on = (w * ITEMS + j) * 64 + lane < valid;
-        const uint32_t d = on ? (key[j] >> shift) & (nb - 1) : nb;          // bit `bits` set: never equal to a digit of the tile
-        const uint64_t same = same_digit(d, bits + 1);
-        const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+        same[j] = same_digit<MAX + 1>(on ? (key[j] >> shift) & (nb - 1) : nb, bits + 1);    // (bit `bits` set: no digit of the tile)
+    }
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+        const bool on = (w * ITEMS + j) * 64 + lane < valid;
+        const uint32_t d = (key[j] >> shift) & (nb - 1);
+        const uint32_t below = __builtin_amdgcn_mbcnt_hi((uint32_t)(same[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same[j], 0));
         uint32_t had = 0;
         if (on) had = mine[d];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");              // every lane has read before the first of them adds
-        if (on && below == 0) mine[d] = (uint16_t)(had + __popcll(same));
+        if (on && below == 0) mine[d] = (uint16_t)(had + __popcll(same[j]));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         rank[j] = had + below;
     }
     __syncthreads();
     for (uint32_t b = threadIdx.x; b < nb; b += WAVES * 64) {
-        uint32_t run = 0;
+        uint32_t c[WAVES], run = 0;
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) c[k] = count[k * nb + b];
+#pragma unroll
         for (int k = 0; k < WAVES; ++k) {
-            const uint32_t c = count[k * nb + b];
             count[k * nb + b] = (uint16_t)run;
-            run += c;
+            run += c[k];
         }
         first[b] = run;
     }
@@ -245,76 +306,85 @@ __device__ __forceinline__ void rank_tile(const uint32_t (&key)[ITEMS], uint32_t
         }
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) k_sort_move(const SortArgs a)
+template <int THREADS, int ITEMS>
+__global__ void __launch_bounds__(THREADS) k_sort_move(const SortArgs a)
 {
-    __shared__ uint32_t lkey[SORT_TILE], lrow[SORT_TILE];                   // 64 KiB
-    __shared__ uint16_t count[SORT_WAVES << SORT_MAX_BITS];                 // 32 KiB
-    __shared__ uint32_t first[1 << SORT_MAX_BITS], base[1 << SORT_MAX_BITS], tmp[SORT_WAVES];
+    constexpr int WAVES = THREADS / 64;
+    constexpr uint32_t TILE = THREADS * ITEMS;
+    __shared__ uint32_t lkey[TILE], lrow[TILE], tmp[WAVES];
+    extern __shared__ uint32_t tables[];                                    // per bin: first, base, and WAVES 2-byte counters
     const uint32_t nb = 1u << a.bits, tile = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint32_t begin = tile * SORT_TILE, valid = min(a.N - begin, SORT_TILE);
-    uint32_t key[SORT_ITEMS], row[SORT_ITEMS], rank[SORT_ITEMS];
+    if (tile >= a.tiles) return zero_rows(a.zero, a.start, a.K, tile - a.tiles, THREADS);
+    uint32_t *first = tables, *base = tables + nb;
+    uint16_t *count = (uint16_t *)(tables + 2 * nb);
+    const uint32_t begin = tile * TILE, valid = min(a.N - begin, TILE);
+    uint32_t key[ITEMS], row[ITEMS], rank[ITEMS];
 #pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const uint32_t p = (w * SORT_ITEMS + j) * 64 + lane;
+    for (int j = 0; j < ITEMS; ++j) {
+        const uint32_t p = (w * ITEMS + j) * 64 + lane;
         key[j] = p < valid ? load_key(a, begin + p) : 0;
         row[j] = p < valid ? (a.idx ? begin + p : a.rows_in[begin + p]) : 0;
     }
-    for (uint32_t b = threadIdx.x; b < nb; b += SORT_THREADS) base[b] = a.total[b];
+    for (uint32_t b = threadIdx.x; b < nb; b += THREADS) base[b] = a.total[b];
     __syncthreads();
-    scan_bins<SORT_THREADS>(base, nb, tmp);
-    rank_tile<SORT_WAVES, SORT_ITEMS>(key, valid, a.shift, a.bits, count, first, tmp, rank);
+    scan_bins<THREADS>(base, nb, tmp);
+    rank_tile<WAVES, ITEMS, SORT_MAX_BITS>(key, valid, a.shift, a.bits, count, first, tmp, rank);
+    // where this tile's elements of a digit go, less their first place in the tile
+    for (uint32_t b = threadIdx.x; b < nb; b += THREADS) base[b] += a.hist[(size_t)b * a.tiles + tile] - first[b];
 #pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j)
-        if ((w * SORT_ITEMS + j) * 64 + lane < valid) {
+    for (int j = 0; j < ITEMS; ++j)
+        if ((w * ITEMS + j) * 64 + lane < valid) {
             lkey[rank[j]] = key[j];
             lrow[rank[j]] = row[j];
         }
     __syncthreads();
     // through LDS in the order of the places, so that the elements of a digit leave as one consecutive piece
-    for (uint32_t p = threadIdx.x; p < valid; p += SORT_THREADS) {
-        const uint32_t k = lkey[p], d = (k >> a.shift) & (nb - 1);
-        const uint32_t to = base[d] + a.hist[(size_t)d * a.tiles + tile] + (p - first[d]);
+    for (uint32_t p = threadIdx.x; p < valid; p += THREADS) {
+        const uint32_t k = lkey[p], to = base[(k >> a.shift) & (nb - 1)] + p;
         a.keys[to] = k;
         a.rows[to] = lrow[p];
     }
 }
 
-// All passes in one workgroup and one launch, for at most SMALL_TILE rows.
-constexpr int SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64, SMALL_ITEMS = 8;
-constexpr uint32_t SMALL_TILE = SMALL_THREADS * SMALL_ITEMS;
-constexpr int SMALL_MAX_BITS = 9;
+// All passes in one workgroup and one launch, for at most THREADS x ITEMS rows.
+constexpr uint32_t SMALL_TILE = 8192;
+constexpr int SMALL_MAX_BITS = 8;
 
-__global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(const SortArgs a, int key_bits)
+template <int THREADS, int ITEMS>
+__global__ void __launch_bounds__(THREADS) k_sort_small(const SortArgs a, int key_bits)
 {
-    __shared__ uint32_t lkey[SMALL_TILE], lrow[SMALL_TILE];                 // 64 KiB
-    __shared__ uint16_t count[SMALL_WAVES << SMALL_MAX_BITS];               // 16 KiB
-    __shared__ uint32_t first[1 << SMALL_MAX_BITS], tmp[SMALL_WAVES];
+    constexpr int WAVES = THREADS / 64;
+    constexpr uint32_t TILE = THREADS * ITEMS;
+    __shared__ uint32_t lkey[TILE], lrow[TILE];                             // 64 KiB at most
+    __shared__ __attribute__((aligned(4))) uint16_t count[WAVES << SMALL_MAX_BITS];
+    __shared__ uint32_t first[1 << SMALL_MAX_BITS], tmp[WAVES];
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    if (blockIdx.x != 0) {                                                  // the other workgroups only set `start`
-        for (uint64_t k = (uint64_t)(blockIdx.x - 1) * SMALL_THREADS + threadIdx.x; k < a.K; k += (uint64_t)(gridDim.x - 1) * SMALL_THREADS) a.start[k] = NONE;
+    if (blockIdx.x != 0) {                                                  // the other workgroups only set `start`, or clear rows
+        if (a.zero.blocks) return zero_rows(a.zero, a.start, a.K, blockIdx.x - 1, THREADS);
+        for (uint64_t k = (uint64_t)(blockIdx.x - 1) * THREADS + threadIdx.x; k < a.K; k += (uint64_t)(gridDim.x - 1) * THREADS) a.start[k] = NONE;
         return;
     }
-    uint32_t key[SMALL_ITEMS], row[SMALL_ITEMS], rank[SMALL_ITEMS];
+    uint32_t key[ITEMS], row[ITEMS], rank[ITEMS];
 #pragma unroll
-    for (int j = 0; j < SMALL_ITEMS; ++j) {
-        const uint32_t p = (w * SMALL_ITEMS + j) * 64 + lane;
+    for (int j = 0; j < ITEMS; ++j) {
+        const uint32_t p = (w * ITEMS + j) * 64 + lane;
         key[j] = p < a.N ? load_key(a, p) : 0;
         row[j] = p;
     }
     const int passes = (key_bits + SMALL_MAX_BITS - 1) / SMALL_MAX_BITS, bits = (key_bits + passes - 1) / passes;
     for (int pass = 0; pass < passes; ++pass) {
-        rank_tile<SMALL_WAVES, SMALL_ITEMS>(key, a.N, pass * bits, bits, count, first, tmp, rank);
+        rank_tile<WAVES, ITEMS, SMALL_MAX_BITS>(key, a.N, pass * bits, bits, count, first, tmp, rank);
 #pragma unroll
-        for (int j = 0; j < SMALL_ITEMS; ++j)
-            if ((w * SMALL_ITEMS + j) * 64 + lane < a.N) {
+        for (int j = 0; j < ITEMS; ++j)
+            if ((w * ITEMS + j) * 64 + lane < a.N) {
                 lkey[rank[j]] = key[j];
                 lrow[rank[j]] = row[j];
             }
         __syncthreads();
         if (pass + 1 < passes) {
 #pragma unroll
-            for (int j = 0; j < SMALL_ITEMS; ++j) {
-                const uint32_t p = (w * SMALL_ITEMS + j) * 64 + lane;
+            for (int j = 0; j < ITEMS; ++j) {
+                const uint32_t p = (w * ITEMS + j) * 64 + lane;
                 if (p < a.N) {
                     key[j] = lkey[p];
                     row[j] = lrow[p];
@@ -323,11 +393,29 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(const SortArgs a, 
             __syncthreads();
         }
     }
-    for (uint32_t p = threadIdx.x; p < a.N; p += SMALL_THREADS) {
+    for (uint32_t p = threadIdx.x; p < a.N; p += THREADS) {
         a.keys[p] = lkey[p];
         a.rows[p] = lrow[p];
     }
 }
+
+template <int THREADS, int ITEMS>
+void run_sort_small(const SortArgs &a, int key_bits, hipStream_t s)
+{
+    const uint32_t fill = a.zero.blocks ? a.zero.blocks : std::min<uint32_t>((a.K + THREADS - 1) / THREADS, 256);
+    hipLaunchKernelGGL((k_sort_small<THREADS, ITEMS>), dim3(1 + fill), dim3(THREADS), 0, s, a, key_bits);
+}
+
+template <int THREADS, int ITEMS>
+void run_sort_pass(const SortArgs &a, hipStream_t s)
+{
+    const uint32_t nb = 1u << a.bits, marks = a.mark ? std::min<uint32_t>((a.N + 255) / 256, 1024) : 0;
+    hipLaunchKernelGGL((k_sort_count<THREADS, ITEMS>), dim3(a.tiles), dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL(k_sort_scan, dim3(nb + marks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_sort_move<THREADS, ITEMS>), dim3(a.tiles + a.zero.blocks), dim3(THREADS), nb * (8 + THREADS / 64 * 2), s, a);
+}
+
+__global__ void __launch_bounds__(256) k_mark(const SortArgs a) { mark_present(a, (uint64_t)blockIdx.x * 256 + threadIdx.x, (uint64_t)gridDim.x * 256); }
 
 __global__ void k_fill_u32(uint32_t *p, uint64_t n, uint32_t v)
 {
@@ -343,7 +431,7 @@ struct GradArgs {
     float scale;
     void *G;
     uint64_t ldg;
-    int accumulate;
+    int accumulate, cleared;        // cleared: the rows no index names are zero already
     uint32_t *start, *end;          // K each: first place and place behind the last of every index that occurs
     uint32_t *counts;               // nullable
     float *parts;                   // [chunks][2][dpad]: head (a run that began in an earlier chunk), tail (one that goes on)
@@ -487,7 +575,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad_join(const GradArgs a, ui
     for (uint64_t k = (uint64_t)(blockIdx.x - join_blocks) * groups + gi; k < a.K; k += lanes) {
         const uint32_t s = a.start[k];
         if (a.counts && gl == 0) a.counts[k] = s == NONE ? 0 : a.end[k] - s;
-        if (s != NONE || a.accumulate) continue;
+        if (s != NONE || a.accumulate || a.cleared) continue;
         Pack<TO, E * (int)sizeof(TO)> zero;
 #pragma unroll
         for (int e = 0; e < E; ++e) zero.v[e] = (TO)0.0f;
@@ -497,7 +585,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad_join(const GradArgs a, ui
 
 // ---------------------------------------------------------------------------------------------- plan of one gradient call
 struct GradPlan {
-    uint32_t tiles, chunk, chunks, dpad;
+    uint32_t tile, tiles, chunk, chunks, dpad;
     int key_bits, passes, bits;
     bool small;
     size_t keys[2], rows[2], hist, total, start, end, parts, bytes;      // offsets into the workspace
@@ -510,7 +598,9 @@ GradPlan plan_gradient(uint64_t N, uint32_t K, uint32_t D)
     p.key_bits = 32 - __builtin_clz(K);                                   // indices 0 .. K - 1, and K for the rows without a place
     p.passes = (p.key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     p.bits = (p.key_bits + p.passes - 1) / p.passes;
-    p.tiles = (uint32_t)((N + SORT_TILE - 1) / SORT_TILE);
+    // small tiles spread a sort over the card; of very many rows they would make the table of counts large
+    p.tile = N <= (4u << 20) ? 2048 : 8192;
+    p.tiles = (uint32_t)((N + p.tile - 1) / p.tile);
     // chunks: enough groups of lanes to fill the card (8192 waves) however the runs lie, at least 8 rows each, so that the
     // parts of runs that cross chunk borders stay a small share of the rows read
     const uint64_t units = N * ((D + 255) / 256);
@@ -591,12 +681,31 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
     const GradPlan p = plan_gradient(N, K, D);
     char *w = (char *)dwork;
     auto at = [&](size_t o) { return (uint32_t *)(w + o); };
-    SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), (uint32_t)N, K, p.tiles, 0, p.bits};
+    const size_t bi = elem_bytes(dtype), bo = elem_bytes(out_dtype);
+    const int wo = widest_access(bo, (uint64_t)(uintptr_t)dT | ldt * bo | (uint64_t)D * bo);
+    // Rows no index names are cleared beside the sort, whose few workgroups leave the memory idle, where clearing takes longer
+    // than telling the rows apart beforehand (two small launches; 16384 rows of 4096 over 65536: 334 us without, 286 with).
+    const bool early = N > 0 && !accumulate && (uint64_t)K * D * bo >= (32u << 20);
+    SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), nullptr, (uint32_t)N, K, p.tiles, 0, p.bits, {}};
+    ZeroArgs zero{(char *)dT, ldt * bo, (uint64_t)D * bo, (uint32_t)wo, 0, 0};
+    while (((uint64_t)wo << zero.log2g) < zero.bytes && zero.log2g < 6) ++zero.log2g;
+    zero.blocks = early ? std::min<uint32_t>((K + 15) / 16, 4096) : 0;
+    const uint32_t few = std::min<uint32_t>((K + 255) / 256, 4096);
     if (N == 0) {
-        hipLaunchKernelGGL(k_fill_u32, dim3(std::min<uint32_t>((K + 255) / 256, 4096)), dim3(256), 0, s, q.start, (uint64_t)K, NONE);
+        hipLaunchKernelGGL(k_fill_u32, dim3(few), dim3(256), 0, s, q.start, (uint64_t)K, NONE);
     } else if (p.small) {
-        const uint32_t fill = std::min<uint32_t>((K + SMALL_THREADS - 1) / SMALL_THREADS, 256);
-        hipLaunchKernelGGL(k_sort_small, dim3(1 + fill), dim3(SMALL_THREADS), 0, s, q, p.key_bits);
+        if (early) {
+            q.mark = didx;
+            hipLaunchKernelGGL(k_fill_u32, dim3(few), dim3(256), 0, s, q.start, (uint64_t)K, NONE);
+            hipLaunchKernelGGL(k_mark, dim3((uint32_t)(N + 255) / 256), dim3(256), 0, s, q);
+            q.zero = zero;
+        }
+        if (N <= 1024)
+            run_sort_small<256, 4>(q, p.key_bits, s);
+        else if (N <= 4096)
+            run_sort_small<1024, 4>(q, p.key_bits, s);
+        else
+            run_sort_small<1024, 8>(q, p.key_bits, s);
     } else {
         for (int pass = 0; pass < p.passes; ++pass) {
             const int to = (p.passes - 1 - pass) & 1;                       // the last pass ends in buffer 0
@@ -606,20 +715,21 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
             q.keys = at(p.keys[to]);
             q.rows = at(p.rows[to]);
             q.shift = pass * p.bits;
-            hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(SORT_THREADS), 0, s, q);
-            hipLaunchKernelGGL(k_sort_scan, dim3(1u << p.bits), dim3(256), 0, s, q.hist, q.total, p.tiles);
-            hipLaunchKernelGGL(k_sort_move, dim3(p.tiles), dim3(SORT_THREADS), 0, s, q);
+            q.mark = early && pass == 0 ? didx : nullptr;
+            q.zero = pass == 0 ? zero : ZeroArgs{};
+            if (p.tile == 2048)
+                run_sort_pass<256, 8>(q, s);
+            else
+                run_sort_pass<512, 16>(q, s);
         }
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const GradArgs a{dG, ldg, at(p.keys[0]), at(p.rows[0]), (uint32_t)N, K, D, scale, dT, ldt, accumulate ? 1 : 0, at(p.start), at(p.end), dcounts,
+    const GradArgs a{dG, ldg, at(p.keys[0]), at(p.rows[0]), (uint32_t)N, K, D, scale, dT, ldt, accumulate ? 1 : 0, early ? 1 : 0, at(p.start), at(p.end), dcounts,
                      (float *)(w + p.parts), p.dpad, p.chunk, p.chunks, 0, 0};
     // elements a lane takes at once: what 16 bytes of the rows hold, if rows, table and strides are aligned for it
-    const size_t bi = elem_bytes(dtype), bo = elem_bytes(out_dtype);
     const int wi = widest_access(bi, (uint64_t)(uintptr_t)dG | ldg * bi | (uint64_t)D * bi);
-    const int wo = widest_access(bo, (uint64_t)(uintptr_t)dT | ldt * bo | (uint64_t)D * bo);
-    const int n = std::min(wi / (int)bi, wo >= 16 ? 16 : wo / (int)bo);
+    const int n = std::min(wi / (int)bi, wo / (int)bo);
     if (dtype == VQHIP_F32) return run_reduce_width<float, float>(a, n, s);
     if (dtype == VQHIP_BF16) return out_dtype == VQHIP_F32 ? run_reduce_width<__bf16, float>(a, n, s) : run_reduce_width<__bf16, __bf16>(a, n, s);
     return out_dtype == VQHIP_F32 ? run_reduce_width<_Float16, float>(a, n, s) : run_reduce_width<_Float16, _Float16>(a, n, s);
