@@ -14,9 +14,9 @@ namespace vq {
 template <class T> __device__ __forceinline__ float widen(T v) { return (float)v; }
 template <class T> __device__ __forceinline__ T narrow(float v) { return (T)v; }
 
-// BYTES of consecutive elements, moved by one load or store (32: by two); the address is a multiple of BYTES, at most 16
+// BYTES of consecutive elements, moved by one load or store; the address is a multiple of BYTES
 template <class T, int BYTES>
-struct alignas(BYTES > 16 ? 16 : BYTES) Pack {
+struct alignas(BYTES) Pack {
     static constexpr int E = BYTES / (int)sizeof(T);
     T v[E];
 };

@@ -17,6 +17,7 @@
 //              chunk borders go to the workspace in f32
 //     join     k_grad_join: adds up the parts of those runs in order, writes the rows no index names, and the counts
 #include <algorithm>
+#include <type_traits>
 
 #include "codes_device.h"
 
@@ -24,7 +25,19 @@ namespace vq {
 
 namespace {
 
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
+
 // ---------------------------------------------------------------------------------------------- lookup
+// A store that does not stay in the caches: what is written here is read once at best, and the table is read over and over.
+template <class T, int BYTES>
+__device__ __forceinline__ void store_past(T *to, const Pack<T, BYTES> &v)
+{
+    using V = typename std::conditional<BYTES == 16, u32x4, typename std::conditional<BYTES == 8, u32x2,
+                                        typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type>::type;
+    __builtin_nontemporal_store(__builtin_bit_cast(V, v), (V *)to);
+}
+
 struct LookupArgs {
     const void *T;
     uint64_t ldt;
@@ -76,7 +89,7 @@ __global__ void __launch_bounds__(LOOK_THREADS) k_lookup(const LookupArgs a)
 #pragma unroll
                 for (int e = 0; e < P::E; ++e) v[u].v[e] = narrow<T>(widen(v[u].v[e]) * a.scale);
             }
-            *(P *)(out + i * a.ldy) = v[u];
+            store_past(out + i * a.ldy, v[u]);
         }
     }
 }
@@ -164,18 +177,18 @@ template <class V>
 __device__ __forceinline__ void zero_rows_by(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
 {
     const uint32_t gl = threadIdx.x & ((1u << z.log2g) - 1), groups = threads >> z.log2g;
-    const V zero{};
+    const V zero = 0;
     for (uint64_t k = (uint64_t)block * groups + (threadIdx.x >> z.log2g); k < K; k += (uint64_t)z.blocks * groups) {
         if (start[k] != NONE) continue;
         char *row = z.G + k * z.pitch;
-        for (uint64_t at = gl * sizeof(V); at < z.bytes; at += sizeof(V) << z.log2g) *(V *)(row + at) = zero;
+        for (uint64_t at = gl * sizeof(V); at < z.bytes; at += sizeof(V) << z.log2g) __builtin_nontemporal_store(zero, (V *)(row + at));
     }
 }
 __device__ __forceinline__ void zero_rows(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
 {
     switch (z.width) {
-    case 16: return zero_rows_by<uint4>(z, start, K, block, threads);
-    case 8: return zero_rows_by<uint2>(z, start, K, block, threads);
+    case 16: return zero_rows_by<u32x4>(z, start, K, block, threads);
+    case 8: return zero_rows_by<u32x2>(z, start, K, block, threads);
     case 4: return zero_rows_by<uint32_t>(z, start, K, block, threads);
     default: return zero_rows_by<uint16_t>(z, start, K, block, threads);
     }
@@ -456,7 +469,7 @@ __device__ __forceinline__ void store_grad(const GradArgs &a, uint32_t k, uint32
 #pragma unroll
         for (int e = 0; e < E; ++e) o.v[e] = narrow<TO>(acc[e] * a.scale);
     }
-    *(Pack<TO, E * (int)sizeof(TO)> *)g = o;
+    store_past(g, o);
 }
 
 // 2^log2g lanes own one chunk of sorted places and E * 2^log2g columns of it.
@@ -650,7 +663,9 @@ hipError_t run_reduce(GradArgs a, hipStream_t s)
 template <class T, class TO>
 hipError_t run_reduce_width(const GradArgs &a, int e, hipStream_t s)
 {
-    if (e >= 8 && sizeof(T) == 2) return run_reduce<T, TO, sizeof(T) == 2 ? 8 : 4>(a, s);
+    if constexpr (sizeof(TO) == 2) {
+        if (e >= 8) return run_reduce<T, TO, 8>(a, s);
+    }
     if (e >= 4) return run_reduce<T, TO, 4>(a, s);
     if (e >= 2) return run_reduce<T, TO, 2>(a, s);
     return run_reduce<T, TO, 1>(a, s);
@@ -727,7 +742,7 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
     if (e != hipSuccess) return e;
     const GradArgs a{dG, ldg, at(p.keys[0]), at(p.rows[0]), (uint32_t)N, K, D, scale, dT, ldt, accumulate ? 1 : 0, early ? 1 : 0, at(p.start), at(p.end), dcounts,
                      (float *)(w + p.parts), p.dpad, p.chunk, p.chunks, 0, 0};
-    // elements a lane takes at once: what 16 bytes of the rows hold, if rows, table and strides are aligned for it
+    // elements a lane takes at once: what 16 bytes of the rows and of the table hold, if they and their strides are aligned for it
     const int wi = widest_access(bi, (uint64_t)(uintptr_t)dG | ldg * bi | (uint64_t)D * bi);
     const int n = std::min(wi / (int)bi, wo / (int)bo);
     if (dtype == VQHIP_F32) return run_reduce_width<float, float>(a, n, s);
