@@ -571,3 +571,23 @@ def test_scores_of_long_rows_that_are_not_finite(ctx):
     bad = ~np.isfinite(want)
     assert (np.isnan(S) == np.isnan(want)).all() and (S[bad & ~np.isnan(want)] == want[bad & ~np.isnan(want)]).all()
     assert np.isfinite(S[~bad]).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [5, 250, 1001, 1030, 9001])
+def test_sample_rows_that_begin_anywhere(ctx, V, dtype):
+    """Rows at every offset from a 16-byte boundary; what lies beside them would win if it were read."""
+    g = gen(V)
+    t = TYPES[dtype]
+    buf = torch.full((17, V + 9), 3e4).to(t)
+    for off in range(9):
+        rows = (torch.randn(17, V, generator=g) * 3).to(t)
+        whole = buf.clone()
+        whole[:, off:off + V] = rows
+        u = torch.rand(17, generator=g)
+        check_sample(ctx, rows, u, dev=whole.cuda()[:, off:off + V], **[dict(), dict(top_k=3), dict(top_p=0.7), dict(min_p=0.2), dict(temperature=0.0)][off % 5])
+    first = torch.full((3, V), 0.0).to(t)
+    first[0, 0] = first[1, V - 1] = 50.0
+    first[2, V // 2] = 50.0
+    idx, _ = ctx.sample(first.cuda(), torch.full((3,), 0.5).cuda(), top_p=0.5)
+    assert idx.tolist() == [0, V - 1, V // 2]

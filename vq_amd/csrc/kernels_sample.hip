@@ -409,24 +409,45 @@ constexpr int WAVE_THREADS = 256;
 template <class T, int E, bool VEC>
 __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a)
 {
-    __shared__ __attribute__((aligned(16))) uint32_t bins[WAVE_THREADS / 64][SET_BINS];
+    // (a wave has turned its row before it needs the bins)
+    union PerWave {
+        uint32_t bins[SET_BINS];
+        float turn[VEC ? 1 : 64 * (E + 1)];
+    };
+    __shared__ __attribute__((aligned(16))) PerWave sh[WAVE_THREADS / 64];
+    PerWave &mine = sh[threadIdx.x >> 6];
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t waves = (uint64_t)gridDim.x * (WAVE_THREADS / 64);
     for (uint64_t i = (uint64_t)blockIdx.x * (WAVE_THREADS / 64) + (threadIdx.x >> 6); i < a.N; i += waves) {
         const T *row = (const T *)a.S + i * a.ld;
         WaveSet<E> set;
-        constexpr int LOAD = 16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E;
         const uint32_t j0 = lane * E;
+        if constexpr (VEC) {
+            constexpr int LOAD = 16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E;
 #pragma unroll
-        for (int c = 0; c < E; c += LOAD) {
-            if (VEC && j0 + c + LOAD <= a.V) {
-                const Pack<T, LOAD * (int)sizeof(T)> v = *(const Pack<T, LOAD * (int)sizeof(T)> *)(row + j0 + c);
+            for (int c = 0; c < E; c += LOAD) {
+                if (j0 + c + LOAD <= a.V) {
+                    const Pack<T, LOAD * (int)sizeof(T)> v = *(const Pack<T, LOAD * (int)sizeof(T)> *)(row + j0 + c);
 #pragma unroll
-                for (int e = 0; e < LOAD; ++e) set.l[c + e] = fmaxf(widen(v.v[e]), -INFINITY);      // (NaN: -inf)
-            } else {
+                    for (int e = 0; e < LOAD; ++e) set.l[c + e] = fmaxf(widen(v.v[e]), -INFINITY);      // (NaN: -inf)
+                } else {
 #pragma unroll
-                for (int e = 0; e < LOAD; ++e) set.l[c + e] = j0 + c + e < a.V ? fmaxf(widen(row[j0 + c + e]), -INFINITY) : -INFINITY;
+                    for (int e = 0; e < LOAD; ++e) set.l[c + e] = j0 + c + e < a.V ? fmaxf(widen(row[j0 + c + e]), -INFINITY) : -INFINITY;
+                }
             }
+        } else {
+            // 64 consecutive scores a load, turned in LDS to E consecutive ones a lane (rows a word longer, so that the lanes'
+            // rows begin in different banks)
+            float *turn = mine.turn;
+#pragma unroll
+            for (int c = 0; c < E; ++c) {
+                const uint32_t j = c * 64 + lane;
+                turn[j / E * (E + 1) + j % E] = j < a.V ? fmaxf(widen(row[j]), -INFINITY) : -INFINITY;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int e = 0; e < E; ++e) set.l[e] = turn[lane * (E + 1) + e];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         const RowParams p(a, i);
         float top = -INFINITY;
@@ -447,7 +468,7 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
             } else {
                 set.weigh_all(Weigh(top, p.temperature));
                 double drawn, total;
-                at = set.draw(top, p.top_k, p.top_p, p.min_p, p.u, p.reach(a.V), bins[threadIdx.x >> 6], drawn, total);
+                at = set.draw(top, p.top_k, p.top_p, p.min_p, p.u, p.reach(a.V), mine.bins, drawn, total);
                 prob = (float)(drawn / total);
             }
         }
@@ -508,18 +529,20 @@ struct Drawn {
 };
 
 // One row, worked on by a workgroup: all members are called by all its lanes.  The row is dealt to the waves in consecutive
-// ranges, a range in steps of 64 PER scores, PER consecutive ones per lane: order of index = (wave, step, lane, place).
-template <class T, int THREADS, bool VEC>
+// ranges, a range in steps of 64 PER scores, PER consecutive ones per lane: order of index = (wave, step, lane, place).  Rows
+// begin anywhere: positions count from the 16-byte boundary at or before the first score, so that all loads but those of a row's
+// two ends are aligned ones of 16 bytes; the positions in front of the row are masked scores that are not read.
+template <class T, int THREADS>
 struct BlockRow {
     static constexpr int WAVES = THREADS / 64;
-    static constexpr int PER = VEC ? 16 / (int)sizeof(T) : 1;
+    static constexpr int PER = 16 / (int)sizeof(T);
     static constexpr uint32_t STEP = 64 * PER;
     using Piece = Pack<T, PER * (int)sizeof(T)>;
     using GlobalT = const __attribute__((address_space(1))) T;
     using Global16 = const __attribute__((address_space(1))) u32x4s;
 
-    uint64_t row;                       // address of the row in global memory
-    uint32_t V;
+    uint64_t row;                       // address of position 0 in global memory
+    uint32_t first, V;                  // positions of the first score and behind the last
     int s;
     Weigh weigh;
 
@@ -528,6 +551,7 @@ struct BlockRow {
     {
         BlockRow b;
         b.row = same(row);
+        b.first = same(first);
         b.V = same(V);
         b.s = (int)same((uint32_t)s);
         b.weigh.top = same(weigh.top);
@@ -545,27 +569,18 @@ struct BlockRow {
         lo = (uint32_t)min(from, (uint64_t)end);
         hi = (uint32_t)min(from + len, (uint64_t)end);
     }
-    __device__ __forceinline__ Piece load_whole(uint32_t j) const
-    {
-        if constexpr (VEC) {
-            return __builtin_bit_cast(Piece, *(Global16 *)(row + (uint64_t)j * sizeof(T)));
-        } else {
-            Piece v;
-            v.v[0] = ((GlobalT *)row)[j];
-            return v;
-        }
-    }
-    // This lane's scores of one step; what lies behind `hi` is a masked score.
+    __device__ __forceinline__ Piece load_whole(uint32_t j) const { return __builtin_bit_cast(Piece, *(Global16 *)(row + (uint64_t)j * sizeof(T))); }
+    // This lane's scores of one step; what lies in front of the row or behind `hi` is a masked score.
     __device__ __forceinline__ Piece load(uint32_t base, uint32_t hi) const
     {
         const uint32_t j = base + lane() * PER;
-        if (j + PER <= hi) return load_whole(j);
+        if (j >= first && j + PER <= hi) return load_whole(j);
         Piece v;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) v.v[e] = j + e < hi ? ((GlobalT *)row)[j + e] : (T)-INFINITY;
+        for (int e = 0; e < PER; ++e) v.v[e] = j + e >= first && j + e < hi ? ((GlobalT *)row)[j + e] : (T)-INFINITY;
         return v;
     }
-    // f(index of the first, scores) for this lane's scores of one step
+    // f(position of the first, scores) for this lane's scores of one step
     template <class F>
     __device__ __forceinline__ void step_of(uint32_t base, const Piece &v, F &&f) const
     {
@@ -590,6 +605,10 @@ struct BlockRow {
                 step_of(base, now, f);
             }
             return;
+        }
+        if (base < first && base < hi) {
+            step_of(base, load(base, hi), f);
+            base += STEP;
         }
 #pragma unroll 1
         for (; base < hi && hi - base >= FLIGHT * STEP; base += FLIGHT * STEP) {
@@ -751,8 +770,8 @@ __device__ __attribute__((noinline)) Drawn list_draw(const Row r, const RowParam
     WaveSet<E> set;
     row.load_list(set);
     double drawn, total;
-    const uint32_t q = set.draw(row.weigh.top, same(p.top_k), same(p.top_p), same(p.min_p), same(p.u), same(p.reach(row.V)), Row::shared().bins, drawn, total);
-    return {Row::shared().list_at[q], (float)(drawn / total)};
+    const uint32_t q = set.draw(row.weigh.top, same(p.top_k), same(p.top_p), same(p.min_p), same(p.u), same(p.reach(row.V - row.first)), Row::shared().bins, drawn, total);
+    return {Row::shared().list_at[q] - row.first, (float)(drawn / total)};
 }
 
 template <class Row, int E>
@@ -844,7 +863,7 @@ __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long l
     return c;
 }
 
-// Index of the r-th (r >= 1) score equal to v.
+// Position of the r-th (r >= 1) score equal to v.
 template <class Row>
 __device__ __attribute__((noinline)) uint32_t nth_equal(const Row r0, float v, uint32_t r)
 {
@@ -892,7 +911,7 @@ __device__ __attribute__((noinline)) uint32_t nth_equal(const Row r0, float v, u
     return at;
 }
 
-// The draw among scores above `edge` and those equal to it up to index last_equal (edge = -inf: all), with weights of at least
+// The draw among scores above `edge` and those equal to it up to position last_equal (edge = -inf: all), with weights of at least
 // `least`, which scores below `from` do not have.
 template <class Row, int THREADS>
 __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, uint32_t last_equal, double least, float from, float u)
@@ -990,7 +1009,7 @@ __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, ui
                 done = run > target;
             }
         }
-        d.at = (uint32_t)__builtin_amdgcn_readlane((int)(j + place), q);
+        d.at = (uint32_t)__builtin_amdgcn_readlane((int)(j + place), q) - row.first;
         d.prob = (float)(lane_of(drawn, q) / total);
     });
     return d;
@@ -1071,20 +1090,22 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     return c;
 }
 
-template <class T, int THREADS, bool VEC>
+template <class T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
 {
-    using Row = BlockRow<T, THREADS, VEC>;
+    using Row = BlockRow<T, THREADS>;
     auto &sh = Row::shared();
     for (uint64_t i = blockIdx.x; i < a.N; i += gridDim.x) {
-        Row row{(uint64_t)((const T *)a.S + i * a.ld), a.V, a.mass_bits, Weigh()};
+        const uint64_t address = (uint64_t)((const T *)a.S + i * a.ld);
+        const uint32_t first = (uint32_t)(address & 15) / (uint32_t)sizeof(T);
+        Row row{address & ~15ull, first, first + a.V, a.mass_bits, Weigh()};
         const RowParams p(a, i);
         Drawn d{0, 0.0f};
         float mine;
         const float top = row.find_top(mine);
         row.weigh = Weigh(top, p.temperature);
         if (top > -INFINITY && p.greedy) {
-            d = Drawn{nth_equal(row, top, 1), 1.0f};
+            d = Drawn{nth_equal(row, top, 1) - first, 1.0f};
         } else if (top > -INFINITY) {
             Cut c{-INFINITY, 0, 0};
             bool done = false;
@@ -1102,7 +1123,7 @@ __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
             }
             if (!done) {
                 if (p.top_p < 1.0f) c = mass_cut<Row, T, THREADS>(row, p.top_p, p.reach(a.V), c);
-                const uint32_t last_equal = c.r < c.ties ? nth_equal(row, c.t, c.r) : a.V;
+                const uint32_t last_equal = c.r < c.ties ? nth_equal(row, c.t, c.r) : 0xFFFFFFFFu;
                 // scores this far below the maximum miss min_p whatever the rounding
                 const double least = p.min_p > 0.0f ? (double)fminf(p.min_p, 1.0f) : 0.0;
                 const float from = p.min_p > 0.0f && top < INFINITY ? top + p.temperature * (__logf((float)least) * 1.001f - 0.001f) : -INFINITY;
@@ -1134,12 +1155,7 @@ hipError_t run_wave(const SampleArgs &a, hipStream_t s)
 template <class T, int THREADS>
 hipError_t run_block(const SampleArgs &a, hipStream_t s)
 {
-    const bool vec = (((uint64_t)(uintptr_t)a.S | a.ld * sizeof(T)) & 15) == 0;
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>(a.N, 1u << 20);
-    if (vec)
-        hipLaunchKernelGGL((k_sample_block<T, THREADS, true>), dim3(blocks), dim3(THREADS), 0, s, a);
-    else
-        hipLaunchKernelGGL((k_sample_block<T, THREADS, false>), dim3(blocks), dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL((k_sample_block<T, THREADS>), dim3((uint32_t)std::min<uint64_t>(a.N, 1u << 20)), dim3(THREADS), 0, s, a);
     return hipGetLastError();
 }
 
