@@ -55,6 +55,15 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k
 
 // w = exp((l - top) / T) = 2^z, z = (l - top) log2(e) / T <= 0: 2^n by the exponent, 2^f, |f| <= 1/2, by the exponential series of
 // f ln 2 to its 12th power (the next term is 1.7e-16); 0 for -inf and NaN, 1 for the maximum itself, also where that is +inf.
+// p f + c with c in scalar registers: left to itself the compiler keeps the constants of a loop in vector registers and copies each
+// before a multiply-add that overwrites it, which is half as many instructions again.
+__device__ __forceinline__ double horner(double p, double f, double c)
+{
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(p), "v"(f), "s"(c));
+    return r;
+}
+
 struct Weigh {
     float top;
     double scale;                       // log2(e) / T
@@ -64,17 +73,17 @@ struct Weigh {
     {
         const double z = fmax(((double)l - (double)top) * scale, -1100.0), n = rint(z), f = z - n;
         double p = 2.5678435993488206e-11;              // ln2^k / k!
-        p = fma(p, f, 4.4455382718708116e-10);
-        p = fma(p, f, 7.0549116208011233e-09);
-        p = fma(p, f, 1.0178086009239700e-07);
-        p = fma(p, f, 1.3215486790144309e-06);
-        p = fma(p, f, 1.5252733804059840e-05);
-        p = fma(p, f, 1.5403530393381609e-04);
-        p = fma(p, f, 1.3333558146428443e-03);
-        p = fma(p, f, 9.6181291076284772e-03);
-        p = fma(p, f, 5.5504108664821580e-02);
-        p = fma(p, f, 2.4022650695910071e-01);
-        p = fma(p, f, 6.9314718055994531e-01);
+        p = horner(p, f, 4.4455382718708116e-10);
+        p = horner(p, f, 7.0549116208011233e-09);
+        p = horner(p, f, 1.0178086009239700e-07);
+        p = horner(p, f, 1.3215486790144309e-06);
+        p = horner(p, f, 1.5252733804059840e-05);
+        p = horner(p, f, 1.5403530393381609e-04);
+        p = horner(p, f, 1.3333558146428443e-03);
+        p = horner(p, f, 9.6181291076284772e-03);
+        p = horner(p, f, 5.5504108664821580e-02);
+        p = horner(p, f, 2.4022650695910071e-01);
+        p = horner(p, f, 6.9314718055994531e-01);
         p = fma(p, f, 1.0);
         const uint64_t w = (uint64_t)__double_as_longlong(ldexp(p, (int)n));
         const uint32_t hi = l == top ? 0x3FF00000u : (uint32_t)(w >> 32);      // (the low half is 0 for the maximum either way)
@@ -244,7 +253,7 @@ struct WaveSet {
             const float at = fminf((high - l[e]) * per, (float)(SET_BINS - 1));
             bin[e] = l[e] == high ? 0u : (uint32_t)at;
             const uint32_t f = (uint32_t)fma(w[e], 0x1p21, 0.5);
-            if (f) atomicAdd(&bins[bin[e]], f);
+            if (f && bin[e] < SET_BINS - 1) atomicAdd(&bins[bin[e]], f);     // (the last bin holds what the others do not, and is not asked)
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const uint4 c = *(const uint4 *)&bins[4 * lane];
@@ -498,7 +507,7 @@ struct BlockShared {
     uint32_t list_at[LIST];
     unsigned long long wide[WAVES], hist_mass[256], above;
     double sums[WAVES];
-    float queue[WAVES][128];            // scores of the draw on their way to a full wave
+    float queue[WAVES][64 + 64 * 8];    // scores of the draw on their way to a full wave
     uint32_t words[WAVES], hist[256];
     __attribute__((aligned(16))) uint32_t bins[SET_BINS];
     uint32_t n, pick, found;
@@ -518,10 +527,12 @@ __device__ __forceinline__ float same(float v) { return __uint_as_float(same(__f
 __device__ __forceinline__ uint64_t same(uint64_t v) { return (uint64_t)same((uint32_t)(v >> 32)) << 32 | same((uint32_t)v); }
 __device__ __forceinline__ double same(double v) { return __longlong_as_double((long long)same((uint64_t)__double_as_longlong(v))); }
 
-// A cut of the order: it ends with the score t, of which r of `ties` are kept.  t = -inf: not cut.
+// A cut of the order: it ends with the score t, of which r of `ties` are kept, the last of them at position `last` (EVERY: all of
+// them; UNKNOWN: it has to be looked for).  t = -inf: not cut.
+constexpr uint32_t EVERY = 0xFFFFFFFFu, UNKNOWN = 0xFFFFFFFEu;
 struct Cut {
     float t;
-    uint32_t r, ties;
+    uint32_t r, ties, last;
 };
 struct Drawn {
     uint32_t at;
@@ -589,7 +600,7 @@ struct BlockRow {
         for (int e = 0; e < PER; ++e) l[e] = widen(v.v[e]);
         f(base + lane() * PER, l);
     }
-    // ... and of all steps of [lo, hi).  FLIGHT steps are on their way at a time: 4 where f is a few instructions; where it
+    // ... and of all steps of [lo, hi).  FLIGHT steps are on their way at a time: 8 where f is a few instructions; where it
     // computes weights, the one next is, which its hundreds of instructions cover.
     template <uint32_t FLIGHT, class F>
     __device__ __forceinline__ void each(uint32_t lo, uint32_t hi, F &&f) const
@@ -636,7 +647,7 @@ struct BlockRow {
         uint32_t lo = 0, hi = V;
         part(lo, hi);
         float high = -INFINITY;
-        each<4>(lo, hi, [&](uint32_t, const float (&l)[PER]) {
+        each<8>(lo, hi, [&](uint32_t, const float (&l)[PER]) {
 #pragma unroll
             for (int e = 0; e < PER; ++e) high = fmaxf(high, l[e]);
         });
@@ -705,7 +716,7 @@ struct BlockRow {
         uint32_t lo = 0, hi = V, n = 0;
         part(lo, hi);
         const uint32_t w = wave();
-        each<4>(lo, hi, [&](uint32_t j, const float (&l)[PER]) {
+        each<8>(lo, hi, [&](uint32_t j, const float (&l)[PER]) {
             bool some = false;
 #pragma unroll
             for (int e = 0; e < PER; ++e) some |= l[e] >= least && l[e] <= most;
@@ -783,6 +794,21 @@ __device__ __attribute__((noinline)) Cut list_cut(const Row r, double border)
     const float high = set.snap_down(INFINITY), low = set.snap_up(-INFINITY);
     Cut c;
     set.cut_mass(same(border), high, high > low ? high - low : 1.0f, c.t, c.r, c.ties, Row::shared().bins);
+    c.last = EVERY;
+    if (c.r < c.ties) {                                // (all of the row's scores equal to t are in the list)
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine += set.l[e] == c.t;
+        uint32_t before = wave_scan(mine) - mine, at = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool eq = set.l[e] == c.t;
+            before += eq;
+            if (eq && before == c.r) at = Row::lane() * E + e + 1;
+        }
+        const uint64_t hit = __ballot(at != 0);
+        c.last = Row::shared().list_at[(uint32_t)__builtin_amdgcn_readlane((int)at, __ffsll((unsigned long long)hit) - 1) - 1];
+    }
     return c;
 }
 
@@ -795,7 +821,7 @@ __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long l
     const Row row = r0.uniform();
     auto &sh = Row::shared();
     border = same((uint64_t)border);
-    const Cut old{same(o.t), same(o.r), same(o.ties)};
+    const Cut old{same(o.t), same(o.r), same(o.ties), 0};
     const uint32_t t = key_of(old.t);
     uint32_t prefix = 0, found = 0;
     bool first = true;
@@ -848,10 +874,10 @@ __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long l
         first = false;
         __syncthreads();
     }
-    if (found == 0) return old;
+    if (found == 0) return o;
     uint32_t nt = prefix << LAST;
     if (!(nt >> 31)) nt |= (1u << LAST) - 1u;          // a negative score: the folded bits are ones
-    Cut c{value_of(nt), 0, found};
+    Cut c{value_of(nt), 0, found, EVERY};
     const uint32_t most = nt == t ? min(found, old.r) : found;               // the border of an earlier cut
     if (MASS) {
         const unsigned long long w = row.fixed(row.weigh(c.t));
@@ -860,6 +886,7 @@ __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long l
     } else {
         c.r = (uint32_t)min((unsigned long long)most, border - before);
     }
+    if (c.r < c.ties) c.last = UNKNOWN;
     return c;
 }
 
@@ -873,7 +900,7 @@ __device__ __attribute__((noinline)) uint32_t nth_equal(const Row r0, float v, u
     r = same(r);
     uint32_t lo = 0, hi = row.V, n = 0;
     Row::part(lo, hi);
-    row.template each<4>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
+    row.template each<8>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
 #pragma unroll
         for (int e = 0; e < Row::PER; ++e) n += l[e] == v;
     });
@@ -946,22 +973,21 @@ __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, ui
             // few scores are in: they queue up until a whole wave of them can be weighed at once
             float *queue = sh.queue[Row::wave()];
             uint32_t n = 0;
-            row.template each<2>(a, b, [&](uint32_t j, const float (&l)[PER]) {
+            row.template each<4>(a, b, [&](uint32_t j, const float (&l)[PER]) {
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    const bool is = in(l[e], j + e);
+                    bool is = l[e] >= floor;
+                    if (last_equal != EVERY) is = is && !(l[e] == edge && j + e > last_equal);
                     const uint64_t m = __ballot(is);
                     if (is) queue[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = l[e];
                     n += __popcll(m);
-                    if (n >= 64) {
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                        mine += weight(queue[Row::lane()]);
-                        const float rest = queue[64 + Row::lane()];
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                        queue[Row::lane()] = rest;
-                        n -= 64;
-                    }
                 }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                while (n >= 64) {                      // from the end: what stays is in front
+                    n -= 64;
+                    mine += weight(queue[n + Row::lane()]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             });
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (Row::lane() < n) mine += weight(queue[Row::lane()]);
@@ -1023,7 +1049,7 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     constexpr int WAVES = THREADS / 64;
     const Row row = r0.uniform();
     auto &sh = Row::shared();
-    const Cut old{same(o.t), same(o.r), same(o.ties)};
+    const Cut old{same(o.t), same(o.r), same(o.ties), 0};
     top_p = same(top_p);
     const float high = row.weigh.top, per = (float)BINS / same(reach);
     auto bin = [&](float l) {
@@ -1032,15 +1058,20 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     };
     for (uint32_t b = threadIdx.x; b < BINS; b += THREADS) sh.mass[b] = 0;
     __syncthreads();
+    // the last bin, most of a row's scores, in registers: its additions would queue at one address
+    unsigned long long rest = 0;
     uint32_t lo = 0, hi = row.V;
     Row::part(lo, hi);
     row.template each<1>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
 #pragma unroll
         for (int e = 0; e < Row::PER; ++e) {
-            const unsigned long long f = row.fixed(row.weigh(l[e]));
-            if (l[e] > old.t && f) atomicAdd(&sh.mass[bin(l[e])], f);          // (of the scores equal to old.t, r are left: added below)
+            const unsigned long long f = l[e] > old.t ? row.fixed(row.weigh(l[e])) : 0;          // (of the scores equal to old.t, r are left: added below)
+            const uint32_t b = bin(l[e]);
+            rest += b == BINS - 1 ? f : 0;
+            if (b < BINS - 1 && f) atomicAdd(&sh.mass[b], f);
         }
     });
+    if (rest) atomicAdd(&sh.mass[BINS - 1], rest);
     __syncthreads();
     if (old.r != 0 && threadIdx.x == 0) sh.mass[bin(old.t)] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
     __syncthreads();
@@ -1082,10 +1113,11 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
             sh.t = c.t;
             sh.pick = c.r;
             sh.found = c.ties;
+            sh.n = c.last;
         }
     }
     __syncthreads();
-    const Cut c{same(sh.t), same(sh.pick), same(sh.found)};
+    const Cut c{same(sh.t), same(sh.pick), same(sh.found), same(sh.n)};
     __syncthreads();
     return c;
 }
@@ -1107,7 +1139,7 @@ __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
         if (top > -INFINITY && p.greedy) {
             d = Drawn{nth_equal(row, top, 1) - first, 1.0f};
         } else if (top > -INFINITY) {
-            Cut c{-INFINITY, 0, 0};
+            Cut c{-INFINITY, 0, 0, EVERY};
             bool done = false;
             if (p.top_k > 0 && p.top_k < a.V) {
                 // The k-th largest of the lanes' own maxima: at least k scores reach it, and few more do, since the largest
@@ -1123,7 +1155,7 @@ __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
             }
             if (!done) {
                 if (p.top_p < 1.0f) c = mass_cut<Row, T, THREADS>(row, p.top_p, p.reach(a.V), c);
-                const uint32_t last_equal = c.r < c.ties ? nth_equal(row, c.t, c.r) : 0xFFFFFFFFu;
+                const uint32_t last_equal = c.last == UNKNOWN ? nth_equal(row, c.t, c.r) : c.last;
                 // scores this far below the maximum miss min_p whatever the rounding
                 const double least = p.min_p > 0.0f ? (double)fminf(p.min_p, 1.0f) : 0.0;
                 const float from = p.min_p > 0.0f && top < INFINITY ? top + p.temperature * (__logf((float)least) * 1.001f - 0.001f) : -INFINITY;
