@@ -101,8 +101,10 @@ __device__ __forceinline__ uint32_t dpp(uint32_t none, uint32_t v)
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp(double v)
 {
+    // (zero where a lane has no source; rows left out keep what they are given, another zero)
     const uint64_t b = (uint64_t)__double_as_longlong(v);
-    const uint32_t lo = dpp<CTRL, ROWS>(0u, (uint32_t)b), hi = dpp<CTRL, ROWS>(0u, (uint32_t)(b >> 32));
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, ROWS == 0xf);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, ROWS == 0xf);
     return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
 __device__ __forceinline__ double last_lane(double v)
@@ -139,20 +141,27 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v)
 }
 __device__ __forceinline__ double wave_total(double v) { return last_lane(wave_scan(v)); }
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63); }
-// (-inf is what a lane without a source sees)
+// A lane without a source keeps its own value.  (In assembler, where the shift is part of the comparison; a value written by the
+// instruction before needs two cycles until other lanes may read it.)
+#define WAVE_EXTREME(op)                                                                                                                          \
+    "s_nop 1\n" op " %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n"                                                                           \
+    "s_nop 1\n" op " %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n"                                                                           \
+    "s_nop 1\n" op " %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n"                                                                           \
+    "s_nop 1\n" op " %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n"                                                                           \
+    "s_nop 1\n" op " %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n"                                                                        \
+    "s_nop 1\n" op " %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf\n"                                                                        \
+    "s_nop 1"
 __device__ __forceinline__ float wave_max(float v)
 {
-    auto f = [](uint32_t x) { return __uint_as_float(x); };
-    constexpr uint32_t NONE = 0xFF800000u;
-    v = fmaxf(v, f(dpp<0x111, 0xf>(NONE, __float_as_uint(v))));
-    v = fmaxf(v, f(dpp<0x112, 0xf>(NONE, __float_as_uint(v))));
-    v = fmaxf(v, f(dpp<0x114, 0xf>(NONE, __float_as_uint(v))));
-    v = fmaxf(v, f(dpp<0x118, 0xf>(NONE, __float_as_uint(v))));
-    v = fmaxf(v, f(dpp<0x142, 0xa>(NONE, __float_as_uint(v))));
-    v = fmaxf(v, f(dpp<0x143, 0xc>(NONE, __float_as_uint(v))));
-    return f((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+    asm(WAVE_EXTREME("v_max_f32_dpp") : "+v"(v));
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
 }
-__device__ __forceinline__ float wave_min(float v) { return -wave_max(-v); }
+__device__ __forceinline__ float wave_min(float v)
+{
+    asm(WAVE_EXTREME("v_min_f32_dpp") : "+v"(v));
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+#undef WAVE_EXTREME
 
 // ---------------------------------------------------------------------------------------------- a wave's set of scores
 // 64 E scores in the order of their index, lane i holding E consecutive ones, weights beside them.  A score that is out (masked,
@@ -185,6 +194,13 @@ struct WaveSet {
 #pragma unroll
         for (int e = 0; e < E; ++e) n += __popcll(__ballot(l[e] == x));
         return n;
+    }
+    __device__ double mass() const
+    {
+        double s = w[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) s += w[e];
+        return wave_total(s);
     }
     __device__ double mass_above(float x) const
     {
@@ -353,7 +369,7 @@ struct WaveSet {
         if (top_p < 1.0f) {
             float t;
             uint32_t r, ties;
-            cut_mass((double)top_p * mass_above(-INFINITY), top, reach, t, r, ties, bins);
+            cut_mass((double)top_p * mass(), top, reach, t, r, ties, bins);
             apply(t, r, ties);
         }
         if (min_p > 0.0f) {
@@ -361,9 +377,9 @@ struct WaveSet {
 #pragma unroll
             for (int e = 0; e < E; ++e) w[e] = w[e] >= least ? w[e] : 0.0;
         }
-        double mine = 0.0;
+        double mine = w[0];
 #pragma unroll
-        for (int e = 0; e < E; ++e) mine += w[e];
+        for (int e = 1; e < E; ++e) mine += w[e];
         const double upto = wave_scan(mine);
         total = last_lane(upto);
         const double target = (double)u * total;
@@ -425,12 +441,15 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
     };
     __shared__ __attribute__((aligned(16))) PerWave sh[WAVE_THREADS / 64];
     PerWave &mine = sh[threadIdx.x >> 6];
-    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t lane = threadIdx.x & 63, j0 = lane * E;
     const uint64_t waves = (uint64_t)gridDim.x * (WAVE_THREADS / 64);
-    for (uint64_t i = (uint64_t)blockIdx.x * (WAVE_THREADS / 64) + (threadIdx.x >> 6); i < a.N; i += waves) {
-        const T *row = (const T *)a.S + i * a.ld;
-        WaveSet<E> set;
-        const uint32_t j0 = lane * E;
+    uint64_t i = (uint64_t)blockIdx.x * (WAVE_THREADS / 64) + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (i >= a.N) return;
+
+    // A row's scores as they come: E consecutive ones a lane, or (where rows do not allow wide loads) 64 consecutive ones a load
+    T raw[E];
+    auto request = [&](uint64_t at) {
+        const T *row = (const T *)a.S + at * a.ld;
         if constexpr (VEC) {
             constexpr int LOAD = 16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E;
 #pragma unroll
@@ -438,26 +457,38 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
                 if (j0 + c + LOAD <= a.V) {
                     const Pack<T, LOAD * (int)sizeof(T)> v = *(const Pack<T, LOAD * (int)sizeof(T)> *)(row + j0 + c);
 #pragma unroll
-                    for (int e = 0; e < LOAD; ++e) set.l[c + e] = fmaxf(widen(v.v[e]), -INFINITY);      // (NaN: -inf)
+                    for (int e = 0; e < LOAD; ++e) raw[c + e] = v.v[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < LOAD; ++e) set.l[c + e] = j0 + c + e < a.V ? fmaxf(widen(row[j0 + c + e]), -INFINITY) : -INFINITY;
+                    for (int e = 0; e < LOAD; ++e) raw[c + e] = j0 + c + e < a.V ? row[j0 + c + e] : (T)-INFINITY;
                 }
             }
         } else {
-            // 64 consecutive scores a load, turned in LDS to E consecutive ones a lane (rows a word longer, so that the lanes'
-            // rows begin in different banks)
+#pragma unroll
+            for (int c = 0; c < E; ++c) raw[c] = c * 64 + lane < a.V ? row[c * 64 + lane] : (T)-INFINITY;
+        }
+    };
+    request(i);
+    for (;;) {
+        WaveSet<E> set;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) set.l[e] = fmaxf(widen(raw[e]), -INFINITY);                       // (NaN: -inf)
+        } else {
+            // turned in LDS to E consecutive ones a lane (rows a word longer, so that the lanes' rows begin in different banks)
             float *turn = mine.turn;
 #pragma unroll
             for (int c = 0; c < E; ++c) {
                 const uint32_t j = c * 64 + lane;
-                turn[j / E * (E + 1) + j % E] = j < a.V ? fmaxf(widen(row[j]), -INFINITY) : -INFINITY;
+                turn[j / E * (E + 1) + j % E] = fmaxf(widen(raw[c]), -INFINITY);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int e = 0; e < E; ++e) set.l[e] = turn[lane * (E + 1) + e];
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+        const bool more = i + waves < a.N;
+        if (more) request(i + waves);                  // on its way while this row is worked on
         const RowParams p(a, i);
         float top = -INFINITY;
 #pragma unroll
@@ -485,6 +516,8 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
             a.idx[i] = at;
             if (a.prob) a.prob[i] = prob;
         }
+        if (!more) return;
+        i += waves;
     }
 }
 
@@ -1176,7 +1209,7 @@ hipError_t run_wave(const SampleArgs &a, hipStream_t s)
     constexpr int LOAD = 16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E;
     const uint64_t align = LOAD * sizeof(T) - 1;
     const bool vec = (((uint64_t)(uintptr_t)a.S | a.ld * sizeof(T)) & align) == 0;
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.N + WAVE_THREADS / 64 - 1) / (WAVE_THREADS / 64), 1u << 20);
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.N + WAVE_THREADS / 64 - 1) / (WAVE_THREADS / 64), 16384);     // row after row, the next on its way
     if (vec)
         hipLaunchKernelGGL((k_sample_wave<T, E, true>), dim3(blocks), dim3(WAVE_THREADS), 0, s, a);
     else
