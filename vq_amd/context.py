@@ -3,6 +3,7 @@ device memory and streams; numpy arrays take the pinned host path of the library
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -22,27 +23,12 @@ def _is_torch(x) -> bool:
     return type(x).__module__.startswith("torch")
 
 
-class _Dtypes:
-    """The element types of scores and tables, asked of torch only when a call needs them."""
+@functools.lru_cache(None)
+def _codes():
+    """torch's element types of scores and tables -> vqhip_dtype"""
+    import torch
 
-    def __iter__(self):
-        import torch
-
-        return iter((torch.float32, torch.bfloat16, torch.float16))
-
-    def __contains__(self, d):
-        return any(d == x for x in self)
-
-
-_DTYPES = _Dtypes()
-
-
-def _dtype(d) -> int:
-    """torch dtype -> vqhip_dtype"""
-    for code, x in enumerate(_DTYPES):
-        if d == x:
-            return code
-    raise ValueError(f"unsupported type {d}")
+    return {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 class Context:
@@ -330,42 +316,35 @@ class Context:
             raise VqhipError(_lib.ERR_STATE, "no prototypes set (vqhip_set_prototypes)")
         N = X.shape[0]
         if out is None:
-            out = torch.empty((N, self.K), dtype=torch.float32, device=X.device)
+            out, ld = torch.empty((N, self.K), dtype=torch.float32, device=X.device), self.K
         else:
-            self._check_rows(out, "out", (N, self.K), (torch.float32,))
-        self._chk(self._L.vqhip_scores_device(self._h, X.data_ptr(), N, out.data_ptr(), self._ld(out), self._stream(X)))
+            self._check_rows(out, "out")
+            ld = self._check_out(out, N, self.K, (torch.float32,))
+        self._chk(self._L.vqhip_scores_device(self._h, X.data_ptr(), N, out.data_ptr(), ld, self._stream()))
         return out
 
     def sample(self, scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """vqhip_sample_device: one index per row of scores (N x V float32, bfloat16 or float16; rows may be strided), drawn from
         softmax(scores / temperature) cut to top_k, top_p and min_p, with the given numbers u (N float32 in [0, 1))
         -> (idx int32, prob float32).  Each parameter is a number or a CUDA tensor of N (float32; top_k int32)."""
-        import torch
-
-        N = self._check_rows(scores, "scores", (None, None), _DTYPES)
-        V = scores.shape[1]
+        N, V, ld, code = self._check_rows(scores, "scores")
         how = self._sampling(N, u, temperature, top_k, top_p, min_p)
-        idx = torch.empty(N, dtype=torch.int32, device=scores.device)
-        prob = torch.empty(N, dtype=torch.float32, device=scores.device)
-        self._chk(self._L.vqhip_sample_device(self._h, scores.data_ptr(), _dtype(scores.dtype), N, V, self._ld(scores), C.byref(how), u.data_ptr(),
-                                              idx.data_ptr(), prob.data_ptr(), self._stream(scores)))
+        idx, prob = self._drawn(N, scores)
+        self._chk(self._L.vqhip_sample_device(self._h, scores.data_ptr(), code, N, V, ld, how, u.data_ptr(), idx.data_ptr(), prob.data_ptr(), self._stream()))
         return idx, prob
 
     def assign_sampled(self, X, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """vqhip_assign_sampled_device: assign with the winner drawn from softmax(-||x - w||^2 / temperature) instead of nearest
         (temperature 0: the nearest) -> (idx int32, prob float32).  Equals sample(scores(X), u, ...)."""
-        import torch
-
         self._check_torch(X)
         N = X.shape[0]
         how = self._sampling(N, u, temperature, top_k, top_p, min_p)
         need = C.c_size_t(0)
-        self._chk(self._L.vqhip_assign_sampled_workspace(self._h, N, C.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=X.device)
-        idx = torch.empty(N, dtype=torch.int32, device=X.device)
-        prob = torch.empty(N, dtype=torch.float32, device=X.device)
-        self._chk(self._L.vqhip_assign_sampled_device(self._h, X.data_ptr(), N, C.byref(how), u.data_ptr(), idx.data_ptr(), prob.data_ptr(),
-                                                      work.data_ptr(), need.value, self._stream(X)))
+        self._chk(self._L.vqhip_assign_sampled_workspace(self._h, N, need))
+        work = self._workspace(need.value, X)
+        idx, prob = self._drawn(N, X)
+        self._chk(self._L.vqhip_assign_sampled_device(self._h, X.data_ptr(), N, how, u.data_ptr(), idx.data_ptr(), prob.data_ptr(), work.data_ptr(),
+                                                      need.value, self._stream()))
         return idx, prob
 
     def lookup(self, idx, table=None, scale=1.0, out=None):
@@ -378,18 +357,17 @@ class Context:
         if table is None:
             if not self.K:
                 raise VqhipError(_lib.ERR_STATE, "no prototypes set (vqhip_set_prototypes)")
-            K, D, ldt, dtype, src = self.K, self.D, self.D, torch.float32, None
+            K, D, ldt, code, dtype, src = self.K, self.D, self.D, _lib.F32, torch.float32, None
         else:
-            K = self._check_rows(table, "table", (None, None), _DTYPES)
-            D, ldt, dtype, src = table.shape[1], self._ld(table), table.dtype, table.data_ptr()
+            K, D, ldt, code = self._check_rows(table, "table")
+            dtype, src = table.dtype, table.data_ptr()
         if out is None:
-            out = torch.empty((*idx.shape, D), dtype=dtype, device=idx.device)
-            ldy = D
+            out, ldy = torch.empty((*idx.shape, D), dtype=dtype, device=idx.device), D
         else:
             rows = self._rows_of(out, "out", idx, D)
-            self._check_rows(rows, "out", (N, D), (dtype,))
-            ldy = self._ld(rows)
-        self._chk(self._L.vqhip_lookup_device(self._h, src, _dtype(dtype), K, D, ldt, idx.data_ptr(), N, scale, out.data_ptr(), ldy, self._stream(idx)))
+            self._check_rows(rows, "out")
+            ldy = self._check_out(rows, N, D, (dtype,))
+        self._chk(self._L.vqhip_lookup_device(self._h, src, code, K, D, ldt, idx.data_ptr(), N, scale, out.data_ptr(), ldy, self._stream()))
         return out
 
     def lookup_gradient(self, grad, idx, K=None, scale=1.0, out=None, accumulate=False, out_dtype=None, want_counts=False):
@@ -400,28 +378,30 @@ class Context:
         import torch
 
         N = self._check_index(idx)
-        if grad.dim() == 0:
+        if not _is_torch(grad) or grad.dim() == 0:
             raise ValueError("grad must have the indices' shape and one more dimension")
         D = grad.shape[-1]
         rows = self._rows_of(grad, "grad", idx, D)
-        self._check_rows(rows, "grad", (N, D), _DTYPES)
+        _, _, ldg, code = self._check_rows(rows, "grad")
         K = self.K if K is None else int(K)
         if K < 1 or D < 1:
             raise ValueError("the table must have at least one row and one column")
         if out is None:
             if accumulate:
                 raise ValueError("accumulate needs out")
-            out = torch.empty((K, D), dtype=out_dtype or torch.float32, device=idx.device)
-        if out_dtype is not None and out.dtype != out_dtype:
-            raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
-        self._check_rows(out, "out", (K, D), (torch.float32, grad.dtype))
+            out, ldt = torch.empty((K, D), dtype=out_dtype or torch.float32, device=idx.device), D
+        else:
+            self._check_rows(out, "out")
+            ldt = self._check_out(out, K, D, (out_dtype or out.dtype,))
+        if out.dtype is not torch.float32 and out.dtype != grad.dtype:
+            raise ValueError(f"the gradient is torch.float32 or {grad.dtype}, not {out.dtype}")
         need = C.c_size_t(0)
-        self._chk(self._L.vqhip_lookup_gradient_workspace(self._h, N, K, D, C.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=idx.device)
+        self._chk(self._L.vqhip_lookup_gradient_workspace(self._h, N, K, D, need))
+        work = self._workspace(need.value, idx)
         counts = torch.empty(K, dtype=torch.int32, device=idx.device) if want_counts else None
-        self._chk(self._L.vqhip_lookup_gradient_device(self._h, rows.data_ptr(), _dtype(grad.dtype), self._ld(rows), idx.data_ptr(), N, scale, K, D,
-                                                       out.data_ptr(), _dtype(out.dtype), self._ld(out), bool(accumulate),
-                                                       counts.data_ptr() if want_counts else None, work.data_ptr(), need.value, self._stream(idx)))
+        self._chk(self._L.vqhip_lookup_gradient_device(self._h, rows.data_ptr(), code, ldg, idx.data_ptr(), N, scale, K, D, out.data_ptr(),
+                                                       _codes()[out.dtype], ldt, bool(accumulate), counts.data_ptr() if want_counts else None,
+                                                       work.data_ptr(), need.value, self._stream()))
         return (out, counts) if want_counts else out
 
     def _sampling(self, N, u, temperature, top_k, top_p, min_p):
@@ -431,57 +411,83 @@ class Context:
         def column(v, name, dtype):
             if not _is_torch(v):
                 return None
-            if not (v.is_cuda and v.device.index == self.device and v.dtype == dtype and v.is_contiguous() and tuple(v.shape) == (N,)):
+            if not (v.get_device() == self.device and v.dtype == dtype and v.is_contiguous() and tuple(v.shape) == (N,)):
                 raise ValueError(f"{name} must be a number or a contiguous CUDA {dtype} tensor of {N} values on cuda:{self.device}")
-            return v.data_ptr()
+            return v.data_ptr() if N else None
 
-        if not _is_torch(u) or column(u, "u", torch.float32) is None:
+        if not _is_torch(u):
             raise ValueError(f"u must be a contiguous CUDA torch.float32 tensor of {N} values on cuda:{self.device}")
+        column(u, "u", torch.float32)
         t, k = column(temperature, "temperature", torch.float32), column(top_k, "top_k", torch.int32)
         p, m = column(top_p, "top_p", torch.float32), column(min_p, "min_p", torch.float32)
-        if k is None and not 0 <= top_k < 1 << 32:
+        if _is_torch(temperature):
+            temperature = 1.0
+        if _is_torch(top_p):
+            top_p = 1.0
+        if _is_torch(min_p):
+            min_p = 0.0
+        if _is_torch(top_k):
+            top_k = 0
+        elif not 0 <= top_k < 1 << 32:
             raise ValueError("top_k must not be negative")
-        return _lib.Sampling(1.0 if t else temperature, 1.0 if p else top_p, 0.0 if m else min_p, 0 if k else int(top_k), t, p, m, k)
+        return _lib.Sampling(temperature, top_p, min_p, int(top_k), t, p, m, k)
 
     @staticmethod
-    def _ld(t):
-        """Elements from one row of a matrix to the next (a single row has none: its width)."""
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-    @staticmethod
-    def _stream(t):
+    def _drawn(N, like):
         import torch
 
-        return torch.cuda.current_stream(t.device).cuda_stream
+        return torch.empty(N, dtype=torch.int32, device=like.device), torch.empty(N, dtype=torch.float32, device=like.device)
+
+    @staticmethod
+    def _workspace(size, like):
+        import torch
+
+        return torch.empty(size, dtype=torch.uint8, device=like.device)
+
+    def _stream(self):
+        """torch's current stream on the context's GPU as the library takes it (an object per call would cost 2 us)."""
+        import torch
+
+        return torch._C._cuda_getCurrentRawStream(self.device)
 
     @staticmethod
     def _rows_of(t, name, idx, D):
         """A tensor of shape idx.shape + (D,) as N rows."""
-        if tuple(t.shape) != (*idx.shape, D):
+        if not _is_torch(t) or t.shape[:-1] != idx.shape or t.shape[-1] != D:
             raise ValueError(f"{name} must be of shape {(*idx.shape, D)}")
         if t.dim() == 2:
             return t
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous unless it is a matrix")
-        return t.view(-1, D) if D else t.reshape(idx.numel(), 0)
+        return t.view(idx.numel(), D)
 
     def _check_index(self, idx):
         import torch
 
-        if not (_is_torch(idx) and idx.is_cuda and idx.device.index == self.device and idx.dtype == torch.int32 and idx.is_contiguous()):
+        if not (_is_torch(idx) and idx.get_device() == self.device and idx.dtype is torch.int32 and idx.is_contiguous()):
             raise ValueError(f"idx must be a contiguous CUDA int32 tensor on cuda:{self.device}")
         return idx.numel()
 
-    def _check_rows(self, t, name, shape, dtypes):
-        """A matrix on the context's GPU whose rows are contiguous and do not overlap -> its number of rows."""
-        if not (_is_torch(t) and t.is_cuda and t.device.index == self.device and t.dtype in dtypes and t.dim() == 2):
-            raise ValueError(f"{name} must be a matrix of {' or '.join(str(d) for d in dtypes)} on cuda:{self.device}")
-        for have, want in zip(t.shape, shape):
-            if want is not None and have != want:
-                raise ValueError(f"{name} must be {shape[0]} x {shape[1]}, not {tuple(t.shape)}")
-        if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    def _check_rows(self, t, name):
+        """A matrix on the context's GPU whose rows are contiguous and do not overlap -> rows, columns, elements from one row to
+        the next (a single row has none: its width), vqhip_dtype."""
+        if not (_is_torch(t) and t.get_device() == self.device and t.dim() == 2):
+            raise ValueError(f"{name} must be a matrix on cuda:{self.device}")
+        code = _codes().get(t.dtype)
+        if code is None:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+        n, width = t.shape
+        ld, step = t.stride()
+        if (width > 1 and step != 1) or (n > 1 and ld < width):
             raise ValueError(f"{name} must have contiguous rows that do not overlap")
-        return t.shape[0]
+        return n, width, ld if n > 1 else width, code
+
+    @staticmethod
+    def _check_out(t, n, width, dtypes):
+        """A matrix of _check_rows that a call writes -> elements from one row to the next."""
+        if tuple(t.shape) != (n, width) or t.dtype not in dtypes:
+            raise ValueError(f"out must be {n} x {width} of {' or '.join(str(d) for d in dtypes)}, not {tuple(t.shape)} of {t.dtype}")
+        return t.stride(0) if n > 1 else width
 
     def _assign_torch(self, X, y, want_dist):
         import torch
