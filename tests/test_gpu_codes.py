@@ -591,3 +591,21 @@ def test_sample_rows_that_begin_anywhere(ctx, V, dtype):
     first[2, V // 2] = 50.0
     idx, _ = ctx.sample(first.cuda(), torch.full((3,), 0.5).cuda(), top_p=0.5)
     assert idx.tolist() == [0, V - 1, V // 2]
+
+
+@pytest.mark.parametrize("N,K,D", [(1, 70000, 3), (64, 64, 64), (1024, 1, 512), (1025, 4096, 24), (4096, 3, 40), (4096, 40000, 96), (4097, 40000, 96), (3001, 997, 515),
+                                   (700, 65, 9000), (4000, 9, 4096), (300, 3000, 3000)])
+@pytest.mark.parametrize("spread", ["even", "one", "few"])
+def test_gradient_on_both_sides_of_one_launch(ctx, N, K, D, spread):
+    """Sizes around the rule for the form that is one launch, with even, single and crowded indices; sums and counts, and a second
+    call that adds to the first's."""
+    g = gen(N + K)
+    grad = torch.randn(N, D, generator=g)
+    idx = torch.randint(-1, K, (N,), generator=g).int()
+    if spread == "one":
+        idx[:] = K // 2
+    if spread == "few":
+        idx = torch.where(torch.rand(N, generator=g) < 0.9, torch.minimum(idx, torch.tensor(2).int()), idx)
+    G, _ = check_gradient(ctx, grad, idx, K, scale=2.0)
+    out = ctx.lookup_gradient(grad.cuda(), idx.cuda(), K=K, scale=2.0, out=G.clone(), accumulate=True)
+    assert torch.equal(out, 2 * G)                                   # x + x is exact
