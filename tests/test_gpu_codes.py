@@ -9,6 +9,8 @@ Tolerances, derived before the first run (a rounding to f32 is off by at most 2^
   gradient  a sum of n values in f32, in any order: at most n 2^-24 of the sum of the absolute values, the scaling 2^-24 more,
             then one rounding to the type, eps/2 of the value (and half the least subnormal)
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -505,7 +507,6 @@ def test_c_refusals(ctx):
                  (p, 0, 5, 4, 4, None, 1, 1.0, p, 4), (p, 0, 5, 4, 4, p, 1, 1.0, None, 4), (p, 0, 5, 4, 4, p, 1, 1.0, p, 3), (None, 1, 5, 4, 4, p, 1, 1.0, p, 4),
                  (None, 0, 6, 4, 4, p, 1, 1.0, p, 4), (p + 2, 0, 5, 4, 4, p, 1, 1.0, p, 4), (p, 0, 5, 4, 4, p + 2, 1, 1.0, p, 4)):
         assert L.vqhip_lookup_device(h, *args, None) == bad, args
-    import ctypes as C
     need = C.c_size_t(0)
     assert L.vqhip_lookup_gradient_workspace(h, 10, 5, 4, C.byref(need)) == 0 and need.value > 0
     assert L.vqhip_lookup_gradient_workspace(h, 1 << 31, 5, 4, C.byref(need)) == bad
@@ -609,3 +610,144 @@ def test_gradient_on_both_sides_of_one_launch(ctx, N, K, D, spread):
     G, _ = check_gradient(ctx, grad, idx, K, scale=2.0)
     out = ctx.lookup_gradient(grad.cuda(), idx.cuda(), K=K, scale=2.0, out=G.clone(), accumulate=True)
     assert torch.equal(out, 2 * G)                                   # x + x is exact
+
+
+# ---------------------------------------------------------------------------------------------- what the calls allow at their ends
+@pytest.mark.parametrize("V", [1500, 9001, 40000])
+@pytest.mark.parametrize("order", ["up", "down", "block", "few values"])
+def test_sample_rows_in_order(ctx, V, order):
+    """The largest scores side by side, so that one wave's part of the row holds all of them, and long runs of equal ones."""
+    g = gen(V)
+    row = torch.randn(V, generator=g) * 3
+    if order != "few values":
+        row = row.sort(descending=order == "down").values
+    if order == "block":
+        row = row.roll(V // 3)
+    if order == "few values":
+        row = torch.randint(0, 5, (V,), generator=g).float()
+    rows = row.repeat(4, 1)
+    u = torch.tensor([0.01, 0.4, 0.77, 0.999])
+    for how in (dict(top_k=100), dict(top_k=129), dict(top_k=256), dict(top_k=257), dict(top_k=700, top_p=0.9), dict(top_p=0.95), dict(top_k=V - 1, top_p=0.5, min_p=0.01)):
+        check_sample(ctx, rows, u, **how)
+
+
+def test_scores_under_capture_need_a_first_call(ctx):
+    g = gen(41)
+    W, X = torch.randn(70, 40, generator=g), torch.randn(500, 40, generator=g).cuda()
+    ctx.set_prototypes(W.numpy())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(VqhipError) as e:
+        with torch.cuda.graph(graph):
+            ctx.scores(X)
+    assert e.value.code == _lib.ERR_STATE
+    torch.cuda.synchronize()
+    want = ctx.scores(X)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ctx.scores(X)
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+    ctx.set_prototypes((W * 2).numpy())                         # the layout follows the model
+    assert (wide(ctx.scores(X)) - ref.scores(X.cpu().numpy(), 2 * W.numpy())).max() < 1e-3
+
+
+def test_contexts_and_streams_at_the_same_time():
+    g = gen(42)
+    W = [torch.randn(300, 64, generator=g), torch.randn(200, 64, generator=g)]
+    X, u = torch.randn(4000, 64, generator=g).cuda(), torch.rand(4000, generator=g).cuda()
+    contexts = [Context(0), Context(0)]
+    want = []
+    for c, w in zip(contexts, W):
+        c.set_prototypes(w.numpy())
+        idx, prob = c.assign_sampled(X, u, temperature=20.0)
+        want.append((idx, prob, c.lookup(idx), c.lookup_gradient(X, idx)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                idx, prob = contexts[k].assign_sampled(X, u, temperature=20.0)
+                got[k].append((idx, prob, contexts[k].lookup(idx), contexts[k].lookup_gradient(X, idx)))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for one in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[k]))
+    for c in contexts:
+        c.close()
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """Rows more than 2^31 elements apart: tables, results and scores that lie far from each other in one allocation of 9 GB."""
+    g = gen(43)
+    far = (1 << 31) + 17
+    buf = torch.zeros(2 * far + 64, dtype=torch.float16, device="cuda")
+    rows = buf.as_strided((3, 50), (far, 1))
+    values = torch.randn(3, 50, generator=g).half()
+    rows.copy_(values.cuda())
+    check_sample(ctx, values, torch.tensor([0.2, 0.5, 0.9]), dev=rows, top_p=0.8)
+    idx = torch.tensor([2, 0, 1, 2], dtype=torch.int32)
+    assert torch.equal(ctx.lookup(idx.cuda(), table=rows).cpu(), values[idx.long()])
+    check_gradient(ctx, values, torch.tensor([1, 0, 1], dtype=torch.int32), 4, dev=rows)
+    rows.zero_()
+    out = ctx.lookup(idx[:3].cuda(), table=values.cuda(), out=rows)
+    assert torch.equal(out.cpu(), values[idx[:3].long()])
+    G = ctx.lookup_gradient(values.cuda(), idx[:3].cuda(), K=3, out=rows)
+    want = torch.zeros(3, 50).half().index_add_(0, idx[:3].long(), values)
+    assert torch.equal(G.cpu(), want)
+    del rows, out, G
+    for D in (8, 40):
+        W, X = torch.randn(30, D, generator=g), torch.randn(3, D, generator=g)
+        ctx.set_prototypes(W.numpy())
+        near = ctx.scores(X.cuda())
+        out = buf.view(torch.float32)
+        far32 = (1 << 30) + 9
+        out = out.as_strided((3, 30), (far32, 1))
+        ctx.scores(X.cuda(), out=out)
+        assert torch.equal(out, near)
+    del buf, out
+    torch.cuda.empty_cache()
+
+
+def test_many_rows_and_few(ctx):
+    """More rows than workgroups or waves are launched for (the kernels walk on), and single ones."""
+    g = gen(44)
+    rows = torch.randn(70000, 5, generator=g)
+    u = torch.rand(70000, generator=g)
+    idx, _ = ctx.sample(rows.cuda(), u.cuda(), top_k=3)
+    for i in (0, 1, 65535, 65536, 69999):
+        assert idx[i].item() == ref.sample_row(rows[i].numpy(), u[i].item(), top_k=3)[0]
+    a, b = ctx.sample(rows.cuda(), u.cuda(), top_p=0.7)
+    c, d = ctx.sample(rows[-7:].cuda(), u[-7:].cuda(), top_p=0.7)
+    assert torch.equal(a[-7:], c) and torch.equal(b[-7:], d)
+
+
+@pytest.mark.parametrize("K,D", [(2000, 2), (1 << 20, 1), (600000, 16), (1, 1)])
+def test_gradient_of_very_many_rows(ctx, K, D):
+    """Above four million rows the sort takes larger tiles; K: 11 digits in one pass, two passes, a table cleared beside the sort, one."""
+    g, N = gen(K), (4 << 20) + 70003
+    grad = torch.randint(-8, 9, (N, D), generator=g).half()                # sums of whole numbers: every order gives the same
+    idx = (torch.rand(N, generator=g) ** 2 * (K + 1)).int() - 1
+    G, counts = ctx.lookup_gradient(grad.cuda(), idx.cuda(), K=K, out_dtype=torch.float32, want_counts=True)
+    named = idx >= 0
+    want = torch.zeros(K, D, dtype=torch.float64).index_add_(0, idx[named].long(), grad[named].double())
+    assert want.abs().max() < 2 ** 24
+    assert torch.equal(G.cpu().double(), want)
+    assert torch.equal(counts.cpu().long(), torch.bincount(idx[named].long(), minlength=K))
+
+
+def test_widest_rows(ctx):
+    D = (1 << 22) - 1                                                       # odd: rows of no common alignment
+    T = torch.arange(2 * D, dtype=torch.int32).remainder(251).half().view(2, D).cuda()
+    idx = torch.tensor([1, 0, -1, 1], dtype=torch.int32, device="cuda")
+    Y = ctx.lookup(idx, table=T)
+    assert torch.equal(Y[0], T[1]) and torch.equal(Y[1], T[0]) and not Y[2].any() and torch.equal(Y[3], T[1])
+    G = ctx.lookup_gradient(Y, idx, K=3, out_dtype=torch.float16)
+    assert torch.equal(G[1], 2 * T[1]) and torch.equal(G[0], T[0]) and not G[2].any()
+    L, need = _lib.lib(), C.c_size_t(0)
+    for D, code in ((1 << 22, _lib.OK), ((1 << 22) + 1, _lib.ERR_INVALID)):
+        assert L.vqhip_lookup_gradient_workspace(ctx._h, 4, 3, D, need) == code
+        assert L.vqhip_lookup_device(ctx._h, T.data_ptr(), _lib.F16, 1, D, D, idx.data_ptr(), 0, 1.0, Y.data_ptr(), D, None) == code

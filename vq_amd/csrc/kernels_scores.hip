@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
     uint32_t n = 0;
     auto finish = [&](auto bounded) {
         float *const out = a.S + wrow * a.ld + wcol;
-        const uint32_t at = (uint32_t)(4 * half * a.ld) + l31;
+        const size_t at = 4 * half * a.ld + l31;
 #pragma unroll
         for (int j = 0; j < CW; ++j) {
             const float w2 = nw[wc * NT + j * 32 + l31];
