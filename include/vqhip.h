@@ -310,7 +310,7 @@ int vqhip_assign_sampled_device(vqhip_ctx *ctx, const float *dX, uint64_t N, con
 
 /* Y[i] = scale * T[idx[i]] for N indices: T is K x D of `dtype`, rows ldt apart, Y is N x D of the same type, rows ldy apart.  An
  * index outside [0, K) (VQHIP_NO_INDEX for padding) gives a row of zeros.  dT == NULL: the context's prototypes (f32; K, D and
- * ldt must be the model's). The product is formed in f32 and rounded once. */
+ * ldt must be the model's).  K below 2^31, D at most 2^22.  The product is formed in f32 and rounded once. */
 #define VQHIP_NO_INDEX 0xFFFFFFFFu
 int vqhip_lookup_device(vqhip_ctx *ctx, const void *dT, int dtype, uint32_t K, uint32_t D, uint64_t ldt, const uint32_t *didx, uint64_t N,
                         float scale, void *dY, uint64_t ldy, void *stream);
@@ -320,7 +320,7 @@ int vqhip_lookup_device(vqhip_ctx *ctx, const void *dT, int dtype, uint32_t K, u
  * N x D of `dtype`, rows ldy apart; out_dtype is VQHIP_F32 or `dtype`.  dcounts (nullable): how many indices name each row, so
  * that sums and counts of the samples of every code (the batch update of a codebook) are one call with scale 1.  Indices
  * outside [0, K) contribute nothing; their rows of dY are not read.  Sums are f32 in an order the inputs alone fix: the same
- * inputs give the same bits.  N below 2^31, K in [1, 2^31).  dwork: vqhip_lookup_gradient_workspace bytes, 256-byte aligned,
+ * inputs give the same bits.  N and K below 2^31, D at most 2^22.  dwork: vqhip_lookup_gradient_workspace bytes, 256-byte aligned,
  * free for other use once the call has run. */
 int vqhip_lookup_gradient_workspace(vqhip_ctx *ctx, uint64_t N, uint32_t K, uint32_t D, size_t *bytes);
 int vqhip_lookup_gradient_device(vqhip_ctx *ctx, const void *dY, int dtype, uint64_t ldy, const uint32_t *didx, uint64_t N, float scale, uint32_t K,

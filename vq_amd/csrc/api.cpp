@@ -1430,7 +1430,7 @@ int vqhip_lookup_device(vqhip_ctx *c, const void *dT, int dtype, uint32_t K, uin
 try {
     if (!c) return VQHIP_ERR_INVALID;
     if (!dtype_bytes(dtype)) return c->fail(VQHIP_ERR_INVALID, "lookup_device: unknown dtype");
-    if (K == 0 || K >= (1u << 31) || D == 0 || D > (1u << 24)) return c->fail(VQHIP_ERR_INVALID, "lookup_device: K must lie in [1, 2^31), D in [1, 2^24]");
+    if (K == 0 || K >= (1u << 31) || D == 0 || D > (1u << 22)) return c->fail(VQHIP_ERR_INVALID, "lookup_device: K must lie in [1, 2^31), D in [1, 2^22]");
     if (!dT) {
         if (c->K == 0 || !c->dW) return c->fail(VQHIP_ERR_STATE, "no prototypes set (vqhip_set_prototypes)");
         if (dtype != VQHIP_F32 || K != c->K || D != c->D || ldt != c->D)
@@ -1451,7 +1451,7 @@ VQHIP_CATCH(c)
 
 static int check_gradient_shape(vqhip_ctx *c, uint64_t N, uint32_t K, uint32_t D)
 {
-    if (K == 0 || K >= (1u << 31) || D == 0 || D > (1u << 24)) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient: K must lie in [1, 2^31), D in [1, 2^24]");
+    if (K == 0 || K >= (1u << 31) || D == 0 || D > (1u << 22)) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient: K must lie in [1, 2^31), D in [1, 2^22]");
     if (N >= (1ull << 31)) return c->fail(VQHIP_ERR_INVALID, "lookup_gradient: N must be below 2^31");
     return VQHIP_OK;
 }
