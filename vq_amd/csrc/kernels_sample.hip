@@ -1040,6 +1040,7 @@ __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, ui
             pick = k;
             if (before + sh.sums[k] > target) break;
         }
+        pick = max(pick, 0);                           // (the maximum is always in: there is a sum)
         const uint32_t steps = (hi - lo + Row::STEP - 1) / Row::STEP, len = (steps + WAVES - 1) / WAVES * Row::STEP;
         lo = same(lo + (uint32_t)pick * len);
         hi = same((uint32_t)min((uint64_t)lo + len, (uint64_t)hi));
