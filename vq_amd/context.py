@@ -367,7 +367,7 @@ class Context:
             rows = self._rows_of(out, "out", idx, D)
             self._check_rows(rows, "out")
             ldy = self._check_out(rows, N, D, (dtype,))
-        self._chk(self._L.vqhip_lookup_device(self._h, src, code, K, D, ldt, idx.data_ptr(), N, scale, out.data_ptr(), ldy, self._stream()))
+        self._chk(self._L.vqhip_lookup_device(self._h, src, code, K, D, ldt, idx.data_ptr(), N, float(scale), out.data_ptr(), ldy, self._stream()))
         return out
 
     def lookup_gradient(self, grad, idx, K=None, scale=1.0, out=None, accumulate=False, out_dtype=None, want_counts=False):
@@ -399,7 +399,7 @@ class Context:
         self._chk(self._L.vqhip_lookup_gradient_workspace(self._h, N, K, D, need))
         work = self._workspace(need.value, idx)
         counts = torch.empty(K, dtype=torch.int32, device=idx.device) if want_counts else None
-        self._chk(self._L.vqhip_lookup_gradient_device(self._h, rows.data_ptr(), code, ldg, idx.data_ptr(), N, scale, K, D, out.data_ptr(),
+        self._chk(self._L.vqhip_lookup_gradient_device(self._h, rows.data_ptr(), code, ldg, idx.data_ptr(), N, float(scale), K, D, out.data_ptr(),
                                                        _codes()[out.dtype], ldt, bool(accumulate), counts.data_ptr() if want_counts else None,
                                                        work.data_ptr(), need.value, self._stream()))
         return (out, counts) if want_counts else out
@@ -430,7 +430,7 @@ class Context:
             top_k = 0
         elif not 0 <= top_k < 1 << 32:
             raise ValueError("top_k must not be negative")
-        return _lib.Sampling(temperature, top_p, min_p, int(top_k), t, p, m, k)
+        return _lib.Sampling(float(temperature), float(top_p), float(min_p), int(top_k), t, p, m, k)
 
     @staticmethod
     def _drawn(N, like):
