@@ -751,3 +751,13 @@ def test_widest_rows(ctx):
     for D, code in ((1 << 22, _lib.OK), ((1 << 22) + 1, _lib.ERR_INVALID)):
         assert L.vqhip_lookup_gradient_workspace(ctx._h, 4, 3, D, need) == code
         assert L.vqhip_lookup_device(ctx._h, T.data_ptr(), _lib.F16, 1, D, D, idx.data_ptr(), 0, 1.0, Y.data_ptr(), D, None) == code
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sample_very_long_rows(ctx, dtype):
+    """Long beyond every vocabulary: spread ones, and all of them equal, where the order among equal ones decides."""
+    g, V = gen(45), 500_009
+    rows = torch.stack([torch.randn(V, generator=g) * 4, torch.full((V,), -2.5)]).to(TYPES[dtype])
+    u = torch.tensor([0.37, 0.61])
+    for how in (dict(), dict(top_p=0.9), dict(top_k=100000, top_p=0.5), dict(top_k=200), dict(min_p=0.05)):
+        check_sample(ctx, rows, u, **how)
