@@ -761,3 +761,20 @@ def test_sample_very_long_rows(ctx, dtype):
     u = torch.tensor([0.37, 0.61])
     for how in (dict(), dict(top_p=0.9), dict(top_k=100000, top_p=0.5), dict(top_k=200), dict(min_p=0.05)):
         check_sample(ctx, rows, u, **how)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [1100, 9001])
+def test_sample_cuts_beyond_the_list(ctx, V, dtype):
+    """Counts above what a list of the largest holds, alone and before a nucleus, among spread scores, few values, values around
+    zero and values that are all in one power of two."""
+    g = gen(V + 1)
+    least = torch.finfo(TYPES[dtype]).smallest_normal
+    tiny = torch.tensor([0.0, -0.0, least, -least, least / 4, -least / 4])
+    rows = torch.stack([torch.randn(V, generator=g) * 3, torch.randint(-3, 3, (V,), generator=g).float(), tiny[torch.randint(0, 6, (V,), generator=g)],
+                        1.0 + torch.rand(V, generator=g), -1.0 - torch.rand(V, generator=g) * 2.0 ** -6]).to(TYPES[dtype])
+    rows[:, 11:: 13] = -INF
+    u = torch.tensor([0.05, 0.5, 0.8, 0.97, 0.3])
+    for how in (dict(top_k=209), dict(top_k=353), dict(top_k=600), dict(top_k=V - 200), dict(top_k=V - 1), dict(top_k=600, top_p=0.9), dict(top_k=600, top_p=0.999),
+                dict(top_k=900, top_p=0.3), dict(top_k=208, top_p=0.7)):
+        check_sample(ctx, rows, u, **how)

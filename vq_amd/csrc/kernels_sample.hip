@@ -538,7 +538,7 @@ struct BlockShared {
     };
     float list_l[LIST];
     uint32_t list_at[LIST];
-    unsigned long long wide[WAVES], hist_mass[256], above;
+    unsigned long long wide[WAVES], above, own;
     double sums[WAVES];
     float queue[WAVES][64 + 64 * 8];    // scores of the draw on their way to a full wave
     uint32_t words[WAVES], hist[256];
@@ -741,6 +741,52 @@ struct BlockRow {
         return 255 - 4 * q - at;
     }
 
+    // Over sh.mass, whose bins are in the order of falling scores: this lane's consecutive bins, what lies in front of them and the sum
+    // of all.
+    struct Totals {
+        unsigned long long before, own, all;
+    };
+    __device__ __forceinline__ Totals totals() const
+    {
+        auto &sh = shared();
+        constexpr uint32_t EACH = BINS / THREADS;
+        Totals n{0, 0, 0};
+#pragma unroll
+        for (uint32_t e = 0; e < EACH; ++e) n.own += sh.mass[threadIdx.x * EACH + e];
+        unsigned long long upto = n.own;
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned long long y = __shfl_up(upto, o);
+            if ((int)lane() >= o) upto += y;
+        }
+        if (lane() == 63) sh.wide[wave()] = upto;
+        __syncthreads();
+        n.before = upto - n.own;
+        for (int k = 0; k < WAVES; ++k) {
+            n.before += k < (int)wave() ? sh.wide[k] : 0;
+            n.all += sh.wide[k];
+        }
+        return n;
+    }
+    // The bin that brings the running total to `border` (1 <= border <= the sum of all), what lies in front of it, and its own.
+    __device__ __forceinline__ uint32_t border_of(const Totals &n, unsigned long long border, unsigned long long &above, unsigned long long &own) const
+    {
+        auto &sh = shared();
+        if (n.before < border && border <= n.before + n.own) {
+            unsigned long long before = n.before;
+            uint32_t b = threadIdx.x * (BINS / THREADS);
+            while (before + sh.mass[b] < border) before += sh.mass[b++];
+            sh.pick = b;
+            sh.above = before;
+            sh.own = sh.mass[b];
+        }
+        __syncthreads();
+        const uint32_t at = same(sh.pick);
+        above = same((uint64_t)sh.above);
+        own = same((uint64_t)sh.own);
+        __syncthreads();
+        return at;
+    }
+
     // The scores in [least, most] that `in` says, in the order of their index, into the list.  False if they do not fit.
     template <class P>
     __device__ __forceinline__ bool collect(float least, float most, P &&in) const
@@ -791,7 +837,7 @@ struct BlockRow {
     }
 
     // The list as a wave's set.
-    template <int E>
+    template <int E, bool WEIGH = true>
     __device__ __forceinline__ void load_list(WaveSet<E> &set) const
     {
         auto &sh = shared();
@@ -801,7 +847,7 @@ struct BlockRow {
             const uint32_t q = lane() * E + e;
             set.l[e] = q < n ? sh.list_l[q] : -INFINITY;
         }
-        set.weigh_all(weigh);
+        if (WEIGH) set.weigh_all(weigh);
     }
 };
 
@@ -818,15 +864,19 @@ __device__ __attribute__((noinline)) Drawn list_draw(const Row r, const RowParam
     return {Row::shared().list_at[q] - row.first, (float)(drawn / total)};
 }
 
-template <class Row, int E>
+template <class Row, int E, bool MASS>
 __device__ __attribute__((noinline)) Cut list_cut(const Row r, double border)
 {
     const Row row = r.uniform();
     WaveSet<E> set;
-    row.load_list(set);
-    const float high = set.snap_down(INFINITY), low = set.snap_up(-INFINITY);
+    row.template load_list<E, MASS>(set);
     Cut c;
-    set.cut_mass(same(border), high, high > low ? high - low : 1.0f, c.t, c.r, c.ties, Row::shared().bins);
+    if (MASS) {
+        const float high = set.snap_down(INFINITY), low = set.snap_up(-INFINITY);
+        set.cut_mass(same(border), high, high > low ? high - low : 1.0f, c.t, c.r, c.ties, Row::shared().bins);
+    } else {
+        set.cut_count((uint32_t)same(border), c.t, c.r, c.ties);
+    }
     c.last = EVERY;
     if (c.r < c.ties) {                                // (all of the row's scores equal to t are in the list)
         uint32_t mine = 0;
@@ -845,9 +895,30 @@ __device__ __attribute__((noinline)) Cut list_cut(const Row r, double border)
     return c;
 }
 
-// Radix selection over the whole row, 8 bits of the ordered key at a time, for the rows the list does not serve (top_k beyond it,
-// a border among more equal or nearly equal scores than it holds).  `old`: an earlier cut.  By count: the first `border`.  By
-// mass: those whose mass before them is below it.
+// The cut among the scores of the list, by the first wave, told to all.
+template <class Row, bool MASS>
+__device__ __forceinline__ Cut cut_of_list(const Row row, double border)
+{
+    auto &sh = Row::shared();
+    if (threadIdx.x < 64) {
+        const Cut c = sh.n <= 256 ? list_cut<Row, 4, MASS>(row, border) : list_cut<Row, 8, MASS>(row, border);
+        if (threadIdx.x == 0) {
+            sh.t = c.t;
+            sh.pick = c.r;
+            sh.found = c.ties;
+            sh.n = c.last;
+        }
+    }
+    __syncthreads();
+    const Cut c{same(sh.t), same(sh.pick), same(sh.found), same(sh.n)};
+    __syncthreads();
+    return c;
+}
+
+// Radix selection over the whole row, up to 11 bits of the ordered key at a time, for the rows the list does not serve at once
+// (top_k beyond it, a border among more equal or nearly equal scores than it holds).  `old`: an earlier cut.  By count: the
+// first `border`; by mass: those whose mass before them is below it.  (Digits of 8 bits are the sign and seven of the exponent
+// first: a handful of bins, at whose addresses the additions queue.)
 template <class Row, class T, int THREADS, bool MASS>
 __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long long border, const Cut o)
 {
@@ -856,68 +927,71 @@ __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long l
     border = same((uint64_t)border);
     const Cut old{same(o.t), same(o.r), same(o.ties), 0};
     const uint32_t t = key_of(old.t);
-    uint32_t prefix = 0, found = 0;
-    bool first = true;
-    unsigned long long before = 0;
     // the low bits of a widened 16-bit score follow from its sign: 16 of them for bf16, 13 for f16
-    constexpr int LAST = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 16 : 8;
+    constexpr int LAST = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 16 : 13;
+    uint32_t prefix = 0;
+    unsigned long long above = 0, own = 0;
+    int shift = 32;
+    bool listed = false;
 #pragma unroll 1
-    for (int shift = 24; shift >= LAST; shift -= 8) {
-        if (threadIdx.x < 256) {
-            sh.hist[threadIdx.x] = 0;
-            sh.hist_mass[threadIdx.x] = 0;
-        }
+    while (shift > LAST) {
+        const int from = shift, bits = min(11, from - LAST);
+        shift -= bits;
+        for (uint32_t b = threadIdx.x; b < BINS; b += THREADS) sh.mass[b] = 0;
         __syncthreads();
+        const uint32_t mask = (1u << bits) - 1;
+        auto ours = [&](uint32_t k) { return from == 32 || (k >> (from & 31)) == prefix; };
         uint32_t lo = 0, hi = row.V;
         Row::part(lo, hi);
-        row.template each<1>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
+        row.template each<MASS ? 1 : 4>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
 #pragma unroll
             for (int e = 0; e < Row::PER; ++e) {
                 const uint32_t k = key_of(l[e]);
-                if (k < t || k <= KEY_LEAST || (!first && (k >> (shift + 8)) != prefix)) continue;
-                const uint32_t b = (k >> shift) & 255;
-                atomicAdd(&sh.hist[b], 1u);
-                if (MASS && k > t) atomicAdd(&sh.hist_mass[b], row.fixed(row.weigh(l[e])));
+                if (k <= KEY_LEAST || k < t || (MASS && k == t) || !ours(k)) continue;
+                atomicAdd(&sh.mass[mask - ((k >> shift) & mask)], MASS ? row.fixed(row.weigh(l[e])) : 1ull);
             }
         });
         __syncthreads();
-        if (threadIdx.x == 0) {
-            // of the scores equal to t only r are left
-            if (MASS && old.r != 0 && (first || (t >> (shift + 8)) == prefix)) sh.hist_mass[(t >> shift) & 255] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
-            // the bin of the last score kept: the lowest whose total above it is below the border
-            unsigned long long run = before, above = before;
-            uint32_t pick = 0;
-            bool any = false;
-            for (int b = 255; b >= 0; --b) {
-                if (sh.hist[b] == 0) continue;
-                if (run >= border && any) break;
-                any = true;
-                pick = b;
-                above = run;
-                run += MASS ? sh.hist_mass[b] : sh.hist[b];
-            }
-            sh.pick = pick;
-            sh.above = above;
-            sh.found = any ? sh.hist[pick] : 0;
+        if (MASS && old.r != 0 && ours(t)) {           // of the scores equal to t only r are left
+            if (threadIdx.x == 0) sh.mass[mask - ((t >> shift) & mask)] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
+            __syncthreads();
         }
-        __syncthreads();
-        prefix = (prefix << 8) | same(sh.pick);
-        before = same((uint64_t)sh.above);
-        found = same(sh.found);
-        first = false;
-        __syncthreads();
+        const typename Row::Totals n = row.totals();
+        const unsigned long long rest = border - above;
+        if (rest > n.all) return o;                    // (by count: the row has no more)
+        unsigned long long front;
+        const uint32_t d = mask - row.border_of(n, rest, front, own);
+        prefix = from == 32 ? d : prefix << bits | d;
+        above += front;
+        if (!MASS && shift > LAST && own <= LIST && !listed) {               // few are left: to the list (once: one wave may hold too many of them)
+            listed = true;
+            const uint32_t first = max(prefix << shift, KEY_LEAST + 1), last = min(prefix << shift | ((1u << shift) - 1), key_of(INFINITY));
+            if (row.collect(value_of(first), value_of(last), [&](float l) { return key_of(l) >> shift == prefix; })) return cut_of_list<Row, false>(row, (double)(border - above));
+        }
     }
-    if (found == 0) return o;
     uint32_t nt = prefix << LAST;
     if (!(nt >> 31)) nt |= (1u << LAST) - 1u;          // a negative score: the folded bits are ones
-    Cut c{value_of(nt), 0, found, EVERY};
-    const uint32_t most = nt == t ? min(found, old.r) : found;               // the border of an earlier cut
+    Cut c{value_of(nt), 0, 0, EVERY};
+    uint32_t lo = 0, hi = row.V, ties = 0;
     if (MASS) {
+        Row::part(lo, hi);
+        row.template each<8>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
+#pragma unroll
+            for (int e = 0; e < Row::PER; ++e) ties += l[e] == c.t;
+        });
+        ties = wave_total(ties);
+        if (Row::lane() == 0) sh.words[Row::wave()] = ties;
+        __syncthreads();
+        for (int k = 0; k < Row::WAVES; ++k) c.ties += sh.words[k];
+        __syncthreads();
+        c.ties = same(c.ties);
+        const uint32_t most = nt == t ? min(c.ties, old.r) : c.ties;         // the border of an earlier cut
         const unsigned long long w = row.fixed(row.weigh(c.t));
-        c.r = border <= before ? 1 : w == 0 ? most : (uint32_t)min((unsigned long long)most, (border - before + w - 1) / w);
+        c.r = (uint32_t)min((unsigned long long)most, (border - above + w - 1) / max(w, 1ull));
         c.r = max(c.r, 1u);
     } else {
-        c.r = (uint32_t)min((unsigned long long)most, border - before);
+        c.ties = (uint32_t)own;
+        c.r = (uint32_t)(border - above);
     }
     if (c.r < c.ties) c.last = UNKNOWN;
     return c;
@@ -1080,7 +1154,6 @@ __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, ui
 template <class Row, class T, int THREADS>
 __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, float reach, const Cut o)
 {
-    constexpr int WAVES = THREADS / 64;
     const Row row = r0.uniform();
     auto &sh = Row::shared();
     const Cut old{same(o.t), same(o.r), same(o.ties), 0};
@@ -1109,51 +1182,16 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     __syncthreads();
     if (old.r != 0 && threadIdx.x == 0) sh.mass[bin(old.t)] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
     __syncthreads();
-    // running totals of the bins
-    constexpr uint32_t EACH = BINS / THREADS;
-    unsigned long long sum = 0;
-#pragma unroll
-    for (uint32_t e = 0; e < EACH; ++e) sum += sh.mass[threadIdx.x * EACH + e];
-    unsigned long long upto = sum;
-    for (int o1 = 1; o1 < 64; o1 <<= 1) {
-        const unsigned long long y = __shfl_up(upto, o1);
-        if ((int)Row::lane() >= o1) upto += y;
-    }
-    if (Row::lane() == 63) sh.wide[Row::wave()] = upto;
-    __syncthreads();
-    unsigned long long before = upto - sum, z = 0;
-    for (int k = 0; k < WAVES; ++k) {
-        before += k < (int)Row::wave() ? sh.wide[k] : 0;
-        z += sh.wide[k];
-    }
-    const unsigned long long border = same((uint64_t)ceil((double)top_p * (double)z));
-    if (before < border && border <= before + sum) {
-        uint32_t b = threadIdx.x * EACH;
-        while (before + sh.mass[b] < border) before += sh.mass[b++];
-        sh.pick = b;
-        sh.above = before;
-    }
-    __syncthreads();
-    const uint32_t at_bin = same(sh.pick);
-    const unsigned long long above = same((uint64_t)sh.above);
+    const typename Row::Totals n = row.totals();
+    const unsigned long long border = same((uint64_t)ceil((double)top_p * (double)n.all));
+    unsigned long long above, own;
+    const uint32_t at_bin = row.border_of(n, border, above, own);
     // (half a bin to spare on either side: the exact answer is bin()'s)
     const float step = 1.0f / per, most = high - ((float)at_bin - 0.5f) * step;
     const float least = at_bin + 1 < BINS ? high - ((float)at_bin + 1.5f) * step : -FLT_MAX;
-    if (old.r != 0 || !row.collect(least, most, [&](float l) { return bin(l) == at_bin; })) return radix_cut<Row, T, THREADS, true>(row, border, old);
-    if (threadIdx.x < 64) {
-        const double room = (double)(border - above) * __longlong_as_double((long long)(1023 - row.s) << 52);
-        const Cut c = sh.n <= 256 ? list_cut<Row, 4>(row, room) : list_cut<Row, 8>(row, room);
-        if (threadIdx.x == 0) {
-            sh.t = c.t;
-            sh.pick = c.r;
-            sh.found = c.ties;
-            sh.n = c.last;
-        }
-    }
-    __syncthreads();
-    const Cut c{same(sh.t), same(sh.pick), same(sh.found), same(sh.n)};
-    __syncthreads();
-    return c;
+    // (where the border of an earlier cut is in the step too, not all that are equal to it are in)
+    if ((old.r != 0 && bin(old.t) == at_bin) || !row.collect(least, most, [&](float l) { return bin(l) == at_bin; })) return radix_cut<Row, T, THREADS, true>(row, border, old);
+    return cut_of_list<Row, true>(row, (double)(border - above) * __longlong_as_double((long long)(1023 - row.s) << 52));
 }
 
 template <class T, int THREADS>
@@ -1177,8 +1215,9 @@ __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
             bool done = false;
             if (p.top_k > 0 && p.top_k < a.V) {
                 // The k-th largest of the lanes' own maxima: at least k scores reach it, and few more do, since the largest
-                // scores rarely share a lane.
-                if (p.top_k <= (THREADS < 1024 ? THREADS / 2 : 256)) {
+                // scores rarely share a lane: of scores in no order -n ln(1 - k / n) for n lanes, which is 430 of the 512 the
+                // list holds at these k.
+                if (p.top_k <= (THREADS < 1024 ? 208 : 352)) {
                     const uint32_t least = max(row.kth_largest(key_of(mine), p.top_k), KEY_LEAST + 1);
                     if (row.collect(value_of(least), INFINITY, [](float) { return true; })) {
                         if (threadIdx.x < 64) d = sh.n <= 256 ? list_draw<Row, 4>(row, p) : list_draw<Row, 8>(row, p);
