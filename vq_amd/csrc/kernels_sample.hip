@@ -64,11 +64,22 @@ __device__ __forceinline__ double horner(double p, double f, double c)
     return r;
 }
 
+// 1 / x to ~2^-46 for x in [2^-149, 2^128): the instruction's 23 bits and one step of Newton's.  A division is eleven instructions.
+__device__ __forceinline__ double inverse(double x)
+{
+    const double r = __builtin_amdgcn_rcp(x);
+    return fma(fma(-x, r, 1.0), r, r);
+}
+
 struct Weigh {
     float top;
     double scale;                       // log2(e) / T
     __device__ Weigh() {}
-    __device__ Weigh(float maximum, float temperature) : top(maximum), scale(1.4426950408889634 / (double)temperature) {}
+    __device__ Weigh(float maximum, float temperature) : top(maximum)
+    {
+        const double r = inverse((double)temperature), q = 1.4426950408889634 * r;
+        scale = fma(fma(-(double)temperature, q, 1.4426950408889634), r, q);
+    }
     __device__ __forceinline__ double operator()(float l) const
     {
         const double z = fmax(((double)l - (double)top) * scale, -1100.0), n = rint(z), f = z - n;
@@ -139,7 +150,17 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v)
     v += dpp<0x143, 0xc>(0u, v);
     return v;
 }
-__device__ __forceinline__ double wave_total(double v) { return last_lane(wave_scan(v)); }
+__device__ __forceinline__ double wave_total(double v)
+{
+    // (as the scan, but that only the last lane has to be right: the rows in between may add what they like)
+    v += dpp<0x111, 0xf>(v);
+    v += dpp<0x112, 0xf>(v);
+    v += dpp<0x114, 0xf>(v);
+    v += dpp<0x118, 0xf>(v);
+    v += dpp<0x142, 0xf>(v);
+    v += dpp<0x143, 0xf>(v);
+    return last_lane(v);
+}
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63); }
 // A lane without a source keeps its own value.  (In assembler, where the shift is part of the comparison; a value written by the
 // instruction before needs two cycles until other lanes may read it.)
@@ -176,10 +197,12 @@ struct WaveSet {
     __device__ __forceinline__ void weigh_all(const Weigh &weigh)
     {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            w[e] = weigh(l[e]);
-            l[e] = w[e] > 0.0 ? l[e] : -INFINITY;
-        }
+        for (int e = 0; e < E; ++e) w[e] = weigh(l[e]);
+    }
+    __device__ __forceinline__ void drop_weightless()
+    {
+#pragma unroll
+        for (int e = 0; e < E; ++e) l[e] = w[e] > 0.0 ? l[e] : -INFINITY;
     }
     __device__ uint32_t count_above(float x) const
     {
@@ -254,22 +277,22 @@ struct WaveSet {
 
     // A bracket for cut_mass by a histogram over even steps of the score, `span` of it in all, from the maximum `high` down.  Its
     // masses are integers, w 2^21 rounded, which at most 1024 of them put at most 512 off: with 600 to spare on either side
-    // the border lies in the bins found, whatever their order of addition.
-    __device__ __forceinline__ void narrow(double border, float high, float span, float &lo, float &hi, uint32_t *bins) const
+    // the border lies in the bins found, whatever their order of addition.  True if they hold one score alone, the last one
+    // kept: hi.
+    __device__ __forceinline__ bool narrow(double border, float high, float span, float &lo, float &hi, uint32_t *bins) const
     {
         static_assert(E <= 16, "at most 1024 scores");
-        const float per = (float)SET_BINS / span;
+        const float per = (float)SET_BINS * __builtin_amdgcn_rcpf(span);
         const uint32_t lane = threadIdx.x & 63;
         *(uint4 *)&bins[4 * lane] = make_uint4(0, 0, 0, 0);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         uint32_t bin[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            // (a maximum or a step beyond all bounds: 0 * inf and the like go to the last bin, but for the maximum itself)
-            const float at = fminf((high - l[e]) * per, (float)(SET_BINS - 1));
-            bin[e] = l[e] == high ? 0u : (uint32_t)at;
+            // (a maximum or a step beyond all bounds: inf - inf and 0 * inf go to the first bin)
+            bin[e] = (uint32_t)fminf(fmaxf((high - l[e]) * per, 0.0f), (float)(SET_BINS - 1));
             const uint32_t f = (uint32_t)fma(w[e], 0x1p21, 0.5);
-            if (f && bin[e] < SET_BINS - 1) atomicAdd(&bins[bin[e]], f);     // (the last bin holds what the others do not, and is not asked)
+            if (bin[e] < SET_BINS - 1) atomicAdd(&bins[bin[e]], f);          // (the last bin holds what the others do not, and is not asked)
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const uint4 c = *(const uint4 *)&bins[4 * lane];
@@ -283,6 +306,22 @@ struct WaveSet {
         };
         const double units = border * 0x1p21;
         const uint32_t b0 = first(units > 600.0 ? (uint32_t)(units - 600.0) : 0u), b1 = first((uint32_t)fmin(units + 600.0, 4294967295.0));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        uint64_t lanes = 0;
+        uint32_t n = 0;
+        float one = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool in = bin[e] - b0 <= b1 - b0;
+            const uint64_t m = __ballot(in);
+            lanes |= m;
+            n += __popcll(m);
+            one = in ? l[e] : one;
+        }
+        if (n == 1) {
+            hi = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(one), __ffsll((unsigned long long)lanes) - 1));
+            return true;
+        }
         float top = -INFINITY, below = -INFINITY;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -291,7 +330,7 @@ struct WaveSet {
         }
         hi = wave_max(top);
         lo = wave_max(below);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        return false;
     }
 
     // Those whose mass before them in the order is below `border` (> 0), the first always: they end with the score t, of which r of
@@ -299,7 +338,11 @@ struct WaveSet {
     __device__ __forceinline__ void cut_mass(double border, float high, float span, float &t, uint32_t &r, uint32_t &ties, uint32_t *bins) const
     {
         float lo = -INFINITY, hi = high;               // mass above hi below the border, mass above lo not
-        narrow(border, high, span, lo, hi, bins);
+        if (narrow(border, high, span, lo, hi, bins)) {
+            t = hi;
+            r = ties = 1;
+            return;
+        }
         for (;;) {
             const float least = snap_up(lo);
             if (least >= hi) break;
@@ -360,11 +403,14 @@ struct WaveSet {
     __device__ __forceinline__ uint32_t draw(float top, uint32_t top_k, float top_p, float min_p, float u, float reach, uint32_t *bins, double &drawn,
                                              double &total)
     {
-        if (top_k > 0 && count_above(-INFINITY) > top_k) {
-            float t;
-            uint32_t r, ties;
-            cut_count(top_k, t, r, ties);
-            apply(t, r, ties);
+        if (top_k > 0) {
+            drop_weightless();
+            if (count_above(-INFINITY) > top_k) {
+                float t;
+                uint32_t r, ties;
+                cut_count(top_k, t, r, ties);
+                apply(t, r, ties);
+            }
         }
         if (top_p < 1.0f) {
             float t;
@@ -424,7 +470,10 @@ struct RowParams {
     }
     // How far below the maximum the border of a nucleus among V scores lies at most: all scores more than ln(V / (1 - p)) below
     // it (in units of T) together weigh less than 1 - p.
-    __device__ float reach(uint32_t V) const { return (__logf((float)V) - __logf(fmaxf(1.0f - top_p, 0x1p-24f)) + 1.0f) * temperature; }
+    __device__ float reach(uint32_t V) const
+    {
+        return (__builtin_amdgcn_logf((float)V) - __builtin_amdgcn_logf(fmaxf(1.0f - top_p, 0x1p-24f)) + 1.5f) * 0.6932f * temperature;
+    }
 };
 
 // ---------------------------------------------------------------------------------------------- a wave per row
@@ -509,7 +558,7 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
                 set.weigh_all(Weigh(top, p.temperature));
                 double drawn, total;
                 at = set.draw(top, p.top_k, p.top_p, p.min_p, p.u, p.reach(a.V), mine.bins, drawn, total);
-                prob = (float)(drawn / total);
+                prob = (float)(drawn * inverse(total));
             }
         }
         if (lane == 0) {
@@ -847,7 +896,10 @@ struct BlockRow {
             const uint32_t q = lane() * E + e;
             set.l[e] = q < n ? sh.list_l[q] : -INFINITY;
         }
-        if (WEIGH) set.weigh_all(weigh);
+        if (WEIGH) {
+            set.weigh_all(weigh);
+            set.drop_weightless();
+        }
     }
 };
 
@@ -861,7 +913,7 @@ __device__ __attribute__((noinline)) Drawn list_draw(const Row r, const RowParam
     row.load_list(set);
     double drawn, total;
     const uint32_t q = set.draw(row.weigh.top, same(p.top_k), same(p.top_p), same(p.min_p), same(p.u), same(p.reach(row.V - row.first)), Row::shared().bins, drawn, total);
-    return {Row::shared().list_at[q] - row.first, (float)(drawn / total)};
+    return {Row::shared().list_at[q] - row.first, (float)(drawn * inverse(total))};
 }
 
 template <class Row, int E, bool MASS>
@@ -1144,7 +1196,7 @@ __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, ui
             }
         }
         d.at = (uint32_t)__builtin_amdgcn_readlane((int)(j + place), q) - row.first;
-        d.prob = (float)(lane_of(drawn, q) / total);
+        d.prob = (float)(lane_of(drawn, q) * inverse(total));
     });
     return d;
 }
@@ -1159,10 +1211,7 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     const Cut old{same(o.t), same(o.r), same(o.ties), 0};
     top_p = same(top_p);
     const float high = row.weigh.top, per = (float)BINS / same(reach);
-    auto bin = [&](float l) {
-        const float below = high - l;
-        return below > 0.0f ? (uint32_t)fminf(below * per, (float)(BINS - 1)) : 0u;
-    };
+    auto bin = [&](float l) { return (uint32_t)fminf(fmaxf((high - l) * per, 0.0f), (float)(BINS - 1)); };      // (inf - inf: the first)
     for (uint32_t b = threadIdx.x; b < BINS; b += THREADS) sh.mass[b] = 0;
     __syncthreads();
     // the last bin, most of a row's scores, in registers: its additions would queue at one address
@@ -1172,10 +1221,12 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     row.template each<1>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
 #pragma unroll
         for (int e = 0; e < Row::PER; ++e) {
-            const unsigned long long f = l[e] > old.t ? row.fixed(row.weigh(l[e])) : 0;          // (of the scores equal to old.t, r are left: added below)
+            const unsigned long long f = row.fixed(row.weigh(l[e] > old.t ? l[e] : -INFINITY));  // (of the scores equal to old.t, r are left: added below)
             const uint32_t b = bin(l[e]);
-            rest += b == BINS - 1 ? f : 0;
-            if (b < BINS - 1 && f) atomicAdd(&sh.mass[b], f);
+            if (b < BINS - 1)
+                atomicAdd(&sh.mass[b], f);
+            else
+                rest += f;
         }
     });
     if (rest) atomicAdd(&sh.mass[BINS - 1], rest);
