@@ -80,7 +80,9 @@ struct Weigh {
         const double r = inverse((double)temperature), q = 1.4426950408889634 * r;
         scale = fma(fma(-(double)temperature, q, 1.4426950408889634), r, q);
     }
-    __device__ __forceinline__ double operator()(float l) const
+    // FINITE: the maximum is
+    template <bool FINITE = false>
+    __device__ __forceinline__ double of(float l) const
     {
         const double z = fmax(((double)l - (double)top) * scale, -1100.0), n = rint(z), f = z - n;
         double p = 2.5678435993488206e-11;              // ln2^k / k!
@@ -96,10 +98,13 @@ struct Weigh {
         p = horner(p, f, 2.4022650695910071e-01);
         p = horner(p, f, 6.9314718055994531e-01);
         p = fma(p, f, 1.0);
-        const uint64_t w = (uint64_t)__double_as_longlong(ldexp(p, (int)n));
+        p = ldexp(p, (int)n);
+        if (FINITE) return p;
+        const uint64_t w = (uint64_t)__double_as_longlong(p);
         const uint32_t hi = l == top ? 0x3FF00000u : (uint32_t)(w >> 32);      // (the low half is 0 for the maximum either way)
         return __longlong_as_double((long long)((uint64_t)hi << 32 | (uint32_t)w));
     }
+    __device__ __forceinline__ double operator()(float l) const { return of(l); }
 };
 
 // Lanes below move up within the wave by data-parallel primitives: rows of 16 by shifts, then across rows.  Lanes without a
@@ -194,10 +199,11 @@ struct WaveSet {
     float l[E];
     double w[E];
 
+    template <bool FINITE = false>
     __device__ __forceinline__ void weigh_all(const Weigh &weigh)
     {
 #pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = weigh(l[e]);
+        for (int e = 0; e < E; ++e) w[e] = weigh.of<FINITE>(l[e]);
     }
     __device__ __forceinline__ void drop_weightless()
     {
@@ -429,11 +435,30 @@ struct WaveSet {
         const double upto = wave_scan(mine);
         total = last_lane(upto);
         const double target = (double)u * total;
-        // the first lane past the target; should rounding leave the target at the very end, the last lane that holds anything
-        const uint64_t some = __ballot(mine > 0.0), hit = __ballot(mine > 0.0 && upto > target);
-        const int q = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(some);
+        // the first lane past the target, the first of its scores past it
+        const uint64_t past = __ballot(upto > target);
+        uint32_t at = E;
         double run = upto - mine;
-        uint32_t at = 0;
+        drawn = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            run += w[e];
+            const bool here = at == E && run > target;
+            at = here ? e : at;
+            drawn = here ? w[e] : drawn;
+        }
+        int q = past ? __ffsll((unsigned long long)past) - 1 : 0;
+        if (lane_of(drawn, q) > 0.0) {
+            at = (uint32_t)__builtin_amdgcn_readlane((int)at, q);
+            drawn = lane_of(drawn, q);
+            return (uint32_t)q * E + at;
+        }
+        // rounding has left the target at the very end of a lane's scores, or of all: among those that weigh something, the last where
+        // none is past it
+        const uint64_t some = __ballot(mine > 0.0), hit = __ballot(mine > 0.0 && upto > target);
+        q = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(some);
+        run = upto - mine;
+        at = 0;
         bool done = false;
         drawn = 0.0;
 #pragma unroll
@@ -555,7 +580,12 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
                 at = (uint32_t)q * E + (uint32_t)__builtin_amdgcn_readlane((int)e1, q);
                 prob = 1.0f;
             } else {
-                set.weigh_all(Weigh(top, p.temperature));
+                if (top == INFINITY) {                 // the rows' own order, with a finite maximum
+#pragma unroll
+                    for (int e = 0; e < E; ++e) set.l[e] = set.l[e] == top ? 0.0f : -INFINITY;
+                    top = 0.0f;
+                }
+                set.template weigh_all<true>(Weigh(top, p.temperature));
                 double drawn, total;
                 at = set.draw(top, p.top_k, p.top_p, p.min_p, p.u, p.reach(a.V), mine.bins, drawn, total);
                 prob = (float)(drawn * inverse(total));
