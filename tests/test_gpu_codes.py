@@ -778,3 +778,19 @@ def test_sample_cuts_beyond_the_list(ctx, V, dtype):
     for how in (dict(top_k=209), dict(top_k=353), dict(top_k=600), dict(top_k=V - 200), dict(top_k=V - 1), dict(top_k=600, top_p=0.9), dict(top_k=600, top_p=0.999),
                 dict(top_k=900, top_p=0.3), dict(top_k=208, top_p=0.7)):
         check_sample(ctx, rows, u, **how)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("N,V", [(5, 257), (5, 511), (5, 512), (5, 513), (3, 8192), (3, 8193), (3, 32768), (3, 32769), (258, 40000), (3, 65537)])
+def test_sample_where_the_kernels_change(ctx, N, V, dtype):
+    g = gen(V + N)
+    rows = (torch.randn(N, V, generator=g) * 3).to(TYPES[dtype])
+    u = torch.rand(N, generator=g)
+    for how in (dict(), dict(top_k=50, top_p=0.9), dict(top_k=250), dict(top_k=300), dict(top_p=0.8, min_p=0.001)):
+        if N <= 5:
+            check_sample(ctx, rows, u, **how)
+        else:                                                # a few of many rows
+            idx, prob = ctx.sample(rows.cuda(), u.cuda(), **how)
+            some = torch.tensor([0, 100, N - 1])
+            one = ctx.sample(rows[some].cuda(), u[some].cuda(), **how)
+            assert torch.equal(idx[some.cuda()], one[0]) and torch.allclose(prob[some.cuda()], one[1], rtol=2e-7, atol=0)

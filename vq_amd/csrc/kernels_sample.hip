@@ -1298,7 +1298,7 @@ __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
                 // The k-th largest of the lanes' own maxima: at least k scores reach it, and few more do, since the largest
                 // scores rarely share a lane: of scores in no order -n ln(1 - k / n) for n lanes, which is 430 of the 512 the
                 // list holds at these k.
-                if (p.top_k <= (THREADS < 1024 ? 208 : 352)) {
+                if (p.top_k <= (THREADS == 256 ? 208 : THREADS == 512 ? 290 : 352)) {
                     const uint32_t least = max(row.kth_largest(key_of(mine), p.top_k), KEY_LEAST + 1);
                     if (row.collect(value_of(least), INFINITY, [](float) { return true; })) {
                         if (threadIdx.x < 64) d = sh.n <= 256 ? list_draw<Row, 4>(row, p) : list_draw<Row, 8>(row, p);
@@ -1348,9 +1348,16 @@ hipError_t run_block(const SampleArgs &a, hipStream_t s)
 template <class T>
 hipError_t run_sample(const SampleArgs &a, hipStream_t s)
 {
+    // A wave per row, all of it in registers, up to 1024 scores, with room for no more than it takes.  us, f32, top_p 0.9: 65536 x 256
+    // 54 (with room for 1024 160), 32768 x 512 49 (91; by workgroups 314), 32768 x 1000 103 (345)
     if (a.V <= 256) return run_wave<T, 4>(a, s);
+    if (a.V <= 512) return run_wave<T, 8>(a, s);
     if (a.V <= 1024) return run_wave<T, 16>(a, s);
+    // A small workgroup wastes less at its barriers, a large one is done sooner where there are fewer rows than CUs, or long ones.  us at
+    // 256 / 512 / 1024 lanes, top_p 0.9: 8192 x 4096 150 / - / 461; 256 x 16384 32 / 25 / 27, 1024 x 16384 59 / 64 / 100; 256 x 50000
+    // 79 / 58 / 55, 512 x 50000 101 / 87 / 103; bf16 256 x 131072 187 / 118 / 105, 512 x 131072 224 / 225 / 193
     if (a.V <= 8192) return run_block<T, 256>(a, s);
+    if (a.V <= 32768 || (a.V <= 65536 && a.N > 256)) return run_block<T, 512>(a, s);
     return run_block<T, 1024>(a, s);
 }
 
