@@ -781,7 +781,7 @@ def test_sample_cuts_beyond_the_list(ctx, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("N,V", [(5, 257), (5, 511), (5, 512), (5, 513), (3, 8192), (3, 8193), (3, 32768), (3, 32769), (258, 40000), (3, 65537)])
+@pytest.mark.parametrize("N,V", [(5, 65), (5, 128), (5, 129), (5, 257), (5, 511), (5, 512), (5, 513), (3, 8192), (3, 8193), (3, 32768), (3, 32769), (258, 40000), (3, 65537)])
 def test_sample_where_the_kernels_change(ctx, N, V, dtype):
     g = gen(V + N)
     rows = (torch.randn(N, V, generator=g) * 3).to(TYPES[dtype])
@@ -794,3 +794,27 @@ def test_sample_where_the_kernels_change(ctx, N, V, dtype):
             some = torch.tensor([0, 100, N - 1])
             one = ctx.sample(rows[some].cuda(), u[some].cuda(), **how)
             assert torch.equal(idx[some.cuda()], one[0]) and torch.allclose(prob[some.cuda()], one[1], rtol=2e-7, atol=0)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [1, 3, 4, 5, 15, 16, 17, 31, 32, 33, 50, 63, 64])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_sample_short_rows(ctx, V, dtype, pad):
+    """Many short rows in one wave, each with its own parameters, ties, masks, infinities and nothing at all."""
+    g, N = gen(V), 131
+    rows = torch.randn(N, V, generator=g) * 3
+    rows[::4] = torch.randint(-2, 3, (len(rows[::4]), V), generator=g).float()
+    rows[1::5] = torch.where(torch.rand(len(rows[1::5]), V, generator=g) < 0.5, -INF, rows[1::5])
+    rows[2::11], rows[3::13, V // 2], rows[5::17, 0], rows[7::19] = -INF, INF, NAN, torch.finfo(TYPES[dtype]).min
+    rows[8::23] += 1e4
+    rows = rows.to(TYPES[dtype])
+    u = torch.rand(N, generator=g)
+    buf = torch.full((N, V + pad), 7.0, dtype=TYPES[dtype]).cuda()
+    dev = buf[:, :V]
+    dev.copy_(rows.cuda())
+    for how in (dict(), dict(temperature=0.0), dict(top_k=3), dict(top_p=0.6), dict(min_p=0.2), dict(top_k=5, top_p=0.9, min_p=0.05, temperature=0.3), dict(temperature=50.0, top_p=0.99),
+                dict(temperature=1e-3, top_p=0.5), dict(top_p=0.9999999)):
+        check_sample(ctx, rows, u, dev=dev, **how)
+    per = dict(temperature=torch.rand(N, generator=g) * 2 * (torch.rand(N, generator=g) > 0.2), top_k=torch.randint(0, V + 2, (N,), generator=g).int(),
+               top_p=torch.rand(N, generator=g) * 1.2, min_p=torch.rand(N, generator=g) * 0.3)
+    check_sample(ctx, rows, u, dev=dev, **per)

@@ -12,9 +12,16 @@
 // the order (w 2^s rounded, s chosen so that V of them fit 63 bits).  Two correct evaluations still part where u Z or top_p Z1
 // falls within ~1e-11 of a border.
 //
-// Two kernels.  Up to 1024 scores: k_sample_wave, a wave per row, the row in registers, no LDS.  Longer rows:
-// k_sample_block, a workgroup per row, which first cuts the row down to the few hundred scores the filters are decided
-// among and hands those to the same code as a wave's row.
+// Three kernels.  Up to 64 scores: k_sample_quad, four lanes per row.  Up to 1024: k_sample_wave, a wave per row.  Both hold the row in
+// registers and read it once.  Longer rows: k_sample_block, a workgroup per row, which first cuts the row down to the few
+// hundred scores the filters are decided among and hands those to the same code as a wave's row; it reads the row three or
+// four times, all but the first from the caches.
+//
+// What bounds them: the vector units, not memory.  A weight in f64 is 23 instructions and there is no shorter exact way.  400000 x
+// 256 f32 with top_p 0.9: 236 us, 354 vector instructions a row, the units busy all the time (reading the scores once is 103 us
+// at the rate of a large copy).  256 x 131072 bf16 with top_p 0.9: 100 us, of which the weights and their histogram are about
+// 40, the four passes over memory and caches the rest.  1 x 131072 bf16 with top_k 50 and top_p 0.9: 19 us, one workgroup's
+// latency.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -597,6 +604,254 @@ __global__ void __launch_bounds__(WAVE_THREADS) k_sample_wave(const SampleArgs a
         }
         if (!more) return;
         i += waves;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- four lanes per row
+// Short rows: a wave works on 16 of them at once, so that what a row costs beside its weights (sums, extremes, the search for a
+// border) is shared by 16.  What the lanes of a row exchange are permutations within four lanes; rows of a wave part ways in
+// loops and branches, the lanes of one never do.
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+template <int CTRL>
+__device__ __forceinline__ float quad(float v) { return __uint_as_float(quad<CTRL>(__float_as_uint(v))); }
+template <int CTRL>
+__device__ __forceinline__ double quad(double v)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)quad<CTRL>((uint32_t)(b >> 32)) << 32 | quad<CTRL>((uint32_t)b)));
+}
+constexpr int NEIGHBOUR = 0xB1, OPPOSITE = 0x4E, LANE = 0x55;        // the lane beside, the pair beside; k LANE: lane k
+template <class V>
+__device__ __forceinline__ V quad_sum(V v)                           // (the same bits in all four: both sides add the same two)
+{
+    v += quad<NEIGHBOUR>(v);
+    return v + quad<OPPOSITE>(v);
+}
+__device__ __forceinline__ float quad_max(float v)
+{
+    v = fmaxf(v, quad<NEIGHBOUR>(v));
+    return fmaxf(v, quad<OPPOSITE>(v));
+}
+__device__ __forceinline__ float quad_min(float v)
+{
+    v = fminf(v, quad<NEIGHBOUR>(v));
+    return fminf(v, quad<OPPOSITE>(v));
+}
+__device__ __forceinline__ uint32_t quad_min(uint32_t v)
+{
+    v = min(v, quad<NEIGHBOUR>(v));
+    return min(v, quad<OPPOSITE>(v));
+}
+
+// A row of up to 4 E scores, lane i of its four holding E consecutive ones, with WaveSet's conventions.
+template <int E>
+struct QuadSet {
+    float l[E];
+    double w[E];
+
+    __device__ __forceinline__ uint32_t count_above(float x) const
+    {
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) n += l[e] > x;
+        return quad_sum(n);
+    }
+    __device__ __forceinline__ uint32_t count_equal(float x) const
+    {
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) n += l[e] == x;
+        return quad_sum(n);
+    }
+    __device__ __forceinline__ double mass_above(float x) const
+    {
+        double s = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += l[e] > x ? w[e] : 0.0;
+        return quad_sum(s);
+    }
+    __device__ __forceinline__ float snap_down(float x) const
+    {
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, l[e] <= x ? l[e] : -INFINITY);
+        return quad_max(m);
+    }
+    __device__ __forceinline__ float snap_up(float x) const
+    {
+        float m = INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fminf(m, l[e] > x ? l[e] : INFINITY);
+        return quad_min(m);
+    }
+    // Halves the bracket (lo, hi] of scores until hi is the only one in it: below(m) tells that the border lies
+    // at or below m.
+    template <class Below>
+    __device__ __forceinline__ float border(float lo, float hi, Below &&below) const
+    {
+        for (;;) {
+            const float least = snap_up(lo);
+            if (least >= hi) return hi;
+            float m = 0.5f * least + 0.5f * hi;
+            if (!(m >= least && m < hi)) m = least;
+            if (below(m))
+                hi = snap_down(m);
+            else
+                lo = m;
+        }
+    }
+    // Scores behind the r-th of those equal to t go out.
+    __device__ __forceinline__ void apply(float t, uint32_t r, uint32_t ties)
+    {
+        if (r < ties) {
+            uint32_t mine = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) mine += l[e] == t;
+            const uint32_t q = threadIdx.x & 3, n0 = quad<0>(mine), n1 = quad<LANE>(mine), n2 = quad<2 * LANE>(mine);
+            uint32_t before = (q > 0 ? n0 : 0) + (q > 1 ? n1 : 0) + (q > 2 ? n2 : 0);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const bool eq = l[e] == t;
+                if (eq && before >= r) {
+                    l[e] = -INFINITY;
+                    w[e] = 0.0;
+                }
+                before += eq;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool in = l[e] >= t;
+            l[e] = in ? l[e] : -INFINITY;
+            w[e] = in ? w[e] : 0.0;
+        }
+    }
+
+    // The filters, then the draw: its place in the row and its weight in the lane that holds it (true there).
+    __device__ __forceinline__ bool draw(float top, uint32_t top_k, float top_p, float min_p, float u, float reach, uint32_t &place, double &drawn, double &total)
+    {
+        const uint32_t q = threadIdx.x & 3;
+        if (top_k > 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) l[e] = w[e] > 0.0 ? l[e] : -INFINITY;
+            if (count_above(-INFINITY) > top_k) {
+                const float t = border(-INFINITY, top, [&](float m) { return count_above(m) < top_k; });
+                apply(t, top_k - count_above(t), count_equal(t));
+            }
+        }
+        if (top_p < 1.0f) {
+            const double room = (double)top_p * mass_above(-INFINITY);
+            // (what lies further below the maximum cannot hold the border; the second term: rounding of the difference)
+            const float t = border(top - reach - fabsf(top) * 0x1p-22f, top, [&](float m) { return mass_above(m) < room; });
+            const uint32_t ties = count_equal(t);
+            uint32_t r = 1;
+            if (ties > 1) {
+                double wt = 0.0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) wt = l[e] == t ? w[e] : wt;
+                // (lanes without one of them have 0, the others the same weight)
+                wt = fmax(wt, quad<NEIGHBOUR>(wt));
+                wt = fmax(wt, quad<OPPOSITE>(wt));
+                const double left = room - mass_above(t), n = ceil(left / wt);
+                r = n < 1.0 ? 1u : n > (double)ties ? ties : (uint32_t)n;
+                if (r > 1 && (double)(r - 1) * wt >= left) --r;
+                if (r < ties && (double)r * wt < left) ++r;
+            }
+            apply(t, r, ties);
+        }
+        if (min_p > 0.0f) {
+            const double least = (double)fminf(min_p, 1.0f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = w[e] >= least ? w[e] : 0.0;
+        }
+        double mine = w[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) mine += w[e];
+        const double m0 = quad<0>(mine), m1 = quad<LANE>(mine), m2 = quad<2 * LANE>(mine), m3 = quad<3 * LANE>(mine);
+        const double before = (q > 0 ? m0 : 0.0) + (q > 1 ? m1 : 0.0) + (q > 2 ? m2 : 0.0);
+        total = m0 + m1 + m2 + m3;
+        const double target = (double)u * total;
+        // the first lane past the target (u < 1: there is one); should rounding leave the target at the end of its scores, the last of them
+        const uint32_t at = quad_min(mine > 0.0 && before + mine > target ? q : 4u);
+        double run = before;
+        bool done = false;
+        place = 0;
+        drawn = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const double x = w[e];
+            run += x;
+            if (!done && x > 0.0) {
+                place = q * E + e;
+                drawn = x;
+                done = run > target;
+            }
+        }
+        return q == at;
+    }
+};
+
+constexpr int QUAD_THREADS = 256;
+
+// VEC: the rows allow loads of 16 bytes (or of all E where they are fewer)
+template <class T, int E, bool VEC>
+__global__ void __launch_bounds__(QUAD_THREADS) k_sample_quad(const SampleArgs a)
+{
+    constexpr int LOAD = VEC ? (16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E) : 1;
+    const uint32_t q = threadIdx.x & 3, j0 = q * E;
+    for (uint64_t i = (uint64_t)blockIdx.x * (QUAD_THREADS / 4) + (threadIdx.x >> 2); i < a.N; i += (uint64_t)gridDim.x * (QUAD_THREADS / 4)) {
+        const T *row = (const T *)a.S + i * a.ld;
+        QuadSet<E> set;
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < E; c += LOAD) {
+            T raw[LOAD];
+            if (j0 + c + LOAD <= a.V) {
+                const Pack<T, LOAD * (int)sizeof(T)> v = *(const Pack<T, LOAD * (int)sizeof(T)> *)(row + j0 + c);
+#pragma unroll
+                for (int e = 0; e < LOAD; ++e) raw[e] = v.v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < LOAD; ++e) raw[e] = j0 + c + e < a.V ? row[j0 + c + e] : (T)-INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < LOAD; ++e) {
+                set.l[c + e] = fmaxf(widen(raw[e]), -INFINITY);                                              // (NaN: -inf)
+                top = fmaxf(top, set.l[c + e]);
+            }
+        }
+        top = quad_max(top);
+        const RowParams p(a, i);
+        uint32_t at = 0;
+        float prob = 0.0f;
+        bool own = q == 0;
+        if (top > -INFINITY) {
+            if (p.greedy) {
+                at = 4 * E;
+#pragma unroll
+                for (int e = E - 1; e >= 0; --e)
+                    if (set.l[e] == top) at = j0 + e;
+                at = quad_min(at);
+                prob = 1.0f;
+            } else {
+                if (top == INFINITY) {                 // the rows' own order, with a finite maximum
+#pragma unroll
+                    for (int e = 0; e < E; ++e) set.l[e] = set.l[e] == top ? 0.0f : -INFINITY;
+                    top = 0.0f;
+                }
+                const Weigh weigh(top, p.temperature);
+#pragma unroll
+                for (int e = 0; e < E; ++e) set.w[e] = weigh.of<true>(set.l[e]);
+                double drawn, total;
+                own = set.draw(top, p.top_k, p.top_p, p.min_p, p.u, p.reach(a.V), at, drawn, total);
+                prob = (float)(drawn * inverse(total));
+            }
+        }
+        if (own) {
+            a.idx[i] = at;
+            if (a.prob) a.prob[i] = prob;
+        }
     }
 }
 
@@ -1338,6 +1593,18 @@ hipError_t run_wave(const SampleArgs &a, hipStream_t s)
     return hipGetLastError();
 }
 
+template <class T, int E>
+hipError_t run_quad(const SampleArgs &a, hipStream_t s)
+{
+    constexpr int LOAD = 16 / (int)sizeof(T) < E ? 16 / (int)sizeof(T) : E;
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.N + QUAD_THREADS / 4 - 1) / (QUAD_THREADS / 4), 1u << 20);
+    if ((((uint64_t)(uintptr_t)a.S | a.ld * sizeof(T)) & (LOAD * sizeof(T) - 1)) == 0)
+        hipLaunchKernelGGL((k_sample_quad<T, E, true>), dim3(blocks), dim3(QUAD_THREADS), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_sample_quad<T, E, false>), dim3(blocks), dim3(QUAD_THREADS), 0, s, a);
+    return hipGetLastError();
+}
+
 template <class T, int THREADS>
 hipError_t run_block(const SampleArgs &a, hipStream_t s)
 {
@@ -1348,8 +1615,14 @@ hipError_t run_block(const SampleArgs &a, hipStream_t s)
 template <class T>
 hipError_t run_sample(const SampleArgs &a, hipStream_t s)
 {
+    // Four lanes per row up to 64 scores: us for 400000 rows, f32, top_p 0.9 (with a wave per row): 10 scores 28 (216), 32 48
+    // (230), 64 94 (237); with parameters per row 64 130 (387)
+    if (a.V <= 16) return run_quad<T, 4>(a, s);
+    if (a.V <= 32) return run_quad<T, 8>(a, s);
+    if (a.V <= 64) return run_quad<T, 16>(a, s);
     // A wave per row, all of it in registers, up to 1024 scores, with room for no more than it takes.  us, f32, top_p 0.9: 65536 x 256
-    // 54 (with room for 1024 160), 32768 x 512 49 (91; by workgroups 314), 32768 x 1000 103 (345)
+    // 54 (with room for 1024 160), 400000 x 100 187 (with room for 256 247), 32768 x 512 49 (91; by workgroups 314), 32768 x 1000 103 (345)
+    if (a.V <= 128) return run_wave<T, 2>(a, s);
     if (a.V <= 256) return run_wave<T, 4>(a, s);
     if (a.V <= 512) return run_wave<T, 8>(a, s);
     if (a.V <= 1024) return run_wave<T, 16>(a, s);
