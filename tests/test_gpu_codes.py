@@ -2,7 +2,7 @@
 vqhip_lookup_gradient_device against their definitions in 64 bits (tests/codes_reference.py).
 
 Tolerances, derived before the first run (a rounding to f32 is off by at most 2^-24, to bf16 by 2^-8 ... relative):
-  scores    (up to 32 values; longer rows have a bound of their own below) every difference x - w rounds once (2^-24), its square and the running sum add a rounding per value: at most
+  scores    (up to 16 values, or few prototypes; longer rows have a bound of their own below) every difference x - w rounds once (2^-24), its square and the running sum add a rounding per value: at most
             (D + 3) 2^-24 of the sum (all terms have one sign)
   sample    idx equal; prob one rounding of an f64 value: 2^-24, and 1e-9 for the f64 sums
   lookup    f32 product rounded once, then once to the type: 2^-24 (f32) or 2^-24 + eps/2
@@ -40,7 +40,8 @@ def wide(t):
 
 
 # ---------------------------------------------------------------------------------------------- scores
-@pytest.mark.parametrize("N,D,K", [(150, 4, 3), (1, 1, 1), (7, 5, 2), (130, 16, 129), (257, 17, 300), (1000, 2, 1), (2, 32, 513)])
+@pytest.mark.parametrize("N,D,K", [(150, 4, 3), (1, 1, 1), (7, 5, 2), (130, 16, 129), (257, 15, 300), (1000, 2, 1), (2, 16, 513), (300, 32, 11), (257, 17, 15), (600, 4, 32), (513, 3, 31),
+                                   (515, 16, 32), (520, 7, 17), (1030, 9, 64), (259, 16, 40), (300, 5, 192)])
 def test_scores(ctx, N, D, K):
     g = gen(N + D)
     W = torch.rand(K, D, generator=g) * 2 - 1
@@ -521,10 +522,10 @@ def test_c_refusals(ctx):
 
 
 # ---------------------------------------------------------------------------------------------- scores on the matrix cores
-@pytest.mark.parametrize("N,D,K", [(1, 33, 1), (64, 128, 256), (33, 784, 100), (129, 255, 127), (2, 1000, 513), (130, 64, 129), (65, 100, 70), (300, 128, 256), (20, 785, 33), (4100, 40, 2100), (2048, 36, 4096)])
+@pytest.mark.parametrize("N,D,K", [(257, 17, 300), (2, 32, 513), (129, 32, 16), (70, 17, 64), (1, 33, 1), (64, 128, 256), (33, 784, 100), (129, 255, 127), (2, 1000, 513), (130, 64, 129), (65, 100, 70), (300, 128, 256), (20, 785, 33), (4100, 40, 2100), (2048, 36, 4096)])
 @pytest.mark.parametrize("offset", [0.0, 100.0])
 def test_scores_in_the_expanded_form(ctx, N, D, K, offset):
-    """Rows of more than 32 values: distances not below 1/16 of B = |x - c|^2 + |w - c|^2 come from B - 2 (x - c).(w - c).  Its
+    """Rows of more than 16 values (but for a few prototypes): distances not below 1/16 of B = |x - c|^2 + |w - c|^2 come from B - 2 (x - c).(w - c).  Its
     roundings, with e = 2^-24: each centred value 1 e of itself, which moves the distance by at most 2 sqrt(dist) e (|x - c| + |w - c|)
     <= 4 e B; each norm a sum of D squares, D e of itself, together D e B; the product a chain of D terms whose absolute
     values sum to at most B / 2, doubled D e B; the two last additions 2 e B.  (2 D + 6) e B <= 16 (2 D + 6) e dist;

@@ -19,8 +19,7 @@ namespace vq {
 
 namespace {
 
-constexpr int SC_THREADS = 256, SC_M = 128, SC_N = 128, SC_K = 16;
-constexpr int SC_LD = SC_M + 4;       // a row of the tile per reduction value, moved 4 banks on from the one before
+constexpr int SC_THREADS = 256, SC_K = 16;
 
 struct ScoreArgs {
     const float *X, *W, *C;           // C: the mean prototype, D values
@@ -48,42 +47,51 @@ __device__ __forceinline__ float4 load4(const float *base, uint64_t row, bool on
     return v;
 }
 
+// TX lanes side by side, 8 prototypes each: 128, 64 or 32 prototypes a tile, 8 samples each of the 256 / TX lanes above another.
+template <int TX>
 __global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs a)
 {
-    __shared__ __attribute__((aligned(16))) float lx[2][SC_K][SC_LD], lw[2][SC_K][SC_LD];
+    constexpr int SC_M = SC_THREADS / TX * 8, SC_N = TX * 8, XPARTS = SC_M / 64, WPARTS = (SC_N + 63) / 64;
+    // (a row of the tile per reduction value, moved 4 banks on from the one before)
+    __shared__ __attribute__((aligned(16))) float lx[2][SC_K][SC_M + 4], lw[2][SC_K][SC_N + 4];
     const uint64_t tile = blockIdx.x;
     const uint64_t row0 = tile / a.colTiles * SC_M;
     const uint32_t col0 = (uint32_t)(tile % a.colTiles) * SC_N;
     const int t = threadIdx.x;
-    // staging: lane t moves values 4 (t & 3) .. + 3 of rows (t >> 2) and (t >> 2) + 64, of both operands
+    // staging: lane t moves values 4 (t & 3) .. + 3 of rows (t >> 2), (t >> 2) + 64, ... of both operands
     const int sr = t >> 2, sd = (t & 3) * 4;
-    const int ty = t >> 4, tx = t & 15;
+    const int ty = t / TX, tx = t % TX;
     float acc[8][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
 
-    float4 px[2], pw[2];
+    float4 px[XPARTS], pw[WPARTS];
     auto fetch = [&](uint32_t d) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < XPARTS; ++h) {
             const uint64_t r = row0 + sr + 64 * h;
-            const uint32_t c = col0 + sr + 64 * h;
             px[h] = load4(a.X, r, r < a.N, a.D, d + sd, a.vecX);
+        }
+#pragma unroll
+        for (int h = 0; h < WPARTS; ++h) {
+            const uint32_t c = col0 + sr + 64 * h;
             pw[h] = load4(a.W, c, c < a.K, a.D, d + sd, a.vecW);
         }
     };
+    auto put = [&](float *to, int ld, const float4 &v) {
+        to[0] = v.x;
+        to[ld] = v.y;
+        to[2 * ld] = v.z;
+        to[3 * ld] = v.w;
+    };
     auto stage = [&](int b) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float fx[4] = {px[h].x, px[h].y, px[h].z, px[h].w}, fw[4] = {pw[h].x, pw[h].y, pw[h].z, pw[h].w};
+        for (int h = 0; h < XPARTS; ++h) put(&lx[b][sd][sr + 64 * h], SC_M + 4, px[h]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                lx[b][sd + e][sr + 64 * h] = fx[e];
-                lw[b][sd + e][sr + 64 * h] = fw[e];
-            }
-        }
+        for (int h = 0; h < WPARTS; ++h)
+            if (SC_N >= 64 || sr < SC_N) put(&lw[b][sd][sr + 64 * h], SC_N + 4, pw[h]);
     };
     fetch(0);
     stage(0);
@@ -92,13 +100,14 @@ __global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs
     for (uint32_t d = 0; d < a.D; d += SC_K, b ^= 1) {
         const bool more = d + SC_K < a.D;
         if (more) fetch(d + SC_K);
+        const int values = min(SC_K, (int)(a.D - d + 3) & ~3);
 #pragma unroll 4
-        for (int k = 0; k < SC_K; ++k) {
+        for (int k = 0; k < values; ++k) {
             float x[8], w[8];
             *(float4 *)&x[0] = *(const float4 *)&lx[b][k][ty * 4];
-            *(float4 *)&x[4] = *(const float4 *)&lx[b][k][64 + ty * 4];
+            *(float4 *)&x[4] = *(const float4 *)&lx[b][k][SC_M / 2 + ty * 4];
             *(float4 *)&w[0] = *(const float4 *)&lw[b][k][tx * 4];
-            *(float4 *)&w[4] = *(const float4 *)&lw[b][k][64 + tx * 4];
+            *(float4 *)&w[4] = *(const float4 *)&lw[b][k][SC_N / 2 + tx * 4];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -112,11 +121,11 @@ __global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint64_t r = row0 + (i >> 2) * 64 + ty * 4 + (i & 3);
+        const uint64_t r = row0 + (i >> 2) * (SC_M / 2) + ty * 4 + (i & 3);
         if (r >= a.N) continue;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const uint32_t c = col0 + g * 64 + tx * 4;
+            const uint32_t c = col0 + g * (SC_N / 2) + tx * 4;
             float *out = a.S + r * a.ld + c;
             if (a.vecS && c + 4 <= a.K) {
                 *(float4 *)out = make_float4(-acc[i][g * 4], -acc[i][g * 4 + 1], -acc[i][g * 4 + 2], -acc[i][g * 4 + 3]);
@@ -129,8 +138,72 @@ __global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs
     }
 }
 
+// ---------------------------------------------------------------------------------------------- few prototypes
+// A lane per sample, its values in registers; the prototypes' values are the same for all lanes and come through the scalar
+// cache, so that nothing is staged and nobody waits at a barrier.  Tiles of 128 prototypes would be mostly empty here.
+template <int DP>
+__global__ void __launch_bounds__(SC_THREADS) k_scores_few(const ScoreArgs a)
+{
+    using Uniform = const __attribute__((address_space(4))) float;
+    const uint64_t r = (uint64_t)blockIdx.x * SC_THREADS + threadIdx.x;
+    if (r >= a.N) return;
+    const float *row = a.X + r * a.D;
+    float x[DP];
+#pragma unroll
+    for (int d = 0; d < DP; d += 4) {
+        if (a.vecX && (uint32_t)d + 4 <= a.D) {
+            const float4 v = *(const float4 *)(row + d);
+            x[d] = v.x;
+            x[d + 1] = v.y;
+            x[d + 2] = v.z;
+            x[d + 3] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[d + e] = (uint32_t)(d + e) < a.D ? row[d + e] : 0.0f;
+        }
+    }
+    float *out = a.S + r * a.ld;
+    for (uint32_t j = 0; j < a.K; j += 4) {
+        // (behind the last prototype: that one again, not stored)
+        Uniform *w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = (Uniform *)a.W + (size_t)min(j + q, a.K - 1) * a.D;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int d = 0; d < DP; d += 4) {
+            if ((uint32_t)d >= a.D) break;
+            if ((uint32_t)d + 4 <= a.D) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float f = x[d + e] - w[q][d + e];
+                        s[q] = fmaf(f, f, s[q]);
+                    }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if ((uint32_t)(d + e) < a.D)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float f = x[d + e] - w[q][d + e];
+                            s[q] = fmaf(f, f, s[q]);
+                        }
+            }
+        }
+        if (a.vecS && j + 4 <= a.K) {
+            *(float4 *)(out + j) = make_float4(-s[0], -s[1], -s[2], -s[3]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (j + q < a.K) out[j + q] = -s[q];
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- matrix cores
-constexpr uint32_t DIRECT_D = 32;     // rows up to this length: k_scores_direct
+constexpr uint32_t FEW_D = 32, FEW_K = 32;      // k_scores_few
+constexpr uint32_t DIRECT_D = 16;     // rows up to this length: k_scores_direct
 // Of |x - c|^2 + |w - c|^2; distances below it are measured directly.  The products' error is a few 2^-24 of the norms, so at 1/16
 // a distance is within a few 1e-6 of itself (the bar of this library is 1e-5); at 1/8 the samples of a codebook would take
 // their own prototype's way through the direct form too, 45 us more on 500k x 128 against 256.
@@ -444,6 +517,25 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
     }
 }
 
+template <int TX>
+hipError_t run_direct(ScoreArgs a, hipStream_t s)
+{
+    constexpr uint32_t TM = SC_THREADS / TX * 8, TN = TX * 8;
+    a.colTiles = (a.K + TN - 1) / TN;
+    const uint64_t N = a.N, most = std::max<uint64_t>(1, (1u << 30) / a.colTiles) * TM;          // a grid holds fewer than 2^31 workgroups
+    const float *X = a.X;
+    float *S = a.S;
+    for (uint64_t off = 0; off < N; off += most) {
+        a.X = X + off * a.D;
+        a.S = S + off * a.ld;
+        a.N = std::min(N - off, most);
+        hipLaunchKernelGGL(k_scores_direct<TX>, dim3((uint32_t)((a.N + TM - 1) / TM * a.colTiles)), dim3(SC_THREADS), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 template <int RW, int CW, int WR, int WC, int PER_SIMD, bool VEC>
 hipError_t run_mfma_as(ScoreArgs a, hipStream_t s)
 {
@@ -473,9 +565,11 @@ hipError_t run_mfma(const ScoreArgs &a, hipStream_t s)
 
 }  // namespace
 
+static bool is_few(uint32_t K, uint32_t D) { return K <= FEW_K && D <= FEW_D && K * K * D <= 4096; }
+
 size_t scores_image_bytes(uint32_t K, uint32_t D)
 {
-    if (D <= DIRECT_D) return 0;
+    if (D <= DIRECT_D || is_few(K, D)) return 0;
     const size_t blocks = image_blocks(K), steps = (D + MF_K - 1) / MF_K;
     return steps * blocks * IMG_BLOCK * 4 + blocks * 64 * 4;
 }
@@ -493,7 +587,7 @@ hipError_t launch_scores_image(const float *dW, const float *dC, uint32_t K, uin
 hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const float *dC, const void *dImg, uint32_t K, float *dS, uint64_t ld,
                          hipStream_t s)
 {
-    ScoreArgs a{dX, dW, dC, dS, N, ld, K, D, nullptr, nullptr, image_blocks(K), (K + SC_N - 1) / SC_N, 0, 0, 0, 0};
+    ScoreArgs a{dX, dW, dC, dS, N, ld, K, D, nullptr, nullptr, image_blocks(K), 0, 0, 0, 0, 0};
     a.img = (const uint32_t *)dImg;
     a.norms = (const float *)(a.img + (size_t)((D + MF_K - 1) / MF_K) * a.blocks * IMG_BLOCK);
     const bool rows = D % 4 == 0;
@@ -501,27 +595,39 @@ hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *d
     a.vecW = rows && ((uintptr_t)dW & 15) == 0;
     a.vecC = rows && ((uintptr_t)dC & 15) == 0;
     a.vecS = ld % 4 == 0 && ((uintptr_t)dS & 15) == 0;
+    if (is_few(K, D)) {
+        const uint64_t most = (1ull << 30) * SC_THREADS;
+        for (uint64_t off = 0; off < N; off += most) {
+            a.X = dX + off * D;
+            a.S = dS + off * ld;
+            a.N = std::min(N - off, most);
+            const dim3 blocks((uint32_t)((a.N + SC_THREADS - 1) / SC_THREADS));
+            if (D <= 4)
+                hipLaunchKernelGGL(k_scores_few<4>, blocks, dim3(SC_THREADS), 0, s, a);
+            else if (D <= 16)
+                hipLaunchKernelGGL(k_scores_few<16>, blocks, dim3(SC_THREADS), 0, s, a);
+            else
+                hipLaunchKernelGGL(k_scores_few<32>, blocks, dim3(SC_THREADS), 0, s, a);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    }
     if (D > DIRECT_D) {
         // Larger tiles read both operands less often, smaller ones leave fewer of the 512 places (two workgroups a CU) empty in the last
         // round.  us, 128 x 256 / 128 x 128 / 64 x 64 tiles: 500k x 128 against 256 (3907 wide tiles) 270 / 295 / 399, 20011 x 784
         // against 1000 (628) 209 / 203 / 278
-        const uint64_t rows = (N + 127) / 128;
-        if (rows * ((K + 255) / 256) >= 2048) return run_mfma<2, 4, 2, 2, 2>(a, s);
-        if (rows * ((K + 127) / 128) >= 512) return run_mfma<2, 2, 2, 2, 2>(a, s);
+        // Where prototypes would leave a large part of a wide tile empty, a narrower one is taken: what a tile of each kind costs per
+        // column is 1 / 1.1 / 1.5.
+        const uint64_t rows = (N + 127) / 128, c256 = (K + 255) / 256, c128 = (K + 127) / 128, c64 = (K + 63) / 64;
+        const uint64_t wide = c256 * 40, middle = c128 * 22, slim = c64 * 15;
+        if (rows * c256 >= 2048 && wide <= middle && wide <= slim) return run_mfma<2, 4, 2, 2, 2>(a, s);
+        if (rows * c128 >= 512 && middle <= slim) return run_mfma<2, 2, 2, 2, 2>(a, s);
         return run_mfma<1, 1, 2, 2, 4>(a, s);
     }
-    // one grid holds fewer than 2^31 workgroups
-    const uint64_t most = ((1ull << 30) / a.colTiles) * SC_M;
-    for (uint64_t off = 0; off < N; off += most) {
-        a.X = dX + off * D;
-        a.S = dS + off * ld;
-        a.N = std::min(N - off, most);
-        const uint64_t blocks = (a.N + SC_M - 1) / SC_M * a.colTiles;
-        hipLaunchKernelGGL(k_scores_direct, dim3((uint32_t)blocks), dim3(SC_THREADS), 0, s, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    // (the narrowest tile that pads the prototypes least)
+    if (K <= 32) return run_direct<4>(a, s);
+    return (K + 63) / 64 % 2 ? run_direct<8>(a, s) : run_direct<16>(a, s);
 }
 
 }  // namespace vq
