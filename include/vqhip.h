@@ -262,7 +262,7 @@ int vqhip_assign_matched_f64(vqhip_ctx *ctx, const double *X, const uint32_t *y,
  * reference beyond reading `prototypes[idx]` (src/glvq/glvq.rs:231).  All calls take device memory and enqueue on `stream`
  * without host synchronisation; none allocates or keeps anything between calls, so they may be captured into a HIP graph, and
  * calls that overlap are independent as long as their outputs and workspaces are.  The one exception: with prototypes of more
- * than 32 values the first vqhip_scores_device or vqhip_assign_sampled_device call after vqhip_set_prototypes lays them out for
+ * than 16 values the first vqhip_scores_device or vqhip_assign_sampled_device call after vqhip_set_prototypes lays them out for
  * the matrix cores (6 bytes per value) and waits for that; under capture that first call is VQHIP_ERR_STATE.  A captured call
  * reads the model where it lay: no vqhip_set_* between capture and replay.  Rows of a matrix lie `ld` elements
  * apart (ld >= its width); what lies between them is neither read nor written.  Outputs must not overlap inputs.  The device
@@ -272,7 +272,7 @@ typedef enum { VQHIP_F32 = 0, VQHIP_BF16 = 1, VQHIP_F16 = 2 } vqhip_dtype;
 /* Scores of N samples against the context's prototypes: S[i][j] = - sum_d (x[i][d] - w[j][d])^2 (src/helpers.rs:18-20
  * without the root), N x K, rows lds apart.  Euclidean models only (VQHIP_ERR_UNSUPPORTED with an Omega).  A softmax of
  * S / T is the distribution over codes that vqhip_assign_sampled_device draws from.  f32, in the direct form or, for rows of
- * more than 32 values, on the matrix cores as |x - c|^2 + |w - c|^2 - 2 (x - c).(w - c) with c the mean prototype; distances
+ * more than 16 values, on the matrix cores as |x - c|^2 + |w - c|^2 - 2 (x - c).(w - c) with c the mean prototype; distances
  * small beside those norms are measured in the direct form there too, so a sample equal to a prototype scores 0 exactly. */
 int vqhip_scores_device(vqhip_ctx *ctx, const float *dX, uint64_t N, float *dS, uint64_t lds, void *stream);
 

@@ -76,7 +76,7 @@ struct vqhip_ctx {
     std::vector<uint32_t> hcls;
 
     float *dW = nullptr;       // K x D, and one row more: their mean
-    void *dScoreImg = nullptr; // the prototypes laid out for vqhip_scores_device (rows above 32 values), made by its first call
+    void *dScoreImg = nullptr; // the prototypes laid out for vqhip_scores_device (rows above 16 values), made by its first call
     double *dW64 = nullptr;    // K x D in the reference's own number type (f64 entry points only)
     uint32_t *dcls = nullptr;  // K
     float *dOm = nullptr;      // M x D  or  K x M x D

@@ -1,10 +1,11 @@
 // Scores of a batch (vqhip_scores_device in include/vqhip.h): S[i][j] = - sum_d (x[i][d] - w[j][d])^2, N x K in f32: the
 // squared distances of euclidean_distance (src/helpers.rs:18-20) without the root.
 //
-// Two kernels.  Rows of up to DIRECT_D values: k_scores_direct, the formula as it stands on the vector units, a 128 x 128 tile a
-// workgroup, 8 x 8 a lane, so that 16 values read from LDS feed 128 vector instructions.  Longer rows: k_scores_mfma, where the
-// two vector instructions per (sample, prototype, value) of the direct form would bound it, the products run on the bf16
-// matrix cores, six of exact three-piece splits (bf16x6, mfma_device.h), in the expanded form
+// Three kernels.  Few prototypes: k_scores_few, a lane per sample.  Rows of up to DIRECT_D values: k_scores_direct, a tile a
+// workgroup, 8 x 8 scores a lane, so that 16 values read from LDS feed 128 vector instructions.  Both are the formula as it stands
+// on the vector units.  Longer rows: k_scores_mfma, where the two vector instructions per (sample, prototype, value) of the
+// direct form would bound it, the products run on the bf16 matrix cores, six of exact three-piece splits (bf16x6,
+// mfma_device.h), in the expanded form
 //     |x - w|^2 = |x - c|^2 + |w - c|^2 - 2 (x - c).(w - c)
 // with c the mean prototype, so that an offset all values share (pixels) does not cost digits.  Its rounding errors are those
 // of the two norms, so the pairs whose distance is small beside them (below CLOSE of their sum: a sample and the few
@@ -202,8 +203,15 @@ __global__ void __launch_bounds__(SC_THREADS) k_scores_few(const ScoreArgs a)
 }
 
 // ---------------------------------------------------------------------------------------------- matrix cores
+// Which kernel.  us for 500000 samples (a lane per sample / direct tiles of 32, 64 or 128 prototypes / matrix cores):
+//     16 values: 3 prototypes 7.4 / 53 / 25, 16 prototypes 23 / 25 / 27, 32 prototypes 51 / 27 / 28, 64 prototypes 115 / 35 / 28,
+//                256 prototypes 438 / 137 / 116
+//      8 values: 16 prototypes 17 / 21 / 27, 64 prototypes 126 / 30 / 28, 256 prototypes 363 / 95 / 116
+//     32 values: 16 prototypes 35 / 96 / 31, 256 prototypes 524 / 203 / 133
+// The lanes of k_scores_few store K apart, which is what it costs: K^2 D up to 4096.  The direct form is kept to 16 values although
+// the matrix cores are as fast from 9 on: it has the smaller error.
 constexpr uint32_t FEW_D = 32, FEW_K = 32;      // k_scores_few
-constexpr uint32_t DIRECT_D = 16;     // rows up to this length: k_scores_direct
+constexpr uint32_t DIRECT_D = 16;               // k_scores_direct
 // Of |x - c|^2 + |w - c|^2; distances below it are measured directly.  The products' error is a few 2^-24 of the norms, so at 1/16
 // a distance is within a few 1e-6 of itself (the bar of this library is 1e-5); at 1/8 the samples of a codebook would take
 // their own prototype's way through the direct form too, 45 us more on 500k x 128 against 256.
@@ -563,9 +571,9 @@ hipError_t run_mfma(const ScoreArgs &a, hipStream_t s)
     return a.vecX && a.vecC ? run_mfma_as<RW, CW, WR, WC, PER_SIMD, true>(a, s) : run_mfma_as<RW, CW, WR, WC, PER_SIMD, false>(a, s);
 }
 
-}  // namespace
+bool is_few(uint32_t K, uint32_t D) { return K <= FEW_K && D <= FEW_D && K * K * D <= 4096; }
 
-static bool is_few(uint32_t K, uint32_t D) { return K <= FEW_K && D <= FEW_D && K * K * D <= 4096; }
+}  // namespace
 
 size_t scores_image_bytes(uint32_t K, uint32_t D)
 {
