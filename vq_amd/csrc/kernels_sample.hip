@@ -261,37 +261,11 @@ struct WaveSet {
         return wave_min(m);
     }
 
-    // The first k in the order end with the score t, of which r of `ties` are among them; more than k scores are in.
-    __device__ void cut_count(uint32_t k, float &t, uint32_t &r, uint32_t &ties) const
-    {
-        // fewer than k above hi, k or more above lo; hi is one of the scores.  Every step takes at least one value out of the bracket
-        // and, where scores are spread evenly, half of them.
-        float lo = -INFINITY, hi = snap_down(INFINITY);
-        for (;;) {
-            const float least = snap_up(lo);
-            if (least >= hi) break;
-            float m = 0.5f * least + 0.5f * hi;
-            if (!(m >= least && m < hi)) m = least;
-            const uint32_t n = count_above(m);
-            if (n == k) {
-                t = snap_up(m);
-                r = ties = count_equal(t);
-                return;
-            }
-            if (n < k)
-                hi = snap_down(m);
-            else
-                lo = m;
-        }
-        t = hi;
-        ties = count_equal(t);
-        r = k - count_above(t);
-    }
-
-    // A bracket for cut_mass by a histogram over even steps of the score, `span` of it in all, from the maximum `high` down.  Its
+    // A bracket for cut_mass (by MASS) or cut_count by a histogram over even steps of the score, `span` of it in all, from the maximum `high` down.  Its
     // masses are integers, w 2^21 rounded, which at most 1024 of them put at most 512 off: with 600 to spare on either side
-    // the border lies in the bins found, whatever their order of addition.  True if they hold one score alone, the last one
+    // the border lies in the bins found, whatever their order of addition; counts are exact.  True if they hold one score alone, the last one
     // kept: hi.
+    template <bool MASS>
     __device__ __forceinline__ bool narrow(double border, float high, float span, float &lo, float &hi, uint32_t *bins) const
     {
         static_assert(E <= 16, "at most 1024 scores");
@@ -304,7 +278,7 @@ struct WaveSet {
         for (int e = 0; e < E; ++e) {
             // (a maximum or a step beyond all bounds: inf - inf and 0 * inf go to the first bin)
             bin[e] = (uint32_t)fminf(fmaxf((high - l[e]) * per, 0.0f), (float)(SET_BINS - 1));
-            const uint32_t f = (uint32_t)fma(w[e], 0x1p21, 0.5);
+            const uint32_t f = MASS ? (uint32_t)fma(w[e], 0x1p21, 0.5) : l[e] > -INFINITY ? 1u : 0u;
             if (bin[e] < SET_BINS - 1) atomicAdd(&bins[bin[e]], f);          // (the last bin holds what the others do not, and is not asked)
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -317,8 +291,14 @@ struct WaveSet {
             const uint32_t in = (base + p0 < x) + (base + p1 < x) + (base + p2 < x);
             return 4 * q + (uint32_t)__builtin_amdgcn_readlane((int)in, q);
         };
-        const double units = border * 0x1p21;
-        const uint32_t b0 = first(units > 600.0 ? (uint32_t)(units - 600.0) : 0u), b1 = first((uint32_t)fmin(units + 600.0, 4294967295.0));
+        uint32_t b0, b1;
+        if (MASS) {
+            const double units = border * 0x1p21;
+            b0 = first(units > 600.0 ? (uint32_t)(units - 600.0) : 0u);
+            b1 = first((uint32_t)fmin(units + 600.0, 4294967295.0));
+        } else {
+            b0 = b1 = first((uint32_t)border);
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         uint64_t lanes = 0;
         uint32_t n = 0;
@@ -346,12 +326,45 @@ struct WaveSet {
         return false;
     }
 
+    // The first k in the order end with the score t, of which r of `ties` are among them; more than k scores are in.
+    __device__ void cut_count(uint32_t k, float &t, uint32_t &r, uint32_t &ties, uint32_t *bins) const
+    {
+        // fewer than k above hi, k or more above lo; hi is one of the scores.  Every step takes at least one value out of the bracket
+        // and, where scores are spread evenly, half of them.
+        float lo, hi;
+        const float high = snap_down(INFINITY);
+        if (narrow<false>((double)k, high, high - snap_up(-INFINITY), lo, hi, bins)) {
+            t = hi;
+            r = ties = 1;
+            return;
+        }
+        for (;;) {
+            const float least = snap_up(lo);
+            if (least >= hi) break;
+            float m = 0.5f * least + 0.5f * hi;
+            if (!(m >= least && m < hi)) m = least;
+            const uint32_t n = count_above(m);
+            if (n == k) {
+                t = snap_up(m);
+                r = ties = count_equal(t);
+                return;
+            }
+            if (n < k)
+                hi = snap_down(m);
+            else
+                lo = m;
+        }
+        t = hi;
+        ties = count_equal(t);
+        r = k - count_above(t);
+    }
+
     // Those whose mass before them in the order is below `border` (> 0), the first always: they end with the score t, of which r of
     // `ties` are among them.  high: the largest score that is in.
     __device__ __forceinline__ void cut_mass(double border, float high, float span, float &t, uint32_t &r, uint32_t &ties, uint32_t *bins) const
     {
         float lo = -INFINITY, hi = high;               // mass above hi below the border, mass above lo not
-        if (narrow(border, high, span, lo, hi, bins)) {
+        if (narrow<true>(border, high, span, lo, hi, bins)) {
             t = hi;
             r = ties = 1;
             return;
@@ -421,7 +434,7 @@ struct WaveSet {
             if (count_above(-INFINITY) > top_k) {
                 float t;
                 uint32_t r, ties;
-                cut_count(top_k, t, r, ties);
+                cut_count(top_k, t, r, ties, bins);
                 apply(t, r, ties);
             }
         }
@@ -1212,7 +1225,7 @@ __device__ __attribute__((noinline)) Cut list_cut(const Row r, double border)
         const float high = set.snap_down(INFINITY), low = set.snap_up(-INFINITY);
         set.cut_mass(same(border), high, high > low ? high - low : 1.0f, c.t, c.r, c.ties, Row::shared().bins);
     } else {
-        set.cut_count((uint32_t)same(border), c.t, c.r, c.ties);
+        set.cut_count((uint32_t)same(border), c.t, c.r, c.ties, Row::shared().bins);
     }
     c.last = EVERY;
     if (c.r < c.ties) {                                // (all of the row's scores equal to t are in the list)
