@@ -816,12 +816,15 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
     const bool one = N > 0 && N <= SINGLE_ROWS && (uint64_t)K * D * bo <= SINGLE_BYTES && N * D * bi <= (uint64_t)a.slabs * parts * (128u << 10);
     const uint32_t *single = one ? didx : nullptr;
     // Rows no index names are cleared beside the sort, whose few workgroups leave the memory idle, where clearing takes longer
-    // than telling the rows apart beforehand (two small launches; 16384 rows of 4096 over 65536: 334 us without, 286 with).
+    // than telling the rows apart beforehand (two small launches; 16384 rows of 4096 over 65536: 334 us without, 270 with).
     const bool early = N > 0 && !accumulate && (uint64_t)K * D * bo > SINGLE_BYTES;
     SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), nullptr, (uint32_t)N, K, p.tiles, 0, p.bits, {}};
     ZeroArgs zero{(char *)dT, ldt * bo, (uint64_t)D * bo, (uint32_t)wo, 0, 0};
-    while (((uint64_t)wo << zero.log2g) < zero.bytes && zero.log2g < 6) ++zero.log2g;
-    zero.blocks = early ? std::min<uint32_t>((K + 15) / 16, 4096) : 0;
+    while (((uint64_t)wo << zero.log2g) < zero.bytes && zero.log2g < 8) ++zero.log2g;
+    // A row to a workgroup where rows are 2 KiB or more, and the next one from another: 1000 rows of 512 over 131072 54 us, by 4096
+    // workgroups 65; short rows by 4096: 5000 of 64 over 1000000 68 us, by 65536 133.
+    const uint64_t shares = zero.bytes >= 2048 ? std::min<uint64_t>((((uint64_t)K << zero.log2g) + 255) / 256, 65536) : std::min<uint64_t>((K + 15) / 16, 4096);
+    zero.blocks = early ? (uint32_t)shares : 0;
     const uint32_t few = std::min<uint32_t>((K + 255) / 256, 4096);
     a.cleared = early ? 1 : 0;
     if (one) {
