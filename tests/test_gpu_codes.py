@@ -819,3 +819,63 @@ def test_sample_short_rows(ctx, V, dtype, pad):
     per = dict(temperature=torch.rand(N, generator=g) * 2 * (torch.rand(N, generator=g) > 0.2), top_k=torch.randint(0, V + 2, (N,), generator=g).int(),
                top_p=torch.rand(N, generator=g) * 1.2, min_p=torch.rand(N, generator=g) * 0.3)
     check_sample(ctx, rows, u, dev=dev, **per)
+
+
+def test_every_kernel_in_graphs(ctx):
+    """Each size class in two captured graphs, replayed in turn with eager work between and inputs that change in place."""
+    g = gen(46)
+    rows = [torch.randn(9, V, generator=g).cuda() * 3 for V in (10, 30, 64, 100, 200, 400, 1000, 3000, 20000, 70000)]
+    u = torch.rand(9, generator=g).cuda()
+    X = [torch.randn(N, 16, generator=g).cuda() for N in (5, 300)]
+    grads = [(torch.randn(N, D, generator=g).cuda(), torch.randint(-1, K, (N,), generator=g).int().cuda(), K) for N, K, D in
+             ((50, 40, 6), (6000, 40, 6), (9000, 3000, 4), (700, 20000, 512), (9000, 20000, 512), (6000, 20000, 512))]
+    models = [torch.randn(K, 16, generator=g).numpy() for K in (7, 90)]
+    ctx.set_prototypes(models[1])
+
+    def work():
+        out = []
+        for r in rows:
+            out += ctx.sample(r, u, top_k=40, top_p=0.9) + ctx.sample(r, u, top_p=0.8) + ctx.sample(r, u, top_k=600, min_p=0.01)
+        for x in X:
+            out += [ctx.scores(x), *ctx.assign_sampled(x, u[:1].expand(len(x)).contiguous())]
+        for G, idx, K in grads:
+            out += [*ctx.lookup_gradient(G, idx, K=K, want_counts=True), ctx.lookup(idx, table=G)]
+        return out
+
+    work()
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            held.append(work())
+    for step in range(3):
+        for r in rows:
+            r.mul_(0.9).add_(torch.randn(r.shape, generator=g).cuda())
+        for G, idx, K in grads:
+            G.neg_()
+            idx.copy_(torch.randint(-1, K, (len(idx),), generator=g).int())
+        want = work()
+        torch.cuda.synchronize()
+        for graph, out in zip(graphs, held):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), step
+            work()
+
+
+@pytest.mark.parametrize("K,D", [(3, 4), (16, 16), (31, 4), (40, 12), (64, 3), (100, 16), (20, 30), (300, 20)])
+def test_scores_do_not_depend_on_the_rows_beside(ctx, K, D):
+    """What the chunks of assign_sampled rest on.  Up to 16 values the same bits; beyond, a close pair is measured alone or with a
+    whole tile, two orders of the same D terms of one sign: at most 2 (D + 3) 2^-24 of the distance apart."""
+    g = gen(K + D)
+    W, X = torch.randn(K, D, generator=g), torch.randn(700, D, generator=g)
+    X[::7] = W[torch.randint(K, (100,), generator=g)] + 0.05 * torch.randn(100, D, generator=g)
+    X = X.cuda()
+    ctx.set_prototypes(W.numpy())
+    S = ctx.scores(X)
+    for a, b in ((0, 1), (1, 2), (100, 613), (699, 700)):
+        part = ctx.scores(X[a:b].contiguous())
+        if D <= 16:
+            assert torch.equal(part, S[a:b])
+        else:
+            assert ((part - S[a:b]).abs() <= 2 * (D + 3) * 2.0 ** -24 * S[a:b].abs()).all()
