@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
         for (int i = 0; i < COPIES; ++i) pw[i] = img[COPY % THREADS == 0 ? t + i * THREADS : min(t + i * THREADS, COPY - 1)];
         if (step + 1 < steps) img += imgStep;
     };
-    auto stage = [&](int b, int u, uint32_t step) {
+    auto stage = [&](int b, int u, uint32_t step, auto whole) {
 #pragma unroll
         for (int i = 0; i < COPIES; ++i)
             if (COPY % THREADS == 0 || t + i * THREADS < COPY) *(u32x4 *)&lw[b][4 * (t + i * THREADS)] = pw[i];
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
         for (int i = 0; i < XPARTS; ++i) {
             const float4 v = px[u][i];
             float4 x = make_float4(v.x - pc.x, v.y - pc.y, v.z - pc.z, v.w - pc.w);
-            if ((step + 1) * MF_K > a.D) {
+            if (!decltype(whole)::value && (step + 1) * MF_K > a.D) {
                 const uint32_t d = step * MF_K + sd;
                 x = make_float4(d < a.D ? x.x : 0.0f, d + 1 < a.D ? x.y : 0.0f, d + 2 < a.D ? x.z : 0.0f, d + 3 < a.D ? x.w : 0.0f);
             }
@@ -362,35 +362,53 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
     fetch(0);
 #pragma unroll
     for (int u = 0; u < PREFETCH; ++u) samples(u, u);
-    stage(0, 0, 0);
+    stage(0, 0, 0, std::false_type());
     fetch(min(1u, steps - 1));
     samples(0, PREFETCH);
     __syncthreads();
-    for (uint32_t k0 = 0; k0 < steps; k0 += PREFETCH) {
+    auto multiply = [&](int b) {
+        u32x4 fx[RW][3];
+#pragma unroll
+        for (int i = 0; i < RW; ++i)
+#pragma unroll
+            for (int c = 0; c < 3; ++c) fx[i][c] = piece(lx[b], wr * MT + i * 32 + l31, c);
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+            u32x4 fw[3];
+#pragma unroll
+            for (int c = 0; c < 3; ++c) fw[c] = piece(lw[b], wc * NT + j * 32 + l31, c);
+            // the six products that matter, the smallest first
+            constexpr int PX[6] = {2, 0, 1, 1, 0, 0}, PW[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+            for (int p = 0; p < 6; ++p)
+#pragma unroll
+                for (int i = 0; i < RW; ++i) acc[i][j] = mma_bf(fx[i][PX[p]], fw[PW[p]], acc[i][j]);
+        }
+    };
+    // Steps whose successor is whole, without a branch, so that the next step's staging is scheduled among the products: 20011
+    // x 784 against 1000 192 us, with the branch 205
+    const uint32_t whole = a.D / MF_K;
+    uint32_t k0 = 0;
+    for (; k0 + PREFETCH < whole; k0 += PREFETCH) {
+#pragma unroll
+        for (int u = 0; u < PREFETCH; ++u) {
+            const int next = (u + 1) % PREFETCH;
+            multiply(u & 1);
+            stage((u & 1) ^ 1, next, k0 + u + 1, std::true_type());
+            fetch(k0 + u + 2);
+            samples(next, k0 + u + 1 + PREFETCH);
+            __syncthreads();
+        }
+    }
+    for (; k0 < steps; k0 += PREFETCH) {
 #pragma unroll
         for (int u = 0; u < PREFETCH; ++u) {
             const uint32_t k = k0 + u;
             if (k >= steps) break;
-            const int b = u & 1, next = (u + 1) % PREFETCH;
-            u32x4 fx[RW][3];
-#pragma unroll
-            for (int i = 0; i < RW; ++i)
-#pragma unroll
-                for (int c = 0; c < 3; ++c) fx[i][c] = piece(lx[b], wr * MT + i * 32 + l31, c);
-#pragma unroll
-            for (int j = 0; j < CW; ++j) {
-                u32x4 fw[3];
-#pragma unroll
-                for (int c = 0; c < 3; ++c) fw[c] = piece(lw[b], wc * NT + j * 32 + l31, c);
-                // the six products that matter, the smallest first
-                constexpr int PX[6] = {2, 0, 1, 1, 0, 0}, PW[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-                for (int p = 0; p < 6; ++p)
-#pragma unroll
-                    for (int i = 0; i < RW; ++i) acc[i][j] = mma_bf(fx[i][PX[p]], fw[PW[p]], acc[i][j]);
-            }
+            const int next = (u + 1) % PREFETCH;
+            multiply(u & 1);
             if (k + 1 < steps) {
-                stage(b ^ 1, next, k + 1);
+                stage((u & 1) ^ 1, next, k + 1, std::false_type());
                 fetch(k + 2);
                 samples(next, k + 1 + PREFETCH);
             }
