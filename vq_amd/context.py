@@ -316,7 +316,7 @@ class Context:
             raise VqhipError(_lib.ERR_STATE, "no prototypes set (vqhip_set_prototypes)")
         N = X.shape[0]
         if out is None:
-            out, ld = torch.empty((N, self.K), dtype=torch.float32, device=X.device), self.K
+            out, ld = torch.empty(N, self.K, dtype=torch.float32, device=X.device), self.K
         else:
             self._check_rows(out, "out")
             ld = self._check_out(out, N, self.K, (torch.float32,))
@@ -329,7 +329,7 @@ class Context:
         -> (idx int32, prob float32).  Each parameter is a number or a CUDA tensor of N (float32; top_k int32)."""
         N, V, ld, code = self._check_rows(scores, "scores")
         how = self._sampling(N, u, temperature, top_k, top_p, min_p)
-        idx, prob = self._drawn(N, scores)
+        idx, prob = self._drawn(u)
         self._chk(self._L.vqhip_sample_device(self._h, scores.data_ptr(), code, N, V, ld, how, u.data_ptr(), idx.data_ptr(), prob.data_ptr(), self._stream()))
         return idx, prob
 
@@ -342,7 +342,7 @@ class Context:
         need = C.c_size_t(0)
         self._chk(self._L.vqhip_assign_sampled_workspace(self._h, N, need))
         work = self._workspace(need.value, X)
-        idx, prob = self._drawn(N, X)
+        idx, prob = self._drawn(u)
         self._chk(self._L.vqhip_assign_sampled_device(self._h, X.data_ptr(), N, how, u.data_ptr(), idx.data_ptr(), prob.data_ptr(), work.data_ptr(),
                                                       need.value, self._stream()))
         return idx, prob
@@ -362,7 +362,7 @@ class Context:
             K, D, ldt, code = self._check_rows(table, "table")
             dtype, src = table.dtype, table.data_ptr()
         if out is None:
-            out, ldy = torch.empty((*idx.shape, D), dtype=dtype, device=idx.device), D
+            out, ldy = torch.empty(*idx.shape, D, dtype=dtype, device=idx.device), D
         else:
             rows = self._rows_of(out, "out", idx, D)
             self._check_rows(rows, "out")
@@ -389,7 +389,7 @@ class Context:
         if out is None:
             if accumulate:
                 raise ValueError("accumulate needs out")
-            out, ldt = torch.empty((K, D), dtype=out_dtype or torch.float32, device=idx.device), D
+            out, ldt = torch.empty(K, D, dtype=out_dtype or torch.float32, device=idx.device), D
         else:
             self._check_rows(out, "out")
             ldt = self._check_out(out, K, D, (out_dtype or out.dtype,))
@@ -408,35 +408,30 @@ class Context:
         """The vqhip_sampling of a call, and the checks of its device arrays."""
         import torch
 
-        def column(v, name, dtype):
-            if not _is_torch(v):
-                return None
-            if not (v.get_device() == self.device and v.dtype == dtype and v.is_contiguous() and tuple(v.shape) == (N,)):
-                raise ValueError(f"{name} must be a number or a contiguous CUDA {dtype} tensor of {N} values on cuda:{self.device}")
-            return v.data_ptr() if N else None
-
-        if not _is_torch(u):
-            raise ValueError(f"u must be a contiguous CUDA torch.float32 tensor of {N} values on cuda:{self.device}")
-        column(u, "u", torch.float32)
-        t, k = column(temperature, "temperature", torch.float32), column(top_k, "top_k", torch.int32)
-        p, m = column(top_p, "top_p", torch.float32), column(min_p, "min_p", torch.float32)
+        self._column(u, "u", torch.float32, N)
+        t = p = m = k = None
         if _is_torch(temperature):
-            temperature = 1.0
+            temperature, t = 1.0, self._column(temperature, "temperature", torch.float32, N)
         if _is_torch(top_p):
-            top_p = 1.0
+            top_p, p = 1.0, self._column(top_p, "top_p", torch.float32, N)
         if _is_torch(min_p):
-            min_p = 0.0
+            min_p, m = 0.0, self._column(min_p, "min_p", torch.float32, N)
         if _is_torch(top_k):
-            top_k = 0
+            top_k, k = 0, self._column(top_k, "top_k", torch.int32, N)
         elif not 0 <= top_k < 1 << 32:
             raise ValueError("top_k must not be negative")
         return _lib.Sampling(float(temperature), float(top_p), float(min_p), int(top_k), t, p, m, k)
 
+    def _column(self, v, name, dtype, N):
+        if not (_is_torch(v) and v.get_device() == self.device and v.dtype is dtype and v.is_contiguous() and v.shape == (N,)):
+            raise ValueError(f"{name} must be {'' if name == 'u' else 'a number or '}a contiguous CUDA {dtype} tensor of {N} values on cuda:{self.device}")
+        return v.data_ptr() if N else None
+
     @staticmethod
-    def _drawn(N, like):
+    def _drawn(u):
         import torch
 
-        return torch.empty(N, dtype=torch.int32, device=like.device), torch.empty(N, dtype=torch.float32, device=like.device)
+        return torch.empty_like(u, dtype=torch.int32), torch.empty_like(u)
 
     @staticmethod
     def _workspace(size, like):
