@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad_join(const GradArgs a, ui
 // ---------------------------------------------------------------------------------------------- all in one launch
 // For few rows and a table that is not large: every workgroup sorts all indices for itself (a few us, instead of two more launches
 // with their partial sums in memory between them) and then does one column slab of one part of the table.
-constexpr uint32_t SINGLE_ROWS = 4096;                              // indices
+constexpr uint32_t SINGLE_ROWS = 8192;                              // indices
 constexpr uint64_t SINGLE_BYTES = 32u << 20;                        // of the table
 constexpr uint32_t SINGLE_PART = 32768;                             // rows of a part
 
@@ -747,8 +747,10 @@ hipError_t run_reduce(const GradArgs &a, const uint32_t *single, uint32_t parts,
     if (single) {
         if (a.N <= 1024)
             hipLaunchKernelGGL((k_grad_single<T, TO, E, 256, 4>), dim3(a.slabs * parts), dim3(256), 0, s, a, single, key_bits, parts);
-        else
+        else if (a.N <= 4096)
             hipLaunchKernelGGL((k_grad_single<T, TO, E, 1024, 4>), dim3(a.slabs * parts), dim3(1024), 0, s, a, single, key_bits, parts);
+        else
+            hipLaunchKernelGGL((k_grad_single<T, TO, E, 1024, 8>), dim3(a.slabs * parts), dim3(1024), 0, s, a, single, key_bits, parts);
         return hipGetLastError();
     }
     const uint32_t groups = GRAD_THREADS >> a.log2g;
@@ -811,7 +813,7 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
     while ((1u << a.log2g) < steps && a.log2g < 6) ++a.log2g;
     a.slabs = (steps + (1u << a.log2g) - 1) >> a.log2g;
     // One launch: about one workgroup a CU, each with 64 rows of the table or more and no more than 128 KiB to read, which is a few
-    // us.  3001 rows of 515 over 997: 23 us in three launches, 17 in one.
+    // us.  3001 rows of 515 over 997: 23 us in three launches, 17 in one; 8000 of 256 over 30000 32 and 25.
     const uint32_t parts = std::max(std::max(1u, std::min(256 / std::min(a.slabs, 256u), (K + 63) / 64)), (K + SINGLE_PART - 1) / SINGLE_PART);
     const bool one = N > 0 && N <= SINGLE_ROWS && (uint64_t)K * D * bo <= SINGLE_BYTES && N * D * bi <= (uint64_t)a.slabs * parts * (128u << 10);
     const uint32_t *single = one ? didx : nullptr;
