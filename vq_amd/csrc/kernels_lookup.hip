@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(THREADS) k_sort_move(const SortArgs a)
 
 // All passes in one workgroup and one launch, for at most THREADS x ITEMS rows.
 constexpr uint32_t SMALL_TILE = 8192;
-constexpr int SMALL_MAX_BITS = 8;
+constexpr int SMALL_MAX_BITS = 9;                                    // 256 indices and one for the rows without a place: one pass
 
 template <int THREADS, int ITEMS>
 __device__ __forceinline__ void sort_in_lds(const SortArgs &a, int key_bits, uint32_t *lkey, uint32_t *lrow, uint16_t *count, uint32_t *first, uint32_t *tmp)
