@@ -205,6 +205,7 @@ struct SortArgs {
     const uint32_t *mark;           // the indices, or null
     uint32_t N, K, tiles;
     int shift, bits;
+    int scanned;                    // k_sort_scan has summed hist; otherwise every tile of a move does
     ZeroArgs zero;                  // rows to clear beside the first move
 };
 
@@ -339,12 +340,37 @@ __global__ void __launch_bounds__(THREADS) k_sort_move(const SortArgs a)
         key[j] = p < valid ? load_key(a, begin + p) : 0;
         row[j] = p < valid ? (a.idx ? begin + p : a.rows_in[begin + p]) : 0;
     }
-    for (uint32_t b = threadIdx.x; b < nb; b += THREADS) base[b] = a.total[b];
+    constexpr int EACH = (1 << SORT_MAX_BITS) / THREADS;
+    uint32_t before[EACH];                                                  // of this lane's bins: in the tiles in front of this one
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const uint32_t b = threadIdx.x + j * THREADS;
+        before[j] = 0;
+        if (b < nb) {
+            const uint32_t *h = a.hist + (size_t)b * a.tiles;
+            if (a.scanned) {
+                before[j] = h[tile];
+                base[b] = a.total[b];
+            } else {
+                uint32_t all = 0;
+                for (uint32_t i = 0; i < a.tiles; ++i) {
+                    const uint32_t v = h[i];
+                    before[j] += i < tile ? v : 0;
+                    all += v;
+                }
+                base[b] = all;
+            }
+        }
+    }
     __syncthreads();
     scan_bins<THREADS>(base, nb, tmp);
     rank_tile<WAVES, ITEMS, SORT_MAX_BITS>(key, valid, a.shift, a.bits, count, first, tmp, rank);
     // where this tile's elements of a digit go, less their first place in the tile
-    for (uint32_t b = threadIdx.x; b < nb; b += THREADS) base[b] += a.hist[(size_t)b * a.tiles + tile] - first[b];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const uint32_t b = threadIdx.x + j * THREADS;
+        if (b < nb) base[b] += before[j] - first[b];
+    }
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j)
         if ((w * ITEMS + j) * 64 + lane < valid) {
@@ -428,11 +454,14 @@ void run_sort_small(const SortArgs &a, int key_bits, hipStream_t s)
 }
 
 template <int THREADS, int ITEMS>
-void run_sort_pass(const SortArgs &a, hipStream_t s)
+void run_sort_pass(SortArgs a, hipStream_t s)
 {
     const uint32_t nb = 1u << a.bits, marks = a.mark ? std::min<uint32_t>((a.N + 255) / 256, 1024) : 0;
+    // a launch less where the table of counts is small (32 KiB at most) and a row of it short: every tile sums it for itself.  us: 9000
+    // rows of 64 over 256 23.5 / 21.4, 20000 of 64 over 30000 (two passes) 38.9 / 35.5; 49 tiles, 100000 of 8 over 30: 31.9 / 36.7
+    a.scanned = marks || a.tiles > 16 || (uint64_t)nb * a.tiles > 8192;
     hipLaunchKernelGGL((k_sort_count<THREADS, ITEMS>), dim3(a.tiles), dim3(THREADS), 0, s, a);
-    hipLaunchKernelGGL(k_sort_scan, dim3(nb + marks), dim3(256), 0, s, a);
+    if (a.scanned) hipLaunchKernelGGL(k_sort_scan, dim3(nb + marks), dim3(256), 0, s, a);
     hipLaunchKernelGGL((k_sort_move<THREADS, ITEMS>), dim3(a.tiles + a.zero.blocks), dim3(THREADS), nb * (8 + THREADS / 64 * 2), s, a);
 }
 
@@ -820,7 +849,7 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
     // Rows no index names are cleared beside the sort, whose few workgroups leave the memory idle, where clearing takes longer
     // than telling the rows apart beforehand (two small launches; 16384 rows of 4096 over 65536: 334 us without, 270 with).
     const bool early = N > 0 && !accumulate && (uint64_t)K * D * bo > SINGLE_BYTES;
-    SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), nullptr, (uint32_t)N, K, p.tiles, 0, p.bits, {}};
+    SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), nullptr, (uint32_t)N, K, p.tiles, 0, p.bits, 0, {}};
     ZeroArgs zero{(char *)dT, ldt * bo, (uint64_t)D * bo, (uint32_t)wo, 0, 0};
     while (((uint64_t)wo << zero.log2g) < zero.bytes && zero.log2g < 8) ++zero.log2g;
     // A row to a workgroup where rows are 2 KiB or more, and the next one from another: 1000 rows of 512 over 131072 54 us, by 4096
