@@ -22,6 +22,9 @@ namespace {
 
 constexpr int SC_THREADS = 256, SC_K = 16;
 
+// Four floats in one access of 16 bytes, which has to begin at a multiple of 4 only
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
 struct ScoreArgs {
     const float *X, *W, *C;           // C: the mean prototype, D values
     float *S;
@@ -31,21 +34,27 @@ struct ScoreArgs {
     const float *norms;
     uint32_t blocks;                  // of 64 prototypes
     uint32_t colTiles;
-    int vecX, vecW, vecS, vecC;       // rows may be moved 16 bytes at a time
 };
 
 // Reduction values d0 .. d0 + 3 of one row, zero behind D or behind the last row (a pair of zeros adds nothing).
-__device__ __forceinline__ float4 load4(const float *base, uint64_t row, bool on, uint32_t D, uint32_t d0, int vec)
+__device__ __forceinline__ float4 load4(const float *base, uint64_t row, bool on, uint32_t D, uint32_t d0)
 {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (!on || d0 >= D) return v;
     const float *p = base + row * D + d0;
-    if (vec) return *(const float4 *)p;
+    if (d0 + 4 <= D) {
+        const float4u q = *(const float4u *)p;
+        return make_float4(q.x, q.y, q.z, q.w);
+    }
     v.x = p[0];
     if (d0 + 1 < D) v.y = p[1];
     if (d0 + 2 < D) v.z = p[2];
-    if (d0 + 3 < D) v.w = p[3];
     return v;
+}
+__device__ __forceinline__ void store4(float *to, float x, float y, float z, float w)
+{
+    const float4u v = {x, y, z, w};
+    *(float4u *)to = v;
 }
 
 // TX lanes side by side, 8 prototypes each: 128, 64 or 32 prototypes a tile, 8 samples each of the 256 / TX lanes above another.
@@ -73,12 +82,12 @@ __global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs
 #pragma unroll
         for (int h = 0; h < XPARTS; ++h) {
             const uint64_t r = row0 + sr + 64 * h;
-            px[h] = load4(a.X, r, r < a.N, a.D, d + sd, a.vecX);
+            px[h] = load4(a.X, r, r < a.N, a.D, d + sd);
         }
 #pragma unroll
         for (int h = 0; h < WPARTS; ++h) {
             const uint32_t c = col0 + sr + 64 * h;
-            pw[h] = load4(a.W, c, c < a.K, a.D, d + sd, a.vecW);
+            pw[h] = load4(a.W, c, c < a.K, a.D, d + sd);
         }
     };
     auto put = [&](float *to, int ld, const float4 &v) {
@@ -128,8 +137,8 @@ __global__ void __launch_bounds__(SC_THREADS, 2) k_scores_direct(const ScoreArgs
         for (int g = 0; g < 2; ++g) {
             const uint32_t c = col0 + g * (SC_N / 2) + tx * 4;
             float *out = a.S + r * a.ld + c;
-            if (a.vecS && c + 4 <= a.K) {
-                *(float4 *)out = make_float4(-acc[i][g * 4], -acc[i][g * 4 + 1], -acc[i][g * 4 + 2], -acc[i][g * 4 + 3]);
+            if (c + 4 <= a.K) {
+                store4(out, -acc[i][g * 4], -acc[i][g * 4 + 1], -acc[i][g * 4 + 2], -acc[i][g * 4 + 3]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -152,8 +161,8 @@ __global__ void __launch_bounds__(SC_THREADS) k_scores_few(const ScoreArgs a)
     float x[DP];
 #pragma unroll
     for (int d = 0; d < DP; d += 4) {
-        if (a.vecX && (uint32_t)d + 4 <= a.D) {
-            const float4 v = *(const float4 *)(row + d);
+        if ((uint32_t)d + 4 <= a.D) {
+            const float4u v = *(const float4u *)(row + d);
             x[d] = v.x;
             x[d + 1] = v.y;
             x[d + 2] = v.z;
@@ -192,8 +201,8 @@ __global__ void __launch_bounds__(SC_THREADS) k_scores_few(const ScoreArgs a)
                         }
             }
         }
-        if (a.vecS && j + 4 <= a.K) {
-            *(float4 *)(out + j) = make_float4(-s[0], -s[1], -s[2], -s[3]);
+        if (j + 4 <= a.K) {
+            store4(out + j, -s[0], -s[1], -s[2], -s[3]);
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -244,7 +253,7 @@ __global__ void __launch_bounds__(256) k_scores_image(const float *W, const floa
     const uint32_t block = blockIdx.x % blocks, step = blockIdx.x / blocks;
     const int row = threadIdx.x >> 2, quad = threadIdx.x & 3;
     const uint32_t k = block * 64 + row, d = step * MF_K + quad * 4;
-    const float4 w = load4(W, k, k < K, D, d, 0), c = load4(C, 0, k < K, D, d, 0);
+    const float4 w = load4(W, k, k < K, D, d), c = load4(C, 0, k < K, D, d);
     uint32_t p[3], q[3];
     split3(w.x - c.x, w.y - c.y, p[0], p[1], p[2]);
     split3(w.z - c.z, w.w - c.w, q[0], q[1], q[2]);
@@ -273,7 +282,7 @@ __global__ void __launch_bounds__(64) k_scores_norms(const float *W, const float
 // both operands are double buffered there.
 constexpr uint32_t CLOSE_LIST = 512;                   // close pairs a wave measures one by one at most; more: its whole tile
 
-template <int RW, int CW, int WR, int WC, int PER_SIMD, bool VEC>
+template <int RW, int CW, int WR, int WC, int PER_SIMD>
 __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const ScoreArgs a)
 {
     constexpr int THREADS = WR * WC * 64, TM = 32 * RW * WR, TN = 32 * CW * WC, MT = 32 * RW, NT = 32 * CW;
@@ -315,8 +324,8 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
     }
     auto values = [&](const float *row, uint32_t step) -> float4 {
         const uint32_t d = step * MF_K + sd;
-        if constexpr (VEC) return *(const float4 *)(row + min(d, a.D - 4));
-        return make_float4(row[min(d, a.D - 1)], row[min(d + 1, a.D - 1)], row[min(d + 2, a.D - 1)], row[min(d + 3, a.D - 1)]);
+        const float4u v = *(const float4u *)(row + min(d, a.D - 4));               // (the last four where there are fewer left)
+        return make_float4(v.x, v.y, v.z, v.w);
     };
     auto samples = [&](int u, uint32_t step) {
 #pragma unroll
@@ -338,7 +347,8 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
             float4 x = make_float4(v.x - pc.x, v.y - pc.y, v.z - pc.z, v.w - pc.w);
             if (!decltype(whole)::value && (step + 1) * MF_K > a.D) {
                 const uint32_t d = step * MF_K + sd;
-                x = make_float4(d < a.D ? x.x : 0.0f, d + 1 < a.D ? x.y : 0.0f, d + 2 < a.D ? x.z : 0.0f, d + 3 < a.D ? x.w : 0.0f);
+                const uint32_t over = d + 4 > a.D ? d + 4 - a.D : 0;               // values behind the last: what is here is that far ahead
+                x = over == 0 ? x : over == 1 ? make_float4(x.y, x.z, x.w, 0.0f) : over == 2 ? make_float4(x.z, x.w, 0.0f, 0.0f) : over == 3 ? make_float4(x.w, 0.0f, 0.0f, 0.0f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
             sx[i] = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, fmaf(x.w, x.w, sx[i]))));
             uint32_t p[3], q[3];
@@ -485,10 +495,10 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
                 float4 u[4], v[4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    u[h] = load4(x0, 0, true, a.D, d + 64 * h, a.vecX);
-                    v[h] = load4(w0, 0, true, a.D, d + 64 * h, a.vecW);
-                    u[2 + h] = load4(x1, 0, true, a.D, d + 64 * h, a.vecX);
-                    v[2 + h] = load4(w1, 0, true, a.D, d + 64 * h, a.vecW);
+                    u[h] = load4(x0, 0, true, a.D, d + 64 * h);
+                    v[h] = load4(w0, 0, true, a.D, d + 64 * h);
+                    u[2 + h] = load4(x1, 0, true, a.D, d + 64 * h);
+                    v[2 + h] = load4(w1, 0, true, a.D, d + 64 * h);
                 }
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
@@ -521,8 +531,8 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
             float4 x[Q], w[Q];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
-                x[i] = load4(a.X, wrow + ty + 8 * i, wrow + ty + 8 * i < a.N, a.D, d, a.vecX);
-                w[i] = load4(a.W, wcol + c0 + tx + 8 * i, wcol + c0 + tx + 8 * i < a.K, a.D, d, a.vecW);
+                x[i] = load4(a.X, wrow + ty + 8 * i, wrow + ty + 8 * i < a.N, a.D, d);
+                w[i] = load4(a.W, wcol + c0 + tx + 8 * i, wcol + c0 + tx + 8 * i < a.K, a.D, d);
             }
 #pragma unroll
             for (int i = 0; i < Q; ++i)
@@ -562,8 +572,8 @@ hipError_t run_direct(ScoreArgs a, hipStream_t s)
     return hipSuccess;
 }
 
-template <int RW, int CW, int WR, int WC, int PER_SIMD, bool VEC>
-hipError_t run_mfma_as(ScoreArgs a, hipStream_t s)
+template <int RW, int CW, int WR, int WC, int PER_SIMD>
+hipError_t run_mfma(ScoreArgs a, hipStream_t s)
 {
     constexpr uint32_t TM = 32 * RW * WR, TN = 32 * CW * WC;
     static_assert(IMG_PAD % TN == 0, "the image covers every tile");
@@ -576,17 +586,11 @@ hipError_t run_mfma_as(ScoreArgs a, hipStream_t s)
         a.S = S + off * a.ld;
         a.N = std::min(N - off, most);
         const uint64_t tiles = (a.N + TM - 1) / TM * a.colTiles;
-        hipLaunchKernelGGL((k_scores_mfma<RW, CW, WR, WC, PER_SIMD, VEC>), dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(WR * WC * 64), 0, s, a);
+        hipLaunchKernelGGL((k_scores_mfma<RW, CW, WR, WC, PER_SIMD>), dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(WR * WC * 64), 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
-}
-
-template <int RW, int CW, int WR, int WC, int PER_SIMD>
-hipError_t run_mfma(const ScoreArgs &a, hipStream_t s)
-{
-    return a.vecX && a.vecC ? run_mfma_as<RW, CW, WR, WC, PER_SIMD, true>(a, s) : run_mfma_as<RW, CW, WR, WC, PER_SIMD, false>(a, s);
 }
 
 bool is_few(uint32_t K, uint32_t D) { return K <= FEW_K && D <= FEW_D && K * K * D <= 4096; }
@@ -613,14 +617,9 @@ hipError_t launch_scores_image(const float *dW, const float *dC, uint32_t K, uin
 hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const float *dC, const void *dImg, uint32_t K, float *dS, uint64_t ld,
                          hipStream_t s)
 {
-    ScoreArgs a{dX, dW, dC, dS, N, ld, K, D, nullptr, nullptr, image_blocks(K), 0, 0, 0, 0, 0};
+    ScoreArgs a{dX, dW, dC, dS, N, ld, K, D, nullptr, nullptr, image_blocks(K), 0};
     a.img = (const uint32_t *)dImg;
     a.norms = (const float *)(a.img + (size_t)((D + MF_K - 1) / MF_K) * a.blocks * IMG_BLOCK);
-    const bool rows = D % 4 == 0;
-    a.vecX = rows && ((uintptr_t)dX & 15) == 0;
-    a.vecW = rows && ((uintptr_t)dW & 15) == 0;
-    a.vecC = rows && ((uintptr_t)dC & 15) == 0;
-    a.vecS = ld % 4 == 0 && ((uintptr_t)dS & 15) == 0;
     if (is_few(K, D)) {
         const uint64_t most = (1ull << 30) * SC_THREADS;
         for (uint64_t off = 0; off < N; off += most) {
