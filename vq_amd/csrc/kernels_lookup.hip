@@ -165,33 +165,29 @@ __device__ void scan_bins(uint32_t *a, uint32_t n, uint32_t *tmp)
     __syncthreads();
 }
 
-// Rows of zeros where start[k] is NONE, 2^log2g lanes a row, `width` bytes a lane and store
+// Rows of zeros where start[k] is NONE, 2^log2g lanes a row, 16 bytes a lane and store; 2 where rows are no whole words
 struct ZeroArgs {
     char *G;
     uint64_t pitch, bytes;          // of a row, in bytes
-    uint32_t width;
+    int words;
     int log2g;
     uint32_t blocks;                // workgroups that do it, behind the others; 0: none
 };
 
-template <class V>
-__device__ __forceinline__ void zero_rows_by(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
+__device__ __forceinline__ void zero_rows(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
 {
+    typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));                // (16 bytes from any multiple of 4)
     const uint32_t gl = threadIdx.x & ((1u << z.log2g) - 1), groups = threads >> z.log2g;
-    const V zero = 0;
+    const words4 zero = {0, 0, 0, 0};
     for (uint64_t k = (uint64_t)block * groups + (threadIdx.x >> z.log2g); k < K; k += (uint64_t)z.blocks * groups) {
         if (start[k] != NONE) continue;
         char *row = z.G + k * z.pitch;
-        for (uint64_t at = gl * sizeof(V); at < z.bytes; at += sizeof(V) << z.log2g) __builtin_nontemporal_store(zero, (V *)(row + at));
-    }
-}
-__device__ __forceinline__ void zero_rows(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
-{
-    switch (z.width) {
-    case 16: return zero_rows_by<u32x4>(z, start, K, block, threads);
-    case 8: return zero_rows_by<u32x2>(z, start, K, block, threads);
-    case 4: return zero_rows_by<uint32_t>(z, start, K, block, threads);
-    default: return zero_rows_by<uint16_t>(z, start, K, block, threads);
+        if (z.words) {
+            for (uint64_t at = gl * 16; at + 16 <= z.bytes; at += 16ull << z.log2g) __builtin_nontemporal_store(zero, (words4 *)(row + at));
+            for (uint64_t at = (z.bytes & ~15ull) + gl * 4; at < z.bytes; at += 4ull << z.log2g) __builtin_nontemporal_store(0u, (uint32_t *)(row + at));
+        } else {
+            for (uint64_t at = gl * 2; at < z.bytes; at += 2ull << z.log2g) __builtin_nontemporal_store((uint16_t)0, (uint16_t *)(row + at));
+        }
     }
 }
 
@@ -850,8 +846,8 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
     // than telling the rows apart beforehand (two small launches; 16384 rows of 4096 over 65536: 334 us without, 270 with).
     const bool early = N > 0 && !accumulate && (uint64_t)K * D * bo > SINGLE_BYTES;
     SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), nullptr, (uint32_t)N, K, p.tiles, 0, p.bits, 0, {}};
-    ZeroArgs zero{(char *)dT, ldt * bo, (uint64_t)D * bo, (uint32_t)wo, 0, 0};
-    while (((uint64_t)wo << zero.log2g) < zero.bytes && zero.log2g < 8) ++zero.log2g;
+    ZeroArgs zero{(char *)dT, ldt * bo, (uint64_t)D * bo, wo >= 4, 0, 0};
+    while (((wo >= 4 ? 16ull : 2ull) << zero.log2g) < zero.bytes && zero.log2g < 8) ++zero.log2g;
     // A row to a workgroup where rows are 2 KiB or more, and the next one from another: 1000 rows of 512 over 131072 54 us, by 4096
     // workgroups 65; short rows by 4096: 5000 of 64 over 1000000 68 us, by 65536 133.
     const uint64_t shares = zero.bytes >= 2048 ? std::min<uint64_t>((((uint64_t)K << zero.log2g) + 255) / 256, 65536) : std::min<uint64_t>((K + 15) / 16, 4096);
