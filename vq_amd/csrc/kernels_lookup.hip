@@ -53,52 +53,82 @@ struct LookupArgs {
 
 constexpr int LOOK_THREADS = 256;
 
+// 16 bytes of consecutive elements, from any multiple of an element's size: rows of any length and pitch are moved alike
+typedef uint32_t words_by4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t words_by2 __attribute__((ext_vector_type(4), aligned(2)));
+template <class T>
+struct Piece {
+    static constexpr int E = 16 / (int)sizeof(T);
+    using words = typename std::conditional<sizeof(T) == 4, words_by4, words_by2>::type;
+    T v[E];
+};
+template <class T>
+__device__ __forceinline__ Piece<T> load_piece(const T *p) { return __builtin_bit_cast(Piece<T>, (u32x4)*(const typename Piece<T>::words *)p); }
+template <class T>
+__device__ __forceinline__ void store_piece(T *p, const Piece<T> &v) { __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (typename Piece<T>::words *)p); }
+
 // 2^log2g lanes share a row; blockIdx.y picks the column step.  U rows are in flight per lane: index -> row -> store is a
 // chain of two memory latencies, and nothing else hides them.
-template <class T, int BYTES, int U>
+template <class T, int U>
 __global__ void __launch_bounds__(LOOK_THREADS) k_lookup(const LookupArgs a)
 {
-    using P = Pack<T, BYTES>;
+    using P = Piece<T>;
     const int g = 1 << a.log2g;
     const uint32_t col = ((uint32_t)blockIdx.y * g + (threadIdx.x & (g - 1))) * P::E;
     if (col >= a.D) return;
     const uint32_t rows = LOOK_THREADS >> a.log2g;                   // rows of one step of the block
     const T *table = (const T *)a.T + col;
     T *out = (T *)a.Y + col;
-    for (uint64_t base = (uint64_t)blockIdx.x * rows * U + (threadIdx.x >> a.log2g); base < a.N; base += (uint64_t)gridDim.x * rows * U) {
-        uint32_t k[U];
-        P v[U];
+    const uint32_t left = a.D - col;                                 // elements of the row from here on
+    auto work = [&](auto whole) {
+        constexpr bool W = decltype(whole)::value;
+        for (uint64_t base = (uint64_t)blockIdx.x * rows * U + (threadIdx.x >> a.log2g); base < a.N; base += (uint64_t)gridDim.x * rows * U) {
+            uint32_t k[U];
+            P v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t i = base + (uint64_t)u * rows;
-            k[u] = i < a.N ? a.idx[i] : a.K;
-        }
+            for (int u = 0; u < U; ++u) {
+                const uint64_t i = base + (uint64_t)u * rows;
+                k[u] = i < a.N ? a.idx[i] : a.K;
+            }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (k[u] < a.K) {
-                v[u] = *(const P *)(table + (uint64_t)k[u] * a.ldt);
-            } else {
+            for (int u = 0; u < U; ++u) {
+                const T *row = table + (uint64_t)k[u] * a.ldt;
+                if (W && k[u] < a.K) {
+                    v[u] = load_piece(row);
+                } else {
 #pragma unroll
-                for (int e = 0; e < P::E; ++e) v[u].v[e] = (T)0.0f;
+                    for (int e = 0; e < P::E; ++e) v[u].v[e] = !W && k[u] < a.K && (uint32_t)e < left ? row[e] : (T)0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint64_t i = base + (uint64_t)u * rows;
+                if (i >= a.N) break;
+                if (k[u] < a.K) {
+#pragma unroll
+                    for (int e = 0; e < P::E; ++e) v[u].v[e] = narrow<T>(widen(v[u].v[e]) * a.scale);
+                }
+                T *to = out + i * a.ldy;
+                if (W) {
+                    store_piece(to, v[u]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < P::E; ++e)
+                        if ((uint32_t)e < left) to[e] = v[u].v[e];
+                }
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t i = base + (uint64_t)u * rows;
-            if (i >= a.N) break;
-            if (k[u] < a.K) {
-#pragma unroll
-                for (int e = 0; e < P::E; ++e) v[u].v[e] = narrow<T>(widen(v[u].v[e]) * a.scale);
-            }
-            store_past(out + i * a.ldy, v[u]);
-        }
-    }
+    };
+    if (left >= P::E)
+        work(std::true_type());
+    else
+        work(std::false_type());
 }
 
-template <class T, int BYTES>
+template <class T>
 hipError_t run_lookup(LookupArgs a, hipStream_t s)
 {
-    const uint32_t steps = (a.D + BYTES / sizeof(T) - 1) / (uint32_t)(BYTES / sizeof(T));
+    const uint32_t steps = (a.D + Piece<T>::E - 1) / Piece<T>::E;
     a.log2g = 0;
     while ((1u << a.log2g) < steps && a.log2g < 8) ++a.log2g;
     const uint32_t cols = (steps + (1u << a.log2g) - 1) >> a.log2g;
@@ -108,9 +138,9 @@ hipError_t run_lookup(LookupArgs a, hipStream_t s)
     const uint64_t per = four ? 4 * rows : rows;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.N + per - 1) / per, 1u << 20);
     if (four)
-        hipLaunchKernelGGL((k_lookup<T, BYTES, 4>), dim3(blocks, cols), dim3(LOOK_THREADS), 0, s, a);
+        hipLaunchKernelGGL((k_lookup<T, 4>), dim3(blocks, cols), dim3(LOOK_THREADS), 0, s, a);
     else
-        hipLaunchKernelGGL((k_lookup<T, BYTES, 1>), dim3(blocks, cols), dim3(LOOK_THREADS), 0, s, a);
+        hipLaunchKernelGGL((k_lookup<T, 1>), dim3(blocks, cols), dim3(LOOK_THREADS), 0, s, a);
     return hipGetLastError();
 }
 
@@ -176,14 +206,13 @@ struct ZeroArgs {
 
 __device__ __forceinline__ void zero_rows(const ZeroArgs &z, const uint32_t *start, uint32_t K, uint32_t block, uint32_t threads)
 {
-    typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));                // (16 bytes from any multiple of 4)
     const uint32_t gl = threadIdx.x & ((1u << z.log2g) - 1), groups = threads >> z.log2g;
-    const words4 zero = {0, 0, 0, 0};
+    const words_by4 zero = {0, 0, 0, 0};
     for (uint64_t k = (uint64_t)block * groups + (threadIdx.x >> z.log2g); k < K; k += (uint64_t)z.blocks * groups) {
         if (start[k] != NONE) continue;
         char *row = z.G + k * z.pitch;
         if (z.words) {
-            for (uint64_t at = gl * 16; at + 16 <= z.bytes; at += 16ull << z.log2g) __builtin_nontemporal_store(zero, (words4 *)(row + at));
+            for (uint64_t at = gl * 16; at + 16 <= z.bytes; at += 16ull << z.log2g) __builtin_nontemporal_store(zero, (words_by4 *)(row + at));
             for (uint64_t at = (z.bytes & ~15ull) + gl * 4; at < z.bytes; at += 4ull << z.log2g) __builtin_nontemporal_store(0u, (uint32_t *)(row + at));
         } else {
             for (uint64_t at = gl * 2; at < z.bytes; at += 2ull << z.log2g) __builtin_nontemporal_store((uint16_t)0, (uint16_t *)(row + at));
@@ -809,14 +838,10 @@ size_t elem_bytes(int dtype) { return dtype == VQHIP_F32 ? 4 : 2; }
 hipError_t launch_lookup(const void *dT, int dtype, uint64_t ldt, uint32_t K, uint32_t D, const uint32_t *didx, uint64_t N, float scale, void *dY,
                          uint64_t ldy, hipStream_t s)
 {
-    const size_t b = elem_bytes(dtype);
     const LookupArgs a{dT, ldt, didx, N, K, D, scale, dY, ldy, 0};
-    const int w = widest_access(b, (uint64_t)(uintptr_t)dT | (uint64_t)(uintptr_t)dY | ldt * b | ldy * b | (uint64_t)D * b);
-    if (dtype == VQHIP_F32)
-        return w == 16 ? run_lookup<float, 16>(a, s) : w == 8 ? run_lookup<float, 8>(a, s) : run_lookup<float, 4>(a, s);
-    if (dtype == VQHIP_BF16)
-        return w == 16 ? run_lookup<__bf16, 16>(a, s) : w == 8 ? run_lookup<__bf16, 8>(a, s) : w == 4 ? run_lookup<__bf16, 4>(a, s) : run_lookup<__bf16, 2>(a, s);
-    return w == 16 ? run_lookup<_Float16, 16>(a, s) : w == 8 ? run_lookup<_Float16, 8>(a, s) : w == 4 ? run_lookup<_Float16, 4>(a, s) : run_lookup<_Float16, 2>(a, s);
+    if (dtype == VQHIP_F32) return run_lookup<float>(a, s);
+    if (dtype == VQHIP_BF16) return run_lookup<__bf16>(a, s);
+    return run_lookup<_Float16>(a, s);
 }
 
 size_t lookup_gradient_workspace(uint64_t N, uint32_t K, uint32_t D) { return plan_gradient(N, K, D).bytes; }
