@@ -21,13 +21,4 @@ struct alignas(BYTES) Pack {
     T v[E];
 };
 
-// The widest of 16, 8, 4 bytes (or one element) that divides every given address, stride and row length in bytes: what one
-// lane may move at once.  Host side.
-inline int widest_access(size_t elem, uint64_t bits)
-{
-    for (int w : {16, 8, 4})
-        if ((size_t)w >= elem && (bits & (uint64_t)(w - 1)) == 0) return w;
-    return (int)elem;
-}
-
 }  // namespace vq

@@ -27,18 +27,8 @@ namespace vq {
 namespace {
 
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
-using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
 
 // ---------------------------------------------------------------------------------------------- lookup
-// A store that does not stay in the caches: what is written here is read once at best, and the table is read over and over.
-template <class T, int BYTES>
-__device__ __forceinline__ void store_past(T *to, const Pack<T, BYTES> &v)
-{
-    using V = typename std::conditional<BYTES == 16, u32x4, typename std::conditional<BYTES == 8, u32x2,
-                                        typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type>::type;
-    __builtin_nontemporal_store(__builtin_bit_cast(V, v), (V *)to);
-}
-
 struct LookupArgs {
     const void *T;
     uint64_t ldt;
@@ -53,7 +43,8 @@ struct LookupArgs {
 
 constexpr int LOOK_THREADS = 256;
 
-// 16 bytes of consecutive elements, from any multiple of an element's size: rows of any length and pitch are moved alike
+// 16 bytes of consecutive elements, from any multiple of an element's size: rows of any length and pitch are moved alike.  Stores
+// do not stay in the caches: what is written here is read once at best, and the table is read over and over.
 typedef uint32_t words_by4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t words_by2 __attribute__((ext_vector_type(4), aligned(2)));
 template <class T>
@@ -517,21 +508,57 @@ struct GradArgs {
 constexpr int GRAD_THREADS = 256;
 constexpr int GRAD_FLIGHT = 8;      // rows a lane has in flight
 
+// A lane's columns of a row: E of them from `at` on, the first `skip` of which are its neighbour's (the last lane of a row whose
+// length is no multiple of E begins earlier, so that every load is a whole one).
+template <int E>
+struct Columns {
+    uint32_t at, skip;
+    bool mine;
+    __device__ Columns(uint32_t first, uint32_t D) : at(first + E <= D ? first : D - E), skip(first - at), mine(first < D) {}
+};
+template <class T, int E>
+__device__ __forceinline__ Pack<T, E * (int)sizeof(T)> load_columns(const T *p)              // from any multiple of an element's size
+{
+    Pack<T, E * (int)sizeof(T)> v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+}
+template <class T, int E>
+__device__ __forceinline__ void store_columns(T *p, const Pack<T, E * (int)sizeof(T)> &v, uint32_t skip)
+{
+    if (E > 1 && skip == 0) {
+        static_assert(E == 1 || E * sizeof(T) == 16, "one element or 16 bytes");
+        if constexpr (E > 1) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (typename Piece<T>::words *)p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if ((uint32_t)e >= skip) p[e] = v.v[e];
+    }
+}
+
 // One finished row piece: G (+)= scale * sum, rounded once.
 template <class TO, int E>
-__device__ __forceinline__ void store_grad(const GradArgs &a, uint32_t k, uint32_t col, const float (&acc)[E])
+__device__ __forceinline__ void store_grad(const GradArgs &a, uint32_t k, const Columns<E> &c, const float (&acc)[E])
 {
-    TO *g = (TO *)a.G + (uint64_t)k * a.ldg + col;
+    TO *g = (TO *)a.G + (uint64_t)k * a.ldg + c.at;
     Pack<TO, E * (int)sizeof(TO)> o;
     if (a.accumulate) {
-        o = *(const Pack<TO, E * (int)sizeof(TO)> *)g;
+        o = load_columns<TO, E>(g);
 #pragma unroll
         for (int e = 0; e < E; ++e) o.v[e] = narrow<TO>(fmaf(acc[e], a.scale, widen(o.v[e])));
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) o.v[e] = narrow<TO>(acc[e] * a.scale);
     }
-    store_past(g, o);
+    store_columns<TO, E>(g, o, c.skip);
+}
+template <class TO, int E>
+__device__ __forceinline__ void store_zeros(const GradArgs &a, uint64_t k, const Columns<E> &c)
+{
+    Pack<TO, E * (int)sizeof(TO)> zero;
+#pragma unroll
+    for (int e = 0; e < E; ++e) zero.v[e] = (TO)0.0f;
+    store_columns<TO, E>((TO *)a.G + k * a.ldg + c.at, zero, c.skip);
 }
 
 // Sums the runs of the sorted places [p0, p1) over this lane's E columns (at dY; none of its own: !mine) in their order.  done(k,
@@ -558,7 +585,7 @@ __device__ __forceinline__ void sum_runs(const Keys keys, const Keys rows, uint3
         }
 #pragma unroll
         for (int j = 0; j < GRAD_FLIGHT; ++j)                      // (a row without a place is not read: its batch's first is, again)
-            v[j] = *(const Pack<T, E * (int)sizeof(T)> *)(dY + (uint64_t)(key[j] < K ? row[j] : row[0]) * ldy);
+            v[j] = load_columns<T, E>(dY + (uint64_t)(key[j] < K ? row[j] : row[0]) * ldy);
 #pragma unroll
         for (int j = 0; j < GRAD_FLIGHT; ++j) {
             if (p + j < p1) {
@@ -585,22 +612,22 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad_reduce(const GradArgs a)
     const uint32_t c = (uint32_t)(group / a.slabs), slab = (uint32_t)(group % a.slabs);
     if (c >= a.chunks) return;
     const uint32_t gl = threadIdx.x & ((1u << a.log2g) - 1);
-    const uint32_t col = ((slab << a.log2g) + gl) * E;
-    const bool mine = col < a.D, first = slab == 0 && gl == 0;
+    const Columns<E> cols(((slab << a.log2g) + gl) * E, a.D);
+    const bool first = slab == 0 && gl == 0;
     const uint32_t p0 = c * a.chunk, p1 = min(a.N, p0 + a.chunk);
     const bool left = p0 > 0 && a.keys[p0 - 1] == a.keys[p0];     // the first run began in an earlier chunk
     const uint32_t behind = p1 < a.N ? a.keys[p1] : NONE;
-    sum_runs<T, E>(a.keys, a.rows, p0, p1, a.K, (const T *)a.dY + (mine ? col : 0), a.ldy, [&](uint32_t k, uint32_t from, uint32_t upto, const float (&acc)[E]) {
+    sum_runs<T, E>(a.keys, a.rows, p0, p1, a.K, (const T *)a.dY + (cols.mine ? cols.at : 0), a.ldy, [&](uint32_t k, uint32_t from, uint32_t upto, const float (&acc)[E]) {
         const bool l = from == p0 && left, r = upto == p1 && behind == k;
         if (first) {
             if (!l) a.start[k] = from;
             if (!r) a.end[k] = upto;
         }
-        if (!mine) return;
+        if (!cols.mine) return;
         if (!l && !r) {
-            store_grad<TO, E>(a, k, col, acc);
+            store_grad<TO, E>(a, k, cols, acc);
         } else {
-            float *part = a.parts + ((size_t)c * 2 + (l ? 0 : 1)) * a.dpad + col;
+            float *part = a.parts + ((size_t)c * 2 + (l ? 0 : 1)) * a.dpad + cols.at;
 #pragma unroll
             for (int e = 0; e < E; ++e) part[e] = acc[e];
         }
@@ -622,17 +649,16 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad_join(const GradArgs a, ui
         const uint32_t k = a.keys[p1 - 1];
         if (k >= a.K || a.keys[p1] != k || a.start[k] < c * a.chunk) return;
         const uint32_t more = (a.end[k] - 1) / a.chunk - c;                        // chunks behind this one that the run reaches
-        const uint32_t col = (slab * gsize + gl) * E;
-        const bool mine = col < a.D;
+        const Columns<E> cols((slab * gsize + gl) * E, a.D);
         const uint32_t per = (more + groups - 1) / groups;
         float acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-        if (mine) {
+        if (cols.mine) {
             const uint32_t lo = gi * per, hi = min(more, lo + per);
 #pragma unroll 8
             for (uint32_t j = lo; j < hi; ++j) {
-                const float *part = a.parts + (size_t)(c + 1 + j) * 2 * a.dpad + col;
+                const float *part = a.parts + (size_t)(c + 1 + j) * 2 * a.dpad + cols.at;
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] += part[e];
             }
@@ -640,14 +666,14 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad_join(const GradArgs a, ui
 #pragma unroll
         for (int e = 0; e < E; ++e) share[(gi * gsize + gl) * E + e] = acc[e];
         __syncthreads();
-        if (gi != 0 || !mine) return;
-        const float *tail = a.parts + ((size_t)c * 2 + 1) * a.dpad + col;
+        if (gi != 0 || !cols.mine) return;
+        const float *tail = a.parts + ((size_t)c * 2 + 1) * a.dpad + cols.at;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = tail[e];
         for (uint32_t g = 0; g < groups && g * per < more; ++g)
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] += share[(g * gsize + gl) * E + e];
-        store_grad<TO, E>(a, k, col, acc);
+        store_grad<TO, E>(a, k, cols, acc);
         return;
     }
     const uint64_t lanes = (uint64_t)(gridDim.x - join_blocks) * groups;
@@ -655,10 +681,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad_join(const GradArgs a, ui
         const uint32_t s = a.start[k];
         if (a.counts && gl == 0) a.counts[k] = s == NONE ? 0 : a.end[k] - s;
         if (s != NONE || a.accumulate || a.cleared) continue;
-        Pack<TO, E * (int)sizeof(TO)> zero;
-#pragma unroll
-        for (int e = 0; e < E; ++e) zero.v[e] = (TO)0.0f;
-        for (uint32_t col = gl * E; col < a.D; col += gsize * E) *(Pack<TO, E * (int)sizeof(TO)> *)((TO *)a.G + k * a.ldg + col) = zero;
+        for (uint32_t col = gl * E; col < a.D; col += gsize * E) store_zeros<TO, E>(a, k, Columns<E>(col, a.D));
     }
 }
 
@@ -703,8 +726,8 @@ __global__ void __launch_bounds__(THREADS) k_grad_single(const GradArgs a, const
 
     const uint32_t lo = lower_place(lkey, a.N, k0), hi = lower_place(lkey, a.N, k1);
     const uint32_t gsize = 1u << a.log2g, gl = threadIdx.x & (gsize - 1), g = threadIdx.x >> a.log2g, groups = THREADS >> a.log2g;
-    const uint32_t col = (slab * gsize + gl) * E;
-    const bool mine = col < a.D;
+    const Columns<E> cols((slab * gsize + gl) * E, a.D);
+    const bool mine = cols.mine;
     const uint32_t per = (hi - lo + groups - 1) / groups;
     const uint32_t p0 = min(hi, lo + g * per), p1 = min(hi, p0 + per);
     for (uint32_t p = lo + threadIdx.x; p < hi; p += THREADS) {
@@ -715,10 +738,10 @@ __global__ void __launch_bounds__(THREADS) k_grad_single(const GradArgs a, const
     if (p0 < p1) {
         const bool left = p0 > 0 && lkey[p0 - 1] == lkey[p0];
         const uint32_t behind = p1 < a.N ? lkey[p1] : NONE;
-        sum_runs<T, E>(lkey, lrow, p0, p1, a.K, (const T *)a.dY + (mine ? col : 0), a.ldy, [&](uint32_t k, uint32_t from, uint32_t upto, const float (&acc)[E]) {
+        sum_runs<T, E>(lkey, lrow, p0, p1, a.K, (const T *)a.dY + (cols.mine ? cols.at : 0), a.ldy, [&](uint32_t k, uint32_t from, uint32_t upto, const float (&acc)[E]) {
             const bool l = from == p0 && left, r = upto == p1 && behind == k;
             if (!l && !r) {
-                if (mine) store_grad<TO, E>(a, k, col, acc);
+                if (mine) store_grad<TO, E>(a, k, cols, acc);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) part[l ? 0 : 1][threadIdx.x * E + e] = acc[e];
@@ -737,17 +760,13 @@ __global__ void __launch_bounds__(THREADS) k_grad_single(const GradArgs a, const
             for (uint32_t h = 1; at < hi && lkey[at] == k; ++h, at += per)
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] += part[0][(threadIdx.x + h * gsize) * E + e];
-            store_grad<TO, E>(a, k, col, acc);
+            store_grad<TO, E>(a, k, cols, acc);
         }
     }
     for (uint32_t k = k0 + g; k < k1; k += groups) {
         if ((present[(k - k0) / 32] >> ((k - k0) % 32)) & 1) continue;
         if (a.counts && slab == 0 && gl == 0) a.counts[k] = 0;
-        if (a.accumulate || !mine) continue;
-        Pack<TO, E * (int)sizeof(TO)> zero;
-#pragma unroll
-        for (int e = 0; e < E; ++e) zero.v[e] = (TO)0.0f;
-        store_past((TO *)a.G + (uint64_t)k * a.ldg + col, zero);
+        if (!a.accumulate && mine) store_zeros<TO, E>(a, k, cols);
     }
 }
 
@@ -823,12 +842,8 @@ hipError_t run_reduce(const GradArgs &a, const uint32_t *single, uint32_t parts,
 template <class T, class TO>
 hipError_t run_reduce_width(const GradArgs &a, int e, const uint32_t *single, uint32_t parts, int key_bits, hipStream_t s)
 {
-    if constexpr (sizeof(TO) == 2) {
-        if (e >= 8) return run_reduce<T, TO, 8>(a, single, parts, key_bits, s);
-    }
-    if (e >= 4) return run_reduce<T, TO, 4>(a, single, parts, key_bits, s);
-    if (e >= 2) return run_reduce<T, TO, 2>(a, single, parts, key_bits, s);
-    return run_reduce<T, TO, 1>(a, single, parts, key_bits, s);
+    constexpr int E = 16 / (int)sizeof(TO);
+    return e == E ? run_reduce<T, TO, E>(a, single, parts, key_bits, s) : run_reduce<T, TO, 1>(a, single, parts, key_bits, s);
 }
 
 size_t elem_bytes(int dtype) { return dtype == VQHIP_F32 ? 4 : 2; }
@@ -853,26 +868,36 @@ hipError_t launch_lookup_gradient(const void *dG, int dtype, uint64_t ldg, const
     char *w = (char *)dwork;
     auto at = [&](size_t o) { return (uint32_t *)(w + o); };
     const size_t bi = elem_bytes(dtype), bo = elem_bytes(out_dtype);
-    // elements a lane takes at once: what 16 bytes of the rows and of the table hold, if they and their strides are aligned for it
-    const int wi = widest_access(bi, (uint64_t)(uintptr_t)dG | ldg * bi | (uint64_t)D * bi);
-    const int wo = widest_access(bo, (uint64_t)(uintptr_t)dT | ldt * bo | (uint64_t)D * bo);
-    const int n = std::min(wi / (int)bi, wo / (int)bo);
     GradArgs a{dG, ldg, at(p.keys[0]), at(p.rows[0]), (uint32_t)N, K, D, scale, dT, ldt, accumulate ? 1 : 0, 0, at(p.start), at(p.end), dcounts,
                (float *)(w + p.parts), p.dpad, p.chunk, p.chunks, 0, 0};
-    const uint32_t steps = (D + n - 1) / n;
-    while ((1u << a.log2g) < steps && a.log2g < 6) ++a.log2g;
-    a.slabs = (steps + (1u << a.log2g) - 1) >> a.log2g;
-    // One launch: about one workgroup a CU, each with 64 rows of the table or more and no more than 128 KiB to read, which is a few
-    // us.  3001 rows of 515 over 997: 23 us in three launches, 17 in one; 8000 of 256 over 30000 32 and 25.
-    const uint32_t parts = std::max(std::max(1u, std::min(256 / std::min(a.slabs, 256u), (K + 63) / 64)), (K + SINGLE_PART - 1) / SINGLE_PART);
-    const bool one = N > 0 && N <= SINGLE_ROWS && (uint64_t)K * D * bo <= SINGLE_BYTES && N * D * bi <= (uint64_t)a.slabs * parts * (128u << 10);
+    const int wide = (int)(16 / bo);
+    int n = 0;                                                              // elements a lane takes at once
+    uint32_t parts = 0;
+    bool one = false;
+    auto shape = [&](int elements) {
+        n = elements;
+        const uint32_t steps = (D + n - 1) / n;
+        a.log2g = 0;
+        while ((1u << a.log2g) < steps && a.log2g < 6) ++a.log2g;
+        a.slabs = (steps + (1u << a.log2g) - 1) >> a.log2g;
+        // One launch: about one workgroup a CU, each with 64 rows of the table or more and no more than 128 KiB to read, which is a few
+        // us.  3001 rows of 515 over 997: 23 us in three launches, 17 in one; 8000 of 256 over 30000 32 and 25.
+        parts = std::max(std::max(1u, std::min(256 / std::min(a.slabs, 256u), (K + 63) / 64)), (K + SINGLE_PART - 1) / SINGLE_PART);
+        one = N > 0 && N <= SINGLE_ROWS && (uint64_t)K * D * bo <= SINGLE_BYTES && N * D * bi <= (uint64_t)a.slabs * parts * (128u << 10);
+    };
+    // 16 bytes of the table, or one element where they do not divide the row and it is short or the launch the only one: a row's
+    // last lane then stores by elements.  us by 16 bytes / by one: 300000 rows of 203 over 5000 bf16 70 / 108, 50000 of 1001 over
+    // 1000 f32 63 / 90; 1000000 of 5 over 100 f32 76 / 56, 3001 of 515 over 997 f16 (one launch) 20.5 / 16.5
+    shape(D % wide == 0 ? wide : 1);
+    if (!one && D >= 32) shape(wide);
     const uint32_t *single = one ? didx : nullptr;
     // Rows no index names are cleared beside the sort, whose few workgroups leave the memory idle, where clearing takes longer
     // than telling the rows apart beforehand (two small launches; 16384 rows of 4096 over 65536: 334 us without, 270 with).
     const bool early = N > 0 && !accumulate && (uint64_t)K * D * bo > SINGLE_BYTES;
     SortArgs q{didx, nullptr, nullptr, at(p.keys[0]), at(p.rows[0]), at(p.hist), at(p.total), at(p.start), nullptr, (uint32_t)N, K, p.tiles, 0, p.bits, 0, {}};
-    ZeroArgs zero{(char *)dT, ldt * bo, (uint64_t)D * bo, wo >= 4, 0, 0};
-    while (((wo >= 4 ? 16ull : 2ull) << zero.log2g) < zero.bytes && zero.log2g < 8) ++zero.log2g;
+    const bool words = (((uint64_t)(uintptr_t)dT | ldt * bo | (uint64_t)D * bo) & 3) == 0;
+    ZeroArgs zero{(char *)dT, ldt * bo, (uint64_t)D * bo, words, 0, 0};
+    while (((words ? 16ull : 2ull) << zero.log2g) < zero.bytes && zero.log2g < 8) ++zero.log2g;
     // A row to a workgroup where rows are 2 KiB or more, and the next one from another: 1000 rows of 512 over 131072 54 us, by 4096
     // workgroups 65; short rows by 4096: 5000 of 64 over 1000000 68 us, by 65536 133.
     const uint64_t shares = zero.bytes >= 2048 ? std::min<uint64_t>((((uint64_t)K << zero.log2g) + 255) / 256, 65536) : std::min<uint64_t>((K + 15) / 16, 4096);
