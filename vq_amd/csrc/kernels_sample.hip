@@ -18,7 +18,7 @@
 // four times, all but the first from the caches.
 //
 // What bounds them: the vector units, not memory.  A weight in f64 is 23 instructions and there is no shorter exact way.  400000 x
-// 256 f32 with top_p 0.9: 236 us, 354 vector instructions a row, the units busy all the time (reading the scores once is 103 us
+// 256 f32 with top_p 0.9: 236 us, 356 vector instructions a row, the units busy all the time (reading the scores once is 103 us
 // at the rate of a large copy).  256 x 131072 bf16 with top_p 0.9: 100 us, of which the weights and their histogram are about
 // 40, the four passes over memory and caches the rest.  1 x 131072 bf16 with top_k 50 and top_p 0.9: 19 us, one workgroup's
 // latency.
