@@ -1,0 +1,64 @@
+"""vqhip_scores_device and vqhip_assign_sampled_device: the sizes and values where the expanded form of the matrix cores meets the direct
+one.  e = 2^-24, a rounding to f32; the bounds of the two forms are those derived in test_gpu_codes.py: (D + 3) e of the distance for the
+direct one, 8 (2 D + 6) e of it for the expanded one."""
+import numpy as np
+import pytest
+import torch
+
+from vq_amd import Context
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = Context(0)
+    yield c
+    c.close()
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def wide(t):
+    return t.detach().double().cpu().numpy()
+
+
+def exact(X, W):
+    return -torch.cdist(X.double(), W.double(), compute_mode="donot_use_mm_for_euclid_dist").square().numpy()
+
+
+# ---------------------------------------------------------------------------------------------- sizes of values
+@pytest.mark.parametrize("big", [2.0 ** 60, 1.2e19, 1.5e19, 1.8e19, 2.7e19, 3.6e19])
+@pytest.mark.parametrize("K,D", [(2, 40), (5, 40), (5, 100), (70, 33)])
+def test_scores_of_values_whose_squares_nearly_overflow(ctx, K, D, big):
+    """One prototype with one value near the root of the largest float: the norms around the mean, or only their sum, leave the range of
+    f32 where most distances do not.  Where the 64-bit distance is beyond f32 the score is -inf."""
+    g = gen(D)
+    W, X = torch.randn(K, D, generator=g), torch.randn(9, D, generator=g)
+    W[1, 7] = big
+    X[3], X[4] = W[0], W[1]
+    X[5, 7] = big
+    X[6, 7], X[7, 9] = -big, big
+    ctx.set_prototypes(W.numpy())
+    S, want = wide(ctx.scores(X.cuda())), exact(X, W)
+    far = -want > 3.5e38
+    near = -want < 3.3e38
+    assert (S[far] == -np.inf).all()
+    assert np.isfinite(S[near]).all() and (np.abs(S - want)[near] <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want)[near]).all()
+    assert S[3, 0] == 0.0 and S[4, 1] == 0.0
+
+
+@pytest.mark.parametrize("power", [-40, -50, -55, -58, -60, -62, -64, -66, -70])
+def test_scores_of_values_whose_squares_nearly_vanish(ctx, power):
+    """A value's square is below the least normal float from 2^-63 on: every product may lose half a subnormal step, 2^-150, on top of its
+    rounding; 4 products a value."""
+    g, D = gen(1), 40
+    W, X = torch.randn(70, D, generator=g), torch.randn(90, D, generator=g)
+    X[::7] = W[3]
+    W, X = torch.ldexp(W, torch.tensor(power)), torch.ldexp(X, torch.tensor(power))
+    ctx.set_prototypes(W.numpy())
+    S, want = wide(ctx.scores(X.cuda())), exact(X, W)
+    assert (np.abs(S - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want) + 4 * D * 2.0 ** -150).all()
+    assert (S[::7, 3] == 0).all()

@@ -230,6 +230,10 @@ constexpr uint32_t DIRECT_D = 16;               // k_scores_direct
 // their own prototype's way through the direct form too, 45 us more on 500k x 128 against 256.
 constexpr float CLOSE = 0.0625f;
 constexpr int MF_K = 16;
+// Norms above this become NaN, and with them every score made from them, so that such pairs are measured directly: the sum of two norms up
+// to here and the score itself (four times a norm at most) stay finite.  What is beyond f32 is decided by the direct form alone.
+constexpr float NORM_MOST = 0x1p125f;
+__device__ __forceinline__ float finite_norm(float x) { return x <= NORM_MOST ? x : NAN; }
 
 // The sum over 16 consecutive lanes, in the last of them
 __device__ __forceinline__ float row_sum(float v)
@@ -435,9 +439,9 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
         float x = sx[i];
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) x += __shfl_xor(x, o);
-        if ((t & 3) == 0) nx[sr + XROWS * i] = x;
+        if ((t & 3) == 0) nx[sr + XROWS * i] = finite_norm(x);
     }
-    for (int q = t; q < TN; q += THREADS) nw[q] = a.norms[col0 + q];
+    for (int q = t; q < TN; q += THREADS) nw[q] = finite_norm(a.norms[col0 + q]);
     __syncthreads();
 
     // scores, and this wave's list of close pairs (sample << 8 | prototype, inside its tile)
@@ -463,7 +467,7 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
                         const float both = fx2[e] + w2, s = fmaf(2.0f, acc[i][j][4 * g + e], -both);
                         float *const to = out + (size_t)(i * 32 + 8 * g + e) * a.ld + j * 32;
                         const bool on = !decltype(bounded)::value || (wrow + lr < a.N && wcol + lc < a.K);
-                        const bool far = s <= -CLOSE * both;                          // (not so where anything is not finite)
+                        const bool far = s <= -CLOSE * both;                          // (not so where a norm is NaN)
                         const uint64_t m = __ballot(!far);
                         if (m == 0) {
                             if (on) to[at] = s;
