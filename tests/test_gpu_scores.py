@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from vq_amd import Context
+from vq_amd import Context, _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,48 @@ def test_scores_of_values_whose_squares_nearly_vanish(ctx, power):
     S, want = wide(ctx.scores(X.cuda())), exact(X, W)
     assert (np.abs(S - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want) + 4 * D * 2.0 ** -150).all()
     assert (S[::7, 3] == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------- bits that depend on the pair alone
+def groups(N, K, D, crowd, seed):
+    """Samples and prototypes in `crowd` tight groups, sorted, so that whole tiles hold one group; every 29th sample stands alone."""
+    g = gen(seed)
+    centre = torch.randn(crowd, D, generator=g)
+    W = centre[torch.arange(K) * crowd // K] + 1e-3 * torch.randn(K, D, generator=g)
+    X = centre[torch.arange(N) * crowd // N] + 1e-3 * torch.randn(N, D, generator=g)
+    X[::29] = torch.randn(len(X[::29]), D, generator=g)
+    return X, W
+
+
+@pytest.mark.parametrize("D", [17, 20, 32, 48, 128, 200])
+@pytest.mark.parametrize("K,crowd", [(256, 2), (900, 3), (900, 40)])
+def test_a_score_depends_on_its_pair_alone(ctx, K, D, crowd):
+    """Tiles where all pairs are close, a part of them and none; other numbers of rows take other tiles, and begin them elsewhere."""
+    X, W = groups(9000, K, D, crowd, K + D)
+    X = X.cuda()
+    ctx.set_prototypes(W.numpy())
+    S = ctx.scores(X)
+    for a, b in ((0, 1), (8999, 9000), (29, 30), (40, 77), (100, 613), (4000, 8500), (0, 8999)):
+        assert torch.equal(ctx.scores(X[a:b].contiguous()), S[a:b]), (a, b)
+    want = exact(X.cpu(), W)
+    assert (np.abs(wide(S) - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("D", [20, 48])
+def test_assign_sampled_is_scores_and_sample_in_every_workspace(ctx, D):
+    """Chunks that are no multiple of a tile, shorter and longer than one, and a short last one."""
+    N, K = 5000, 900
+    X, W = groups(N, K, D, 3, D)
+    X, u = X.cuda(), torch.rand(N, generator=gen(D)).cuda()
+    ctx.set_prototypes(W.numpy())
+    L = _lib.lib()
+    for how in (dict(temperature=1e-6), dict(temperature=1.0, top_p=0.9)):
+        idx, prob = ctx.sample(ctx.scores(X), u, **how)
+        a, b = ctx.assign_sampled(X, u, **how)
+        assert torch.equal(a, idx) and torch.equal(b, prob)
+        for rows in (7, 100, 513, 1000, 4999):
+            work, i, p = torch.empty(rows * K, device="cuda"), torch.empty_like(idx), torch.empty_like(prob)
+            call = _lib.Sampling(how["temperature"], how.get("top_p", 1.0), 0.0, 0, None, None, None, None)
+            rc = L.vqhip_assign_sampled_device(ctx._h, X.data_ptr(), N, call, u.data_ptr(), i.data_ptr(), p.data_ptr(), work.data_ptr(), rows * K * 4,
+                                               torch.cuda.current_stream().cuda_stream)
+            assert rc == 0 and torch.equal(i, idx) and torch.equal(p, prob), (how, rows)

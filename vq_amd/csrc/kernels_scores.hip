@@ -9,7 +9,9 @@
 //     |x - w|^2 = |x - c|^2 + |w - c|^2 - 2 (x - c).(w - c)
 // with c the mean prototype, so that an offset all values share (pixels) does not cost digits.  Its rounding errors are those
 // of the two norms, so the pairs whose distance is small beside them (below CLOSE of their sum: a sample and the few
-// prototypes next to it) are measured again in the direct form: by 16 lanes a pair, or as a whole tile where they are many.
+// prototypes next to it) are measured again in the direct form, by 4 lanes a pair, or a square of pairs where they are many.  Which
+// form a pair takes and the order of its sums depend on the pair alone, not on the tile or the pairs beside it: a score has the same
+// bits whatever other rows a call has.  500000 x 128 against 256, us: samples with a close prototype each 369, half of all pairs close 1240.
 //
 // What bounds them: the matrix cores where rows are long (20011 x 784 against 1000 178 us, 1060 TFLOP/s over the six products; a
 // library's bf16 product reaches 1195 here), staging, products and the stores of a tile in turn where they are short (500000 x 128 against
@@ -235,15 +237,19 @@ constexpr int MF_K = 16;
 constexpr float NORM_MOST = 0x1p125f;
 __device__ __forceinline__ float finite_norm(float x) { return x <= NORM_MOST ? x : NAN; }
 
-// The sum over 16 consecutive lanes, in the last of them
-__device__ __forceinline__ float row_sum(float v)
+// The sum over 4 consecutive lanes, in all of them
+__device__ __forceinline__ float quad_sum(float v)
 {
-    auto up = [](float x, auto ctrl) { return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, false)); };
-    v += up(v, std::integral_constant<int, 0x111>());
-    v += up(v, std::integral_constant<int, 0x112>());
-    v += up(v, std::integral_constant<int, 0x114>());
-    v += up(v, std::integral_constant<int, 0x118>());
-    return v;
+    auto other = [](float x, auto ctrl) { return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+    v += other(v, std::integral_constant<int, 0xB1>());              // lane ^ 1
+    return v + other(v, std::integral_constant<int, 0x4E>());        // lane ^ 2
+}
+// Four more squares of a pair that is measured directly.  What such a pair's score is does not depend on the pairs beside it: lane l of
+// 4 takes the values 4 l .. 4 l + 3 of every 16 in their order, quad_sum joins the 4 sums.
+__device__ __forceinline__ void add_squares(float &s, const float4 &x, const float4 &w)
+{
+    const float e0 = x.x - w.x, e1 = x.y - w.y, e2 = x.z - w.z, e3 = x.w - w.w;
+    s = fmaf(e0, e0, fmaf(e1, e1, fmaf(e2, e2, fmaf(e3, e3, s))));
 }
 
 // The prototypes as the matrix cores read them, made once per model: per step of 16 reduction values and block of 64 prototypes
@@ -288,7 +294,7 @@ __global__ void __launch_bounds__(64) k_scores_norms(const float *W, const float
 // holds sample l & 31, B operand: prototype l & 31; lanes 0-31 the reduction values 0 .. 7 of a step, lanes 32-63 8 .. 15.
 // Result: lane l holds prototype l & 31 and samples 8 g + 4 (l >> 5) + e.  The samples are centred and split on their way to LDS;
 // both operands are double buffered there.
-constexpr uint32_t CLOSE_LIST = 512;                   // close pairs a wave measures one by one at most; more: its whole tile
+constexpr uint32_t CLOSE_LIST = 512;                   // close pairs a wave measures one by one at most; more: squares of its tile
 
 template <int RW, int CW, int WR, int WC, int PER_SIMD>
 __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const ScoreArgs a)
@@ -444,11 +450,13 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
     for (int q = t; q < TN; q += THREADS) nw[q] = finite_norm(a.norms[col0 + q]);
     __syncthreads();
 
-    // scores, and this wave's list of close pairs (sample << 8 | prototype, inside its tile)
-    uint16_t *list = lists[wave];
+    // scores, and a bit for each of this wave's close pairs, 32 prototypes a word, where the samples were staged
+    static_assert(TM * TN / 32 <= 2 * XSTAGE, "a bit for every pair of the tile");
+    uint32_t *close = &lx[0][0] + wave * MT * CW;
+    for (int q = lane; q < MT * CW; q += 64) close[q] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const uint64_t wrow = row0 + wr * MT;
     const uint32_t wcol = col0 + wc * NT;
-    uint32_t n = 0;
     auto finish = [&](auto bounded) {
         float *const out = a.S + wrow * a.ld + wcol;
         const size_t at = 4 * half * a.ld + l31;
@@ -474,9 +482,7 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
                         } else {
                             if (on && far) to[at] = s;
                             const uint64_t c = __ballot(on && !far);
-                            const uint32_t q = n + __popcll(c & ((1ull << lane) - 1));
-                            if (on && !far && q < CLOSE_LIST) list[q] = (uint16_t)(lr << 8 | lc);
-                            n += __popcll(c);
+                            if (l31 == 0) close[lr * CW + j] = (uint32_t)(half ? c >> 32 : c);
                         }
                     }
                 }
@@ -486,78 +492,93 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
         finish(std::false_type());
     else
         finish(std::true_type());
-    if (n == 0) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    constexpr int WORDS = (MT * CW + 63) / 64;             // a lane's
+    uint32_t word[WORDS], own = 0;
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) {
+        word[k] = lane + 64 * k < MT * CW ? close[lane + 64 * k] : 0;
+        own += __popc(word[k]);
+    }
+    if (__ballot(own != 0) == 0) return;
+    uint32_t upto = own;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(upto, o);
+        if (lane >= o) upto += v;
+    }
+    const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
     if (n <= MT * NT / 32) {
+        // a list of them: sample << 8 | prototype, inside this wave's tile
         static_assert(MT * NT / 32 <= (int)CLOSE_LIST, "the pairs measured one by one are all in the list");
-        // 16 lanes a pair, two pairs at a time
-        const uint32_t g = lane >> 4, gl = lane & 15;
-        for (uint32_t p = g; p < n; p += 8) {
-            const bool two = p + 4 < n;
-            const uint32_t q0 = list[p], q1 = list[two ? p + 4 : p];
-            const float *x0 = a.X + (wrow + (q0 >> 8)) * a.D, *w0 = a.W + (uint64_t)(wcol + (q0 & 255)) * a.D;
-            const float *x1 = a.X + (wrow + (q1 >> 8)) * a.D, *w1 = a.W + (uint64_t)(wcol + (q1 & 255)) * a.D;
-            float s0 = 0.0f, s1 = 0.0f;
-            for (uint32_t d = gl * 4; d < a.D; d += 128) {
-                // (both halves of 128 values on their way at once; what lies behind the row is 0 - 0)
+        uint16_t *list = lists[wave];
+        uint32_t to = upto - own;
+#pragma unroll
+        for (int k = 0; k < WORDS; ++k)
+            for (uint32_t left = word[k]; left; left &= left - 1)
+                list[to++] = (uint16_t)((lane + 64 * k) / CW << 8 | ((lane + 64 * k) % CW * 32 + __ffs(left) - 1));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // 4 lanes a pair
+        const uint32_t gl = lane & 3;
+        for (uint32_t p = lane >> 2; p < n; p += 16) {
+            const uint32_t q = list[p];
+            const float *x = a.X + (wrow + (q >> 8)) * a.D, *w = a.W + (uint64_t)(wcol + (q & 255)) * a.D;
+            float s = 0.0f;
+            for (uint32_t d = gl * 4; d < a.D; d += 64) {
+                // (64 values on their way at once; what lies behind the row is 0 - 0)
                 float4 u[4], v[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    u[h] = load4(x0, 0, true, a.D, d + 64 * h);
-                    v[h] = load4(w0, 0, true, a.D, d + 64 * h);
-                    u[2 + h] = load4(x1, 0, true, a.D, d + 64 * h);
-                    v[2 + h] = load4(w1, 0, true, a.D, d + 64 * h);
+                for (int h = 0; h < 4; ++h) {
+                    u[h] = load4(x, 0, true, a.D, d + 16 * h);
+                    v[h] = load4(w, 0, true, a.D, d + 16 * h);
                 }
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const float e0 = u[h].x - v[h].x, e1 = u[h].y - v[h].y, e2 = u[h].z - v[h].z, e3 = u[h].w - v[h].w;
-                    float &s = h < 2 ? s0 : s1;
-                    s = fmaf(e0, e0, fmaf(e1, e1, fmaf(e2, e2, fmaf(e3, e3, s))));
-                }
+                for (int h = 0; h < 4; ++h) add_squares(s, u[h], v[h]);
             }
-            s0 = row_sum(s0);
-            s1 = row_sum(s1);
-            if (gl == 15) {
-                a.S[(wrow + (q0 >> 8)) * a.ld + wcol + (q0 & 255)] = -s0;
-                if (two) a.S[(wrow + (q1 >> 8)) * a.ld + wcol + (q1 & 255)] = -s1;
-            }
+            s = quad_sum(s);
+            if (gl == 0) a.S[(wrow + (q >> 8)) * a.ld + wcol + (q & 255)] = -s;
         }
         return;
     }
-    // the wave's whole tile, a square of it at a time, Q x Q scores a lane
-    __threadfence();                                   // (its scores so far are written, before other lanes write some of them again)
-    constexpr int Q = 4 * RW;
-    const int ty = lane >> 3, tx = lane & 7;
+    // many: Q x Q pairs per 4 lanes, squares of the tile without a close one left out; a lane's sums are those of a pair measured alone
+    constexpr int Q = 4 * RW, ACROSS = NT / Q;
+    static_assert(32 % Q == 0, "a square's bits lie in one word a row");
+    const uint32_t gl = lane & 3;
 #pragma unroll 1
-    for (uint32_t c0 = 0; c0 < NT; c0 += MT) {
+    for (uint32_t b = lane >> 2; b < MT / Q * ACROSS; b += 16) {
+        const uint32_t r0 = b / ACROSS * Q, c0 = b % ACROSS * Q;
+        uint64_t pairs = 0;                                // bit i Q + j: sample r0 + i, prototype c0 + j
+#pragma unroll
+        for (int i = 0; i < Q; ++i) pairs |= (uint64_t)(close[(r0 + i) * CW + c0 / 32] >> (c0 % 32) & ((1u << Q) - 1)) << (i * Q);
+        if (pairs == 0) continue;
         float sum[Q][Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i)
 #pragma unroll
             for (int j = 0; j < Q; ++j) sum[i][j] = 0.0f;
-        for (uint32_t d = 0; d < a.D; d += 4) {
+        for (uint32_t d = gl * 4; d < a.D; d += 16) {
             float4 x[Q], w[Q];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
-                x[i] = load4(a.X, wrow + ty + 8 * i, wrow + ty + 8 * i < a.N, a.D, d);
-                w[i] = load4(a.W, wcol + c0 + tx + 8 * i, wcol + c0 + tx + 8 * i < a.K, a.D, d);
+                x[i] = load4(a.X, wrow + r0 + i, wrow + r0 + i < a.N, a.D, d);
+                w[i] = load4(a.W, wcol + c0 + i, wcol + c0 + i < a.K, a.D, d);
             }
 #pragma unroll
             for (int i = 0; i < Q; ++i)
 #pragma unroll
-                for (int j = 0; j < Q; ++j) {
-                    const float e0 = x[i].x - w[j].x, e1 = x[i].y - w[j].y, e2 = x[i].z - w[j].z, e3 = x[i].w - w[j].w;
-                    sum[i][j] = fmaf(e3, e3, fmaf(e2, e2, fmaf(e1, e1, fmaf(e0, e0, sum[i][j]))));
-                }
+                for (int j = 0; j < Q; ++j) add_squares(sum[i][j], x[i], w[j]);
         }
+        // lane l of the 4 stores the pairs l, l + 4, ...
 #pragma unroll
-        for (int i = 0; i < Q; ++i)
+        for (int p = 0; p < Q * Q; p += 4) {
+            float mine = 0.0f;
 #pragma unroll
-            for (int j = 0; j < Q; ++j) {
-                const uint64_t r = wrow + ty + 8 * i;
-                const uint32_t c = wcol + c0 + tx + 8 * j;
-                if (r < a.N && c < a.K) a.S[r * a.ld + c] = -sum[i][j];
+            for (int e = 0; e < 4; ++e) {
+                const float s = quad_sum(sum[(p + e) / Q][(p + e) % Q]);
+                mine = gl == (uint32_t)e ? s : mine;
             }
+            const uint32_t j = p % Q + gl;
+            if (pairs >> (p + gl) & 1) a.S[(wrow + r0 + p / Q) * a.ld + wcol + c0 + j] = -mine;
+        }
     }
 }
 
