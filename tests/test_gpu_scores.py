@@ -1,6 +1,8 @@
 """vqhip_scores_device and vqhip_assign_sampled_device: the sizes and values where the expanded form of the matrix cores meets the direct
 one.  e = 2^-24, a rounding to f32; the bounds of the two forms are those derived in test_gpu_codes.py: (D + 3) e of the distance for the
 direct one, 8 (2 D + 6) e of it for the expanded one."""
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -107,3 +109,32 @@ def test_assign_sampled_is_scores_and_sample_in_every_workspace(ctx, D):
             rc = L.vqhip_assign_sampled_device(ctx._h, X.data_ptr(), N, call, u.data_ptr(), i.data_ptr(), p.data_ptr(), work.data_ptr(), rows * K * 4,
                                                torch.cuda.current_stream().cuda_stream)
             assert rc == 0 and torch.equal(i, idx) and torch.equal(p, prob), (how, rows)
+
+
+# ---------------------------------------------------------------------------------------------- models
+def test_scores_follow_the_model(ctx):
+    """A model after another, of other sizes, larger and smaller, with few prototypes and many."""
+    g = gen(5)
+    for K, D in ((70, 40), (70, 40), (300, 100), (3, 4), (9, 33), (2000, 17), (2000, 16), (64, 64)):
+        W, X = torch.randn(K, D, generator=g) * 3 + 1, torch.randn(100, D, generator=g)
+        ctx.set_prototypes(W.numpy())
+        want = exact(X, W)
+        assert (np.abs(wide(ctx.scores(X.cuda())) - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want)).all()
+
+
+def test_a_model_costs_a_copy_until_scores_are_asked_for(ctx):
+    """Setting prototypes keeps them on the host and brings them to the GPU; what only scores need (their mean, their layout) is made by the
+    first scores call.  Four times a copy on each side, at the best of several, leaves room for everything but a pass of arithmetic over them."""
+    W = np.random.default_rng(0).random((131072, 64), np.float32)
+
+    def best(f):
+        t = []
+        for _ in range(7):
+            torch.cuda.synchronize()
+            at = time.perf_counter()
+            f()
+            torch.cuda.synchronize()
+            t.append(time.perf_counter() - at)
+        return min(t)
+
+    assert best(lambda: ctx.set_prototypes(W)) <= 4 * best(lambda: torch.from_numpy(W.copy()).cuda())

@@ -75,7 +75,7 @@ struct vqhip_ctx {
     std::vector<float> hW, hOm;
     std::vector<uint32_t> hcls;
 
-    float *dW = nullptr;       // K x D, and one row more: their mean
+    float *dW = nullptr;       // K x D
     void *dScoreImg = nullptr; // the prototypes laid out for vqhip_scores_device (rows above 16 values), made by its first call
     double *dW64 = nullptr;    // K x D in the reference's own number type (f64 entry points only)
     uint32_t *dcls = nullptr;  // K
@@ -926,16 +926,7 @@ try {
     c->hW.assign(W, W + (size_t)K * D);
     c->K = K;
     c->D = D;
-    // their mean behind them: what vqhip_scores_device measures from (0 where it is not finite)
-    std::vector<double> sum(D, 0.0);
-    for (uint32_t k = 0; k < K; ++k)
-        for (uint32_t d = 0; d < D; ++d) sum[d] += (double)W[(size_t)k * D + d];
-    std::vector<float> all(c->hW);
-    for (uint32_t d = 0; d < D; ++d) {
-        const float mean = (float)(sum[d] / K);
-        all.push_back(std::isfinite(mean) ? mean : 0.0f);
-    }
-    return upload(c, &c->dW, all.data(), all.size());
+    return upload(c, &c->dW, W, (size_t)K * D);
 }
 VQHIP_CATCH(c)
 
@@ -1332,7 +1323,7 @@ int prepare_scores(vqhip_ctx *c, hipStream_t s)
         return c->fail(VQHIP_ERR_STATE, "scores: call once after vqhip_set_prototypes and before the capture");
     void *img = nullptr;
     HIPCHK(c, hipMalloc(&img, bytes));
-    hipError_t e = launch_scores_image(c->dW, c->dW + (size_t)c->K * c->D, c->K, c->D, img, s);
+    hipError_t e = launch_scores_image(c->dW, c->K, c->D, img, s);
     if (e == hipSuccess) e = hipStreamSynchronize(s);
     if (e != hipSuccess) {
         (void)hipFree(img);
@@ -1358,7 +1349,7 @@ try {
     OnDevice on(c->device);
     HIPCHK(c, on.error());
     if ((rc = prepare_scores(c, (hipStream_t)stream)) != VQHIP_OK) return rc;
-    HIPCHK(c, launch_scores(dX, N, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->dScoreImg, c->K, dS, lds, (hipStream_t)stream));
+    HIPCHK(c, launch_scores(dX, N, c->D, c->dW, c->dScoreImg, c->K, dS, lds, (hipStream_t)stream));
     return VQHIP_OK;
 }
 VQHIP_CATCH(c)
@@ -1418,7 +1409,7 @@ try {
         if (h.dtop_p) h.dtop_p += off;
         if (h.dmin_p) h.dmin_p += off;
         if (h.dtop_k) h.dtop_k += off;
-        HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->dW + (size_t)c->K * c->D, c->dScoreImg, c->K, (float *)dwork, c->K, s));
+        HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->dScoreImg, c->K, (float *)dwork, c->K, s));
         HIPCHK(c, launch_sample(dwork, VQHIP_F32, n, c->K, c->K, h, du + off, didx_out + off, dprob_out ? dprob_out + off : nullptr, s));
     }
     return VQHIP_OK;

@@ -32,11 +32,11 @@ constexpr int SC_THREADS = 256, SC_K = 16;
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
 struct ScoreArgs {
-    const float *X, *W, *C;           // C: the mean prototype, D values
+    const float *X, *W, *C;           // C: the mean prototype, D values (any would do for the result; near the mean they keep its digits)
     float *S;
     uint64_t N, ld;
     uint32_t K, D;
-    const uint32_t *img;              // k_scores_image: the prototypes' pieces, then their norms
+    const uint32_t *img;              // k_scores_image: the prototypes' pieces; behind them their norms and their mean
     const float *norms;
     uint32_t blocks;                  // of 64 prototypes
     uint32_t colTiles;
@@ -261,6 +261,23 @@ constexpr uint32_t IMG_PAD = 256;                      // prototypes the image i
 
 __device__ __forceinline__ int piece_slot(int row, int quad) { return (((quad >> 1) ^ (row >> 3)) & 1) * 4 + (quad & 1) * 2; }
 inline uint32_t image_blocks(uint32_t K) { return (uint32_t)(((uint64_t)K + IMG_PAD - 1) / IMG_PAD * (IMG_PAD / 64)); }
+
+// The mean prototype, 16 values a workgroup, rows dealt to its 64 groups of 16 lanes; 0 where it is not finite
+__global__ void __launch_bounds__(1024) k_scores_mean(const float *W, uint32_t K, uint32_t D, float *C)
+{
+    __shared__ double part[64][16];
+    const uint32_t v = threadIdx.x & 15, g = threadIdx.x >> 4, d = blockIdx.x * 16 + v;
+    double s = 0.0;
+    if (d < D)
+#pragma unroll 8
+        for (uint64_t k = g; k < K; k += 64) s += (double)W[k * D + d];
+    part[g][v] = s;
+    __syncthreads();
+    if (g != 0 || d >= D) return;
+    for (int q = 1; q < 64; ++q) s += part[q][v];
+    const float mean = (float)(s / K);
+    C[d] = fabsf(mean) < INFINITY ? mean : 0.0f;
+}
 
 __global__ void __launch_bounds__(256) k_scores_image(const float *W, const float *C, uint32_t K, uint32_t D, uint32_t blocks, uint32_t *img)
 {
@@ -626,29 +643,37 @@ bool is_few(uint32_t K, uint32_t D) { return K <= FEW_K && D <= FEW_D && K * K *
 
 }  // namespace
 
-size_t scores_image_bytes(uint32_t K, uint32_t D)
-{
-    if (D <= DIRECT_D || is_few(K, D)) return 0;
-    const size_t blocks = image_blocks(K), steps = (D + MF_K - 1) / MF_K;
-    return steps * blocks * IMG_BLOCK * 4 + blocks * 64 * 4;
-}
+// The layout's parts: pieces, norms, mean
+struct ScoresImage {
+    uint32_t blocks, steps;
+    size_t norms, mean, bytes;
+    ScoresImage(uint32_t K, uint32_t D) : blocks(image_blocks(K)), steps((uint32_t)(((uint64_t)D + MF_K - 1) / MF_K))
+    {
+        norms = (size_t)steps * blocks * IMG_BLOCK * 4;
+        mean = norms + (size_t)blocks * 64 * 4;
+        bytes = mean + (size_t)D * 4;
+    }
+};
 
-hipError_t launch_scores_image(const float *dW, const float *dC, uint32_t K, uint32_t D, void *dImg, hipStream_t s)
+size_t scores_image_bytes(uint32_t K, uint32_t D) { return D <= DIRECT_D || is_few(K, D) ? 0 : ScoresImage(K, D).bytes; }
+
+hipError_t launch_scores_image(const float *dW, uint32_t K, uint32_t D, void *dImg, hipStream_t s)
 {
-    const uint32_t blocks = image_blocks(K), steps = (D + MF_K - 1) / MF_K;
-    hipLaunchKernelGGL(k_scores_image, dim3((uint32_t)((size_t)blocks * steps)), dim3(256), 0, s, dW, dC, K, D, blocks, (uint32_t *)dImg);
-    const hipError_t e = hipGetLastError();
+    const ScoresImage image(K, D);
+    float *const mean = (float *)((char *)dImg + image.mean);
+    hipLaunchKernelGGL(k_scores_mean, dim3((D + 15) / 16), dim3(1024), 0, s, dW, K, D, mean);
+    hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_scores_norms, dim3(blocks * 64), dim3(64), 0, s, dW, dC, K, D, (float *)((uint32_t *)dImg + (size_t)steps * blocks * IMG_BLOCK));
+    hipLaunchKernelGGL(k_scores_image, dim3((uint32_t)((size_t)image.blocks * image.steps)), dim3(256), 0, s, dW, mean, K, D, image.blocks, (uint32_t *)dImg);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL(k_scores_norms, dim3(image.blocks * 64), dim3(64), 0, s, dW, mean, K, D, (float *)((char *)dImg + image.norms));
     return hipGetLastError();
 }
 
-hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const float *dC, const void *dImg, uint32_t K, float *dS, uint64_t ld,
-                         hipStream_t s)
+hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const void *dImg, uint32_t K, float *dS, uint64_t ld, hipStream_t s)
 {
-    ScoreArgs a{dX, dW, dC, dS, N, ld, K, D, nullptr, nullptr, image_blocks(K), 0};
-    a.img = (const uint32_t *)dImg;
-    a.norms = (const float *)(a.img + (size_t)((D + MF_K - 1) / MF_K) * a.blocks * IMG_BLOCK);
+    const ScoresImage image(K, D);
+    ScoreArgs a{dX, dW, (const float *)((const char *)dImg + image.mean), dS, N, ld, K, D, (const uint32_t *)dImg, (const float *)((const char *)dImg + image.norms), image.blocks, 0};
     if (is_few(K, D)) {
         const uint64_t most = (1ull << 30) * SC_THREADS;
         for (uint64_t off = 0; off < N; off += most) {

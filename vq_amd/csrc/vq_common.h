@@ -120,12 +120,11 @@ hipError_t launch_glvq_gradient(const float *dX, uint64_t N, uint32_t D, uint32_
                                 unsigned long long *dused, hipStream_t s);
 
 // ---------------------------------------------------------------- sampled codes and codebook lookup
-// kernels_scores.hip: S[i][j] = - sum_d (X[i][d] - W[j][d])^2, rows of S `ld` apart; dC: the mean of W's rows (any D values do
-// for the result, near the mean they keep its digits).  dImg: launch_scores_image's layout of W, scores_image_bytes (0: none is
-// needed)
+// kernels_scores.hip: S[i][j] = - sum_d (X[i][d] - W[j][d])^2, rows of S `ld` apart.  dImg: launch_scores_image's layout of W,
+// scores_image_bytes (0: none is needed)
 size_t scores_image_bytes(uint32_t K, uint32_t D);
-hipError_t launch_scores_image(const float *dW, const float *dC, uint32_t K, uint32_t D, void *dImg, hipStream_t s);
-hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const float *dC, const void *dImg, uint32_t K, float *dS, uint64_t ld, hipStream_t s);
+hipError_t launch_scores_image(const float *dW, uint32_t K, uint32_t D, void *dImg, hipStream_t s);
+hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const void *dImg, uint32_t K, float *dS, uint64_t ld, hipStream_t s);
 // kernels_sample.hip: one index per row of scores (include/vqhip.h vqhip_sample_device); dprob nullable
 hipError_t launch_sample(const void *dS, int dtype, uint64_t N, uint32_t V, uint64_t ld, const vqhip_sampling &how, const float *du,
                          uint32_t *didx, float *dprob, hipStream_t s);
