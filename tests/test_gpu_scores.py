@@ -138,3 +138,39 @@ def test_a_model_costs_a_copy_until_scores_are_asked_for(ctx):
         return min(t)
 
     assert best(lambda: ctx.set_prototypes(W)) <= 4 * best(lambda: torch.from_numpy(W.copy()).cuda())
+
+
+# ---------------------------------------------------------------------------------------------- more than a launch holds
+def test_scores_of_more_samples_than_a_grid_has_lanes(ctx):
+    """2^32 samples and 300 more, a lane each: 34 GB of samples and scores."""
+    N = (1 << 32) + 300
+    X = torch.zeros(N, 1, device="cuda")
+    at = [0, 1 << 30, (1 << 32) - 1, 1 << 32, (1 << 32) + 255, (1 << 32) + 256, N - 1]
+    for n, i in enumerate(at):
+        X[i] = n + 1.0
+    ctx.set_prototypes(np.array([[-2.0]], np.float32))
+    S = ctx.scores(X, out=torch.zeros(N, 1, device="cuda"))
+    assert [S[i].item() for i in at] == [-(n + 3.0) ** 2 for n in range(len(at))]
+    assert sum((part == -4.0).sum().item() for part in S.split(1 << 28)) == N - len(at)
+    del X, S
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("K,D,N", [((1 << 28) + 70, 1, 3), ((1 << 26) + 5, 17, 2)])
+def test_scores_against_very_many_prototypes(ctx, K, D, N):
+    """Direct tiles of 64 prototypes beyond 2^22, and a layout whose prototypes are more than a grid has waves."""
+    W = np.zeros((K, D), np.float32)
+    at = [0, 1, 63, 64, 1 << 26, (1 << 26) + 4, K - 71, K - 70, K - 2, K - 1]
+    for n, k in enumerate(at):
+        W[k, n % D] = n + 2.0
+    ctx.set_prototypes(W)
+    X = torch.zeros(N, D)
+    X[1] = 1.0
+    S = ctx.scores(X.cuda())
+    got = S[:, at].cpu()
+    want = exact(X, torch.from_numpy(W[at]))
+    assert (np.abs(wide(got) - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want)).all()
+    assert (S[0] == 0).sum().item() == K - len(set(at)) and ((S[1] + D).abs() <= 1e-4 * D).sum().item() >= K - len(set(at))
+    del S
+    ctx.set_prototypes(W[:3])                                               # (the large layout is not kept)
+    torch.cuda.empty_cache()

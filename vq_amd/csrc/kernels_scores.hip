@@ -27,6 +27,8 @@ namespace vq {
 namespace {
 
 constexpr int SC_THREADS = 256, SC_K = 16;
+// Workgroups of a launch: a grid holds fewer than 2^32 lanes, larger problems are several launches (or steps of a loop)
+constexpr uint32_t GRID = 1u << 22;
 
 // Four floats in one access of 16 bytes, which has to begin at a multiple of 4 only
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -266,45 +268,53 @@ inline uint32_t image_blocks(uint32_t K) { return (uint32_t)(((uint64_t)K + IMG_
 __global__ void __launch_bounds__(1024) k_scores_mean(const float *W, uint32_t K, uint32_t D, float *C)
 {
     __shared__ double part[64][16];
-    const uint32_t v = threadIdx.x & 15, g = threadIdx.x >> 4, d = blockIdx.x * 16 + v;
-    double s = 0.0;
-    if (d < D)
+    const uint32_t v = threadIdx.x & 15, g = threadIdx.x >> 4;
+    for (uint64_t base = (uint64_t)blockIdx.x * 16; base < D; base += (uint64_t)gridDim.x * 16) {
+        const uint64_t d = base + v;
+        double s = 0.0;
+        if (d < D)
 #pragma unroll 8
-        for (uint64_t k = g; k < K; k += 64) s += (double)W[k * D + d];
-    part[g][v] = s;
-    __syncthreads();
-    if (g != 0 || d >= D) return;
-    for (int q = 1; q < 64; ++q) s += part[q][v];
-    const float mean = (float)(s / K);
-    C[d] = fabsf(mean) < INFINITY ? mean : 0.0f;
+            for (uint64_t k = g; k < K; k += 64) s += (double)W[k * D + d];
+        part[g][v] = s;
+        __syncthreads();
+        if (g == 0 && d < D) {
+            for (int q = 1; q < 64; ++q) s += part[q][v];
+            const float mean = (float)(s / K);
+            C[d] = fabsf(mean) < INFINITY ? mean : 0.0f;
+        }
+        __syncthreads();
+    }
 }
 
-__global__ void __launch_bounds__(256) k_scores_image(const float *W, const float *C, uint32_t K, uint32_t D, uint32_t blocks, uint32_t *img)
+__global__ void __launch_bounds__(256) k_scores_image(const float *W, const float *C, uint32_t K, uint32_t D, uint32_t blocks, uint32_t steps, uint32_t *img)
 {
-    const uint32_t block = blockIdx.x % blocks, step = blockIdx.x / blocks;
     const int row = threadIdx.x >> 2, quad = threadIdx.x & 3;
-    const uint32_t k = block * 64 + row, d = step * MF_K + quad * 4;
-    const float4 w = load4(W, k, k < K, D, d), c = load4(C, 0, k < K, D, d);
-    uint32_t p[3], q[3];
-    split3(w.x - c.x, w.y - c.y, p[0], p[1], p[2]);
-    split3(w.z - c.z, w.w - c.w, q[0], q[1], q[2]);
-    uint32_t *to = img + ((size_t)step * blocks + block) * IMG_BLOCK + row * 8 + piece_slot(row, quad);
+    for (uint64_t at = blockIdx.x; at < (uint64_t)blocks * steps; at += gridDim.x) {         // at: step, then block
+        const uint64_t k = at % blocks * 64 + row;
+        const uint32_t d = (uint32_t)(at / blocks) * MF_K + quad * 4;
+        const float4 w = load4(W, k, k < K, D, d), c = load4(C, 0, k < K, D, d);
+        uint32_t p[3], q[3];
+        split3(w.x - c.x, w.y - c.y, p[0], p[1], p[2]);
+        split3(w.z - c.z, w.w - c.w, q[0], q[1], q[2]);
+        uint32_t *to = img + at * IMG_BLOCK + row * 8 + piece_slot(row, quad);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) *(uint2 *)(to + i * 64 * 8) = make_uint2(p[i], q[i]);
+        for (int i = 0; i < 3; ++i) *(uint2 *)(to + i * 64 * 8) = make_uint2(p[i], q[i]);
+    }
 }
 
 // |w - c|^2, a wave per prototype; 0 behind the last
-__global__ void __launch_bounds__(64) k_scores_norms(const float *W, const float *C, uint32_t K, uint32_t D, float *norms)
+__global__ void __launch_bounds__(64) k_scores_norms(const float *W, const float *C, uint32_t K, uint32_t D, uint64_t rows, float *norms)
 {
-    const uint32_t k = blockIdx.x;
-    float s = 0.0f;
-    if (k < K)
-        for (uint32_t d = threadIdx.x; d < D; d += 64) {
-            const float e = W[(size_t)k * D + d] - C[d];
-            s = fmaf(e, e, s);
-        }
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    if (threadIdx.x == 0) norms[k] = s;
+    for (uint64_t k = blockIdx.x; k < rows; k += gridDim.x) {
+        float s = 0.0f;
+        if (k < K)
+            for (uint32_t d = threadIdx.x; d < D; d += 64) {
+                const float e = W[k * D + d] - C[d];
+                s = fmaf(e, e, s);
+            }
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        if (threadIdx.x == 0) norms[k] = s;
+    }
 }
 
 // A workgroup of WR x WC waves, a wave 32 RW x 32 CW scores in RW x CW accumulators of v_mfma_f32_32x32x16_bf16.  A operand: lane l
@@ -599,44 +609,48 @@ __global__ void __launch_bounds__(WR * WC * 64, PER_SIMD) k_scores_mfma(const Sc
     }
 }
 
-template <int TX>
-hipError_t run_direct(ScoreArgs a, hipStream_t s)
+// launch(part, workgroups) for parts of the scores that a launch can hold, of whole tiles of TM samples and TN prototypes; colTiles is set
+template <uint32_t TM, uint32_t TN, class Launch>
+hipError_t in_parts(const ScoreArgs &all, Launch &&launch)
 {
-    constexpr uint32_t TM = SC_THREADS / TX * 8, TN = TX * 8;
-    a.colTiles = (a.K + TN - 1) / TN;
-    const uint64_t N = a.N, most = std::max<uint64_t>(1, (1u << 30) / a.colTiles) * TM;          // a grid holds fewer than 2^31 workgroups
-    const float *X = a.X;
-    float *S = a.S;
-    for (uint64_t off = 0; off < N; off += most) {
-        a.X = X + off * a.D;
-        a.S = S + off * a.ld;
-        a.N = std::min(N - off, most);
-        hipLaunchKernelGGL(k_scores_direct<TX>, dim3((uint32_t)((a.N + TM - 1) / TM * a.colTiles)), dim3(SC_THREADS), 0, s, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+    const uint64_t wide = (uint64_t)GRID * TN;
+    for (uint64_t col = 0; col < all.K; col += wide) {
+        ScoreArgs a = all;
+        a.K = (uint32_t)std::min<uint64_t>(all.K - col, wide);
+        a.colTiles = (uint32_t)(((uint64_t)a.K + TN - 1) / TN);
+        a.W = all.W + col * all.D;
+        a.img = all.img + col / 64 * IMG_BLOCK;
+        a.norms = all.norms + col;
+        const uint64_t most = (uint64_t)(GRID / a.colTiles) * TM;
+        for (uint64_t row = 0; row < all.N; row += most) {
+            a.X = all.X + row * all.D;
+            a.S = all.S + row * all.ld + col;
+            a.N = std::min(all.N - row, most);
+            const hipError_t e = launch(a, (uint32_t)((a.N + TM - 1) / TM * a.colTiles));
+            if (e != hipSuccess) return e;
+        }
     }
     return hipSuccess;
 }
 
+template <int TX>
+hipError_t run_direct(const ScoreArgs &all, hipStream_t s)
+{
+    return in_parts<SC_THREADS / TX * 8, TX * 8>(all, [&](const ScoreArgs &a, uint32_t tiles) {
+        hipLaunchKernelGGL(k_scores_direct<TX>, dim3(tiles), dim3(SC_THREADS), 0, s, a);
+        return hipGetLastError();
+    });
+}
+
 template <int RW, int CW, int WR, int WC, int PER_SIMD>
-hipError_t run_mfma(ScoreArgs a, hipStream_t s)
+hipError_t run_mfma(const ScoreArgs &all, hipStream_t s)
 {
     constexpr uint32_t TM = 32 * RW * WR, TN = 32 * CW * WC;
     static_assert(IMG_PAD % TN == 0, "the image covers every tile");
-    a.colTiles = (a.K + TN - 1) / TN;
-    const uint64_t N = a.N, most = std::max<uint64_t>(1, (1u << 30) / a.colTiles) * TM;          // a grid holds fewer than 2^31 workgroups
-    const float *X = a.X;
-    float *S = a.S;
-    for (uint64_t off = 0; off < N; off += most) {
-        a.X = X + off * a.D;
-        a.S = S + off * a.ld;
-        a.N = std::min(N - off, most);
-        const uint64_t tiles = (a.N + TM - 1) / TM * a.colTiles;
-        hipLaunchKernelGGL((k_scores_mfma<RW, CW, WR, WC, PER_SIMD>), dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(WR * WC * 64), 0, s, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    return in_parts<TM, TN>(all, [&](const ScoreArgs &a, uint32_t tiles) {
+        hipLaunchKernelGGL((k_scores_mfma<RW, CW, WR, WC, PER_SIMD>), dim3((tiles + 7) / 8 * 8), dim3(WR * WC * 64), 0, s, a);
+        return hipGetLastError();
+    });
 }
 
 bool is_few(uint32_t K, uint32_t D) { return K <= FEW_K && D <= FEW_D && K * K * D <= 4096; }
@@ -661,12 +675,13 @@ hipError_t launch_scores_image(const float *dW, uint32_t K, uint32_t D, void *dI
 {
     const ScoresImage image(K, D);
     float *const mean = (float *)((char *)dImg + image.mean);
-    hipLaunchKernelGGL(k_scores_mean, dim3((D + 15) / 16), dim3(1024), 0, s, dW, K, D, mean);
+    hipLaunchKernelGGL(k_scores_mean, dim3(std::min(D / 16 + 1, GRID / 4)), dim3(1024), 0, s, dW, K, D, mean);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_scores_image, dim3((uint32_t)((size_t)image.blocks * image.steps)), dim3(256), 0, s, dW, mean, K, D, image.blocks, (uint32_t *)dImg);
+    hipLaunchKernelGGL(k_scores_image, dim3((uint32_t)std::min<uint64_t>((uint64_t)image.blocks * image.steps, GRID)), dim3(256), 0, s, dW, mean, K, D, image.blocks, image.steps, (uint32_t *)dImg);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL(k_scores_norms, dim3(image.blocks * 64), dim3(64), 0, s, dW, mean, K, D, (float *)((char *)dImg + image.norms));
+    const uint64_t rows = (uint64_t)image.blocks * 64;
+    hipLaunchKernelGGL(k_scores_norms, dim3((uint32_t)std::min<uint64_t>(rows, GRID)), dim3(64), 0, s, dW, mean, K, D, rows, (float *)((char *)dImg + image.norms));
     return hipGetLastError();
 }
 
@@ -675,7 +690,7 @@ hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *d
     const ScoresImage image(K, D);
     ScoreArgs a{dX, dW, (const float *)((const char *)dImg + image.mean), dS, N, ld, K, D, (const uint32_t *)dImg, (const float *)((const char *)dImg + image.norms), image.blocks, 0};
     if (is_few(K, D)) {
-        const uint64_t most = (1ull << 30) * SC_THREADS;
+        const uint64_t most = (uint64_t)GRID * SC_THREADS;
         for (uint64_t off = 0; off < N; off += most) {
             a.X = dX + off * D;
             a.S = dS + off * ld;
@@ -698,7 +713,7 @@ hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *d
         // against 1000 (628) 209 / 203 / 278
         // Where prototypes would leave a large part of a wide tile empty, a narrower one is taken: what a tile of each kind costs per
         // column is 1 / 1.1 / 1.5.
-        const uint64_t rows = (N + 127) / 128, c256 = (K + 255) / 256, c128 = (K + 127) / 128, c64 = (K + 63) / 64;
+        const uint64_t rows = (N + 127) / 128, c64 = ((uint64_t)K + 63) / 64, c128 = (c64 + 1) / 2, c256 = (c64 + 3) / 4;
         const uint64_t wide = c256 * 40, middle = c128 * 22, slim = c64 * 15;
         if (rows * c256 >= 2048 && wide <= middle && wide <= slim) return run_mfma<2, 4, 2, 2, 2>(a, s);
         if (rows * c128 >= 512 && middle <= slim) return run_mfma<2, 2, 2, 2, 2>(a, s);
@@ -706,7 +721,7 @@ hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *d
     }
     // (the narrowest tile that pads the prototypes least)
     if (K <= 32) return run_direct<4>(a, s);
-    return (K + 63) / 64 % 2 ? run_direct<8>(a, s) : run_direct<16>(a, s);
+    return ((uint64_t)K + 63) / 64 % 2 ? run_direct<8>(a, s) : run_direct<16>(a, s);
 }
 
 }  // namespace vq
