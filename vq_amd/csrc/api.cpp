@@ -1368,7 +1368,7 @@ try {
     if (((uintptr_t)du | (uintptr_t)didx_out | (uintptr_t)dprob_out) & 3) return c->fail(VQHIP_ERR_INVALID, "sample_device: device pointers must be 4-byte aligned");
     OnDevice on(c->device);
     HIPCHK(c, on.error());
-    HIPCHK(c, launch_sample(dS, dtype, N, V, lds, *how, du, didx_out, dprob_out, (hipStream_t)stream));
+    HIPCHK(c, launch_sample(dS, dtype, N, V, lds, *how, du, didx_out, dprob_out, N, (hipStream_t)stream));
     return VQHIP_OK;
 }
 VQHIP_CATCH(c)
@@ -1410,7 +1410,7 @@ try {
         if (h.dmin_p) h.dmin_p += off;
         if (h.dtop_k) h.dtop_k += off;
         HIPCHK(c, launch_scores(dX + off * c->D, n, c->D, c->dW, c->dScoreImg, c->K, (float *)dwork, c->K, s));
-        HIPCHK(c, launch_sample(dwork, VQHIP_F32, n, c->K, c->K, h, du + off, didx_out + off, dprob_out ? dprob_out + off : nullptr, s));
+        HIPCHK(c, launch_sample(dwork, VQHIP_F32, n, c->K, c->K, h, du + off, didx_out + off, dprob_out ? dprob_out + off : nullptr, N, s));
     }
     return VQHIP_OK;
 }

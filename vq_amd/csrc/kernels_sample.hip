@@ -47,6 +47,9 @@ struct SampleArgs {
 };
 
 using u32x4s = uint32_t __attribute__((ext_vector_type(4)));
+// 16 bytes from any multiple of an element's size
+typedef uint32_t words_by4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t words_by2 __attribute__((ext_vector_type(4), aligned(2)));
 
 // ---------------------------------------------------------------------------------------------- keys, weights, wave sums
 constexpr uint32_t KEY_LEAST = 0x007FFFFFu;            // key of -inf: masked scores and NaN
@@ -921,8 +924,8 @@ struct Drawn {
 
 // One row, worked on by a workgroup: all members are called by all its lanes.  The row is dealt to the waves in consecutive
 // ranges, a range in steps of 64 PER scores, PER consecutive ones per lane: order of index = (wave, step, lane, place).  Rows
-// begin anywhere: positions count from the 16-byte boundary at or before the first score, so that all loads but those of a row's
-// two ends are aligned ones of 16 bytes; the positions in front of the row are masked scores that are not read.
+// begin anywhere, and are read 16 bytes at a time from there on: how a row is dealt, and with it the last bits of its sums, does not
+// depend on where it lies.
 template <class T, int THREADS>
 struct BlockRow {
     static constexpr int WAVES = THREADS / 64;
@@ -930,10 +933,10 @@ struct BlockRow {
     static constexpr uint32_t STEP = 64 * PER;
     using Piece = Pack<T, PER * (int)sizeof(T)>;
     using GlobalT = const __attribute__((address_space(1))) T;
-    using Global16 = const __attribute__((address_space(1))) u32x4s;
+    using Global16 = const __attribute__((address_space(1))) typename std::conditional<sizeof(T) == 4, words_by4, words_by2>::type;
 
-    uint64_t row;                       // address of position 0 in global memory
-    uint32_t first, V;                  // positions of the first score and behind the last
+    uint64_t row;                       // address of the first score in global memory
+    uint32_t V;
     int s;
     Weigh weigh;
 
@@ -942,7 +945,6 @@ struct BlockRow {
     {
         BlockRow b;
         b.row = same(row);
-        b.first = same(first);
         b.V = same(V);
         b.s = (int)same((uint32_t)s);
         b.weigh.top = same(weigh.top);
@@ -960,15 +962,15 @@ struct BlockRow {
         lo = (uint32_t)min(from, (uint64_t)end);
         hi = (uint32_t)min(from + len, (uint64_t)end);
     }
-    __device__ __forceinline__ Piece load_whole(uint32_t j) const { return __builtin_bit_cast(Piece, *(Global16 *)(row + (uint64_t)j * sizeof(T))); }
-    // This lane's scores of one step; what lies in front of the row or behind `hi` is a masked score.
+    __device__ __forceinline__ Piece load_whole(uint32_t j) const { return __builtin_bit_cast(Piece, (u32x4s)*(Global16 *)(row + (uint64_t)j * sizeof(T))); }
+    // This lane's scores of one step; what lies behind `hi` is a masked score.
     __device__ __forceinline__ Piece load(uint32_t base, uint32_t hi) const
     {
         const uint32_t j = base + lane() * PER;
-        if (j >= first && j + PER <= hi) return load_whole(j);
+        if (j + PER <= hi) return load_whole(j);
         Piece v;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) v.v[e] = j + e >= first && j + e < hi ? ((GlobalT *)row)[j + e] : (T)-INFINITY;
+        for (int e = 0; e < PER; ++e) v.v[e] = j + e < hi ? ((GlobalT *)row)[j + e] : (T)-INFINITY;
         return v;
     }
     // f(position of the first, scores) for this lane's scores of one step
@@ -996,10 +998,6 @@ struct BlockRow {
                 step_of(base, now, f);
             }
             return;
-        }
-        if (base < first && base < hi) {
-            step_of(base, load(base, hi), f);
-            base += STEP;
         }
 #pragma unroll 1
         for (; base < hi && hi - base >= FLIGHT * STEP; base += FLIGHT * STEP) {
@@ -1210,8 +1208,8 @@ __device__ __attribute__((noinline)) Drawn list_draw(const Row r, const RowParam
     WaveSet<E> set;
     row.load_list(set);
     double drawn, total;
-    const uint32_t q = set.draw(row.weigh.top, same(p.top_k), same(p.top_p), same(p.min_p), same(p.u), same(p.reach(row.V - row.first)), Row::shared().bins, drawn, total);
-    return {Row::shared().list_at[q] - row.first, (float)(drawn * inverse(total))};
+    const uint32_t q = set.draw(row.weigh.top, same(p.top_k), same(p.top_p), same(p.min_p), same(p.u), same(p.reach(row.V)), Row::shared().bins, drawn, total);
+    return {Row::shared().list_at[q], (float)(drawn * inverse(total))};
 }
 
 template <class Row, int E, bool MASS>
@@ -1493,7 +1491,7 @@ __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, ui
                 done = run > target;
             }
         }
-        d.at = (uint32_t)__builtin_amdgcn_readlane((int)(j + place), q) - row.first;
+        d.at = (uint32_t)__builtin_amdgcn_readlane((int)(j + place), q);
         d.prob = (float)(lane_of(drawn, q) * inverse(total));
     });
     return d;
@@ -1549,16 +1547,14 @@ __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
     using Row = BlockRow<T, THREADS>;
     auto &sh = Row::shared();
     for (uint64_t i = blockIdx.x; i < a.N; i += gridDim.x) {
-        const uint64_t address = (uint64_t)((const T *)a.S + i * a.ld);
-        const uint32_t first = (uint32_t)(address & 15) / (uint32_t)sizeof(T);
-        Row row{address & ~15ull, first, first + a.V, a.mass_bits, Weigh()};
+        Row row{(uint64_t)((const T *)a.S + i * a.ld), a.V, a.mass_bits, Weigh()};
         const RowParams p(a, i);
         Drawn d{0, 0.0f};
         float mine;
         const float top = row.find_top(mine);
         row.weigh = Weigh(top, p.temperature);
         if (top > -INFINITY && p.greedy) {
-            d = Drawn{nth_equal(row, top, 1) - first, 1.0f};
+            d = Drawn{nth_equal(row, top, 1), 1.0f};
         } else if (top > -INFINITY) {
             Cut c{-INFINITY, 0, 0, EVERY};
             bool done = false;
@@ -1626,7 +1622,7 @@ hipError_t run_block(const SampleArgs &a, hipStream_t s)
 }
 
 template <class T>
-hipError_t run_sample(const SampleArgs &a, hipStream_t s)
+hipError_t run_sample(const SampleArgs &a, uint64_t rows, hipStream_t s)
 {
     // Four lanes per row up to 64 scores: us for 400000 rows, f32, top_p 0.9 (with a wave per row): 10 scores 28 (216), 32 48
     // (230), 64 94 (237); with parameters per row 64 130 (387)
@@ -1643,22 +1639,22 @@ hipError_t run_sample(const SampleArgs &a, hipStream_t s)
     // 256 / 512 / 1024 lanes, top_p 0.9: 8192 x 4096 150 / - / 461; 256 x 16384 32 / 25 / 27, 1024 x 16384 59 / 64 / 100; 256 x 50000
     // 79 / 58 / 55, 512 x 50000 101 / 87 / 103; bf16 256 x 131072 187 / 118 / 105, 512 x 131072 224 / 225 / 193
     if (a.V <= 8192) return run_block<T, 256>(a, s);
-    if (a.V <= 32768 || (a.V <= 65536 && a.N > 256)) return run_block<T, 512>(a, s);
+    if (a.V <= 32768 || (a.V <= 65536 && rows > 256)) return run_block<T, 512>(a, s);
     return run_block<T, 1024>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_sample(const void *dS, int dtype, uint64_t N, uint32_t V, uint64_t ld, const vqhip_sampling &how, const float *du, uint32_t *didx,
-                         float *dprob, hipStream_t s)
+                         float *dprob, uint64_t rows, hipStream_t s)
 {
     int log2v = 0;
     while ((1ull << log2v) < V) ++log2v;
     const SampleArgs a{dS, N, ld, V, std::min(51, 62 - log2v), how.temperature, how.top_p, how.min_p, how.top_k, how.dtemperature, how.dtop_p, how.dmin_p,
                        how.dtop_k, du, didx, dprob};
-    if (dtype == VQHIP_F32) return run_sample<float>(a, s);
-    if (dtype == VQHIP_BF16) return run_sample<__bf16>(a, s);
-    return run_sample<_Float16>(a, s);
+    if (dtype == VQHIP_F32) return run_sample<float>(a, rows, s);
+    if (dtype == VQHIP_BF16) return run_sample<__bf16>(a, rows, s);
+    return run_sample<_Float16>(a, rows, s);
 }
 
 }  // namespace vq

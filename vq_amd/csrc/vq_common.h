@@ -125,9 +125,10 @@ hipError_t launch_glvq_gradient(const float *dX, uint64_t N, uint32_t D, uint32_
 size_t scores_image_bytes(uint32_t K, uint32_t D);
 hipError_t launch_scores_image(const float *dW, uint32_t K, uint32_t D, void *dImg, hipStream_t s);
 hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *dW, const void *dImg, uint32_t K, float *dS, uint64_t ld, hipStream_t s);
-// kernels_sample.hip: one index per row of scores (include/vqhip.h vqhip_sample_device); dprob nullable
+// kernels_sample.hip: one index per row of scores (include/vqhip.h vqhip_sample_device); dprob nullable.  rows: of the whole call, where
+// this is a part of one (what decides which kernel, and with it the last bits of a sum)
 hipError_t launch_sample(const void *dS, int dtype, uint64_t N, uint32_t V, uint64_t ld, const vqhip_sampling &how, const float *du,
-                         uint32_t *didx, float *dprob, hipStream_t s);
+                         uint32_t *didx, float *dprob, uint64_t rows, hipStream_t s);
 // kernels_lookup.hip: Y[i] = scale T[idx[i]]; and its gradient over indices put in order (workspace: lookup_gradient_workspace bytes)
 hipError_t launch_lookup(const void *dT, int dtype, uint64_t ldt, uint32_t K, uint32_t D, const uint32_t *didx, uint64_t N, float scale,
                          void *dY, uint64_t ldy, hipStream_t s);
