@@ -297,9 +297,9 @@ typedef struct {
  * sum over kept i <= j of w_i > u * (sum over all kept), prob = w_idx / (sum over all kept), 1 where T = 0.  dprob may be NULL.
  * NaN and -inf are never drawn; a row of nothing else gives index 0 with probability 0.  A row whose maximum is +inf draws among
  * its +inf.  V >= 1, below 2^31.  w and its sums are f64 (where a row is longer than 1024 scores, the sums that place the border of
- * top_p are integers, in units of 2^-51 up to 2048 scores and of V 2^-62 above): the index is that of the definition unless u
- * times the sum falls within ~1e-14 of a border, or top_p times it within ~1e-11 of one, relative.  The same inputs give the
- * same bits. */
+ * top_p are integers, in units small beside the weights they add: each sum is off by at most V 2^-61 of itself, T above 1e-36): the index is
+ * that of the definition unless u times the sum, or top_p times it, falls within ~1e-14 of a border, relative, or within V 2^-61 where
+ * that is more.  The same inputs give the same bits, wherever they lie. */
 int vqhip_sample_device(vqhip_ctx *ctx, const void *dS, int dtype, uint64_t N, uint32_t V, uint64_t lds, const vqhip_sampling *how,
                         const float *du, uint32_t *didx_out, float *dprob_out, void *stream);
 

@@ -9,8 +9,9 @@
 //
 // Numbers.  The index is an exact answer, so what decides it is computed in more than 32 bits: w in f64, sums in f64 in a fixed
 // order, and where masses are added by atomics (the histogram of k_sample_block) as integers, whose sums do not depend on
-// the order (w 2^s rounded, s chosen so that V of them fit 63 bits).  Two correct evaluations still part where u Z or top_p Z1
-// falls within ~1e-11 of a border.
+// the order: in units of 2^-s of the largest weight a step of the histogram can hold, s chosen so that V of them fit 63 bits.  (Of the
+// row's largest weight they would lose long tails: 2^22 scores of weight 2^-42 beside a 1 are 1e-6 of the row, each below half a unit.)
+// Two correct evaluations still part where u Z or top_p Z1 falls within ~1e-14 of a border, or V 2^-61 where that is more.
 //
 // Three kernels.  Up to 64 scores: k_sample_quad, four lanes per row.  Up to 1024: k_sample_wave, a wave per row.  Both hold the row in
 // registers and read it once.  Longer rows: k_sample_block, a workgroup per row, which first cuts the row down to the few
@@ -518,10 +519,9 @@ struct RowParams {
     }
     // How far below the maximum the border of a nucleus among V scores lies at most: all scores more than ln(V / (1 - p)) below
     // it (in units of T) together weigh less than 1 - p.
-    __device__ float reach(uint32_t V) const
-    {
-        return (__builtin_amdgcn_logf((float)V) - __builtin_amdgcn_logf(fmaxf(1.0f - top_p, 0x1p-24f)) + 1.5f) * 0.6932f * temperature;
-    }
+    __device__ float reach(uint32_t V) const { return octaves(V) * 0.6932f * temperature; }
+    // ... in powers of two of the weight, a little less (0.6932 > ln 2)
+    __device__ float octaves(uint32_t V) const { return __builtin_amdgcn_logf((float)V) - __builtin_amdgcn_logf(fmaxf(1.0f - top_p, 0x1p-24f)) + 1.5f; }
 };
 
 // ---------------------------------------------------------------------------------------------- a wave per row
@@ -889,7 +889,7 @@ struct BlockShared {
     float list_l[LIST];
     uint32_t list_at[LIST];
     unsigned long long wide[WAVES], above, own;
-    double sums[WAVES];
+    double sums[WAVES], room;
     float queue[WAVES][64 + 64 * 8];    // scores of the draw on their way to a full wave
     uint32_t words[WAVES], hist[256];
     __attribute__((aligned(16))) uint32_t bins[SET_BINS];
@@ -920,6 +920,17 @@ struct Cut {
 struct Drawn {
     uint32_t at;
     float prob;
+};
+
+// Even steps of the score, BINS of them over `reach` from the maximum down, what lies further down in the last.
+struct Steps {
+    float high, per;                    // per: steps per unit of the score
+    uint32_t fall;                      // powers of two that a weight falls by in a step, in units of 2^-20
+    __device__ Steps() {}
+    __device__ Steps(float maximum, float reach, float octaves) : high(maximum), per(fminf((float)BINS / reach, FLT_MAX)), fall((uint32_t)(octaves * (0x1p20f / (float)BINS))) {}
+    __device__ __forceinline__ uint32_t of(float l) const { return (uint32_t)fminf(fmaxf((high - l) * per, 0.0f), (float)(BINS - 1)); }      // (inf - inf: the first)
+    // Weights of step b are at most 2^-down(b), but for rounding: the step's largest or, where `per` was cut, less.
+    __device__ __forceinline__ int down(uint32_t b) const { return (int)(b * fall >> 20); }
 };
 
 // One row, worked on by a workgroup: all members are called by all its lanes.  The row is dealt to the waves in consecutive
@@ -1011,10 +1022,12 @@ struct BlockRow {
         for (; base < hi; base += STEP) step_of(base, load(base, hi), f);
     }
 
-    __device__ __forceinline__ unsigned long long fixed(double w) const
+    // A weight of step b in units of 2^-(s + down(b)).
+    __device__ __forceinline__ unsigned long long fixed(double w, const Steps &steps, uint32_t b) const
     {
-        // w 2^s + 2^52 has the rounded integer in its mantissa (s <= 51, w <= 1)
-        const double d = fma(w, __longlong_as_double((long long)(1023 + s) << 52), 0x1p52);
+        // w 2^(s + down) + 2^52 has the rounded integer in its mantissa (s <= 51); the power's exponent is s + b fall's whole part
+        const uint32_t power = (__umul24(b, steps.fall) + ((uint32_t)(1023 + s) << 20)) & 0xFFF00000u;
+        const double d = fma(w, __longlong_as_double((long long)((uint64_t)power << 32)), 0x1p52);
         return (unsigned long long)__double_as_longlong(d) & 0xFFFFFFFFFFFFFull;
     }
 
@@ -1266,13 +1279,18 @@ __device__ __forceinline__ Cut cut_of_list(const Row row, double border)
 // Radix selection over the whole row, up to 11 bits of the ordered key at a time, for the rows the list does not serve at once
 // (top_k beyond it, a border among more equal or nearly equal scores than it holds).  `old`: an earlier cut.  By count: the
 // first `border`; by mass: those whose mass before them is below it.  (Digits of 8 bits are the sign and seven of the exponent
-// first: a handful of bins, at whose addresses the additions queue.)
+// first: a handful of bins, at whose addresses the additions queue.)  By mass: among the scores of step `at`, in its units.
 template <class Row, class T, int THREADS, bool MASS>
-__device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long long border, const Cut o)
+__device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long long border, const Cut o, const Steps st, uint32_t at)
 {
     const Row row = r0.uniform();
     auto &sh = Row::shared();
     border = same((uint64_t)border);
+    at = same(at);
+    Steps steps;
+    steps.high = same(st.high);
+    steps.per = same(st.per);
+    steps.fall = same(st.fall);
     const Cut old{same(o.t), same(o.r), same(o.ties), 0};
     const uint32_t t = key_of(old.t);
     // the low bits of a widened 16-bit score follow from its sign: 16 of them for bf16, 13 for f16
@@ -1295,13 +1313,13 @@ __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long l
 #pragma unroll
             for (int e = 0; e < Row::PER; ++e) {
                 const uint32_t k = key_of(l[e]);
-                if (k <= KEY_LEAST || k < t || (MASS && k == t) || !ours(k)) continue;
-                atomicAdd(&sh.mass[mask - ((k >> shift) & mask)], MASS ? row.fixed(row.weigh(l[e])) : 1ull);
+                if (k <= KEY_LEAST || k < t || (MASS && (k == t || steps.of(l[e]) != at)) || !ours(k)) continue;
+                atomicAdd(&sh.mass[mask - ((k >> shift) & mask)], MASS ? row.fixed(row.weigh(l[e]), steps, at) : 1ull);
             }
         });
         __syncthreads();
-        if (MASS && old.r != 0 && ours(t)) {           // of the scores equal to t only r are left
-            if (threadIdx.x == 0) sh.mass[mask - ((t >> shift) & mask)] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
+        if (MASS && old.r != 0 && steps.of(old.t) == at && ours(t)) {       // of the scores equal to t only r are left
+            if (threadIdx.x == 0) sh.mass[mask - ((t >> shift) & mask)] += (unsigned long long)old.r * row.fixed(row.weigh(old.t), steps, at);
             __syncthreads();
         }
         const typename Row::Totals n = row.totals();
@@ -1334,7 +1352,7 @@ __device__ __attribute__((noinline)) Cut radix_cut(const Row r0, unsigned long l
         __syncthreads();
         c.ties = same(c.ties);
         const uint32_t most = nt == t ? min(c.ties, old.r) : c.ties;         // the border of an earlier cut
-        const unsigned long long w = row.fixed(row.weigh(c.t));
+        const unsigned long long w = row.fixed(row.weigh(c.t), steps, at);
         c.r = (uint32_t)min((unsigned long long)most, (border - above + w - 1) / max(w, 1ull));
         c.r = max(c.r, 1u);
     } else {
@@ -1500,14 +1518,13 @@ __device__ __attribute__((noinline)) Drawn row_draw(const Row r0, float edge, ui
 // The nucleus of a row with none or a count cut: masses by even steps of the score, from the maximum down to where the border
 // can be; then the scores of the step it falls in.
 template <class Row, class T, int THREADS>
-__device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, float reach, const Cut o)
+__device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, float reach, float octaves, const Cut o)
 {
     const Row row = r0.uniform();
     auto &sh = Row::shared();
     const Cut old{same(o.t), same(o.r), same(o.ties), 0};
     top_p = same(top_p);
-    const float high = row.weigh.top, per = (float)BINS / same(reach);
-    auto bin = [&](float l) { return (uint32_t)fminf(fmaxf((high - l) * per, 0.0f), (float)(BINS - 1)); };      // (inf - inf: the first)
+    const Steps steps(row.weigh.top, same(reach), same(octaves));
     for (uint32_t b = threadIdx.x; b < BINS; b += THREADS) sh.mass[b] = 0;
     __syncthreads();
     // the last bin, most of a row's scores, in registers: its additions would queue at one address
@@ -1517,8 +1534,8 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     row.template each<1>(lo, hi, [&](uint32_t, const float (&l)[Row::PER]) {
 #pragma unroll
         for (int e = 0; e < Row::PER; ++e) {
-            const unsigned long long f = row.fixed(row.weigh(l[e] > old.t ? l[e] : -INFINITY));  // (of the scores equal to old.t, r are left: added below)
-            const uint32_t b = bin(l[e]);
+            const uint32_t b = steps.of(l[e]);
+            const unsigned long long f = row.fixed(row.weigh(l[e] > old.t ? l[e] : -INFINITY), steps, b);  // (of the scores equal to old.t, r are left: added below)
             if (b < BINS - 1)
                 atomicAdd(&sh.mass[b], f);
             else
@@ -1527,18 +1544,58 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     });
     if (rest) atomicAdd(&sh.mass[BINS - 1], rest);
     __syncthreads();
-    if (old.r != 0 && threadIdx.x == 0) sh.mass[bin(old.t)] += (unsigned long long)old.r * row.fixed(row.weigh(old.t));
+    if (old.r != 0 && threadIdx.x == 0) {
+        const uint32_t b = steps.of(old.t);
+        sh.mass[b] += (unsigned long long)old.r * row.fixed(row.weigh(old.t), steps, b);
+    }
     __syncthreads();
-    const typename Row::Totals n = row.totals();
-    const unsigned long long border = same((uint64_t)ceil((double)top_p * (double)n.all));
-    unsigned long long above, own;
-    const uint32_t at_bin = row.border_of(n, border, above, own);
-    // (half a bin to spare on either side: the exact answer is bin()'s)
-    const float step = 1.0f / per, most = high - ((float)at_bin - 0.5f) * step;
-    const float least = at_bin + 1 < BINS ? high - ((float)at_bin + 1.5f) * step : -FLT_MAX;
+    // The bins' masses as numbers, summed in a fixed order: the border, the bin that reaches it and the mass in front of that.  (Bins without
+    // mass are passed over, also where a rounding would stop at one.)
+    constexpr uint32_t EACH = BINS / THREADS;
+    const auto mass = [&](uint32_t b) { return ldexp((double)sh.mass[b], -(row.s + steps.down(b))); };
+    double own = 0.0;
+#pragma unroll
+    for (uint32_t e = 0; e < EACH; ++e) own += mass(threadIdx.x * EACH + e);
+    const double upto = wave_scan(own);
+    if (Row::lane() == 63) sh.sums[Row::wave()] = upto;
+    __syncthreads();
+    double front = 0.0, all = 0.0;
+    for (int k = 0; k < Row::WAVES; ++k) {
+        front += k < (int)Row::wave() ? sh.sums[k] : 0.0;
+        all += sh.sums[k];
+    }
+    const double border = (double)top_p * all;
+    const uint64_t past = __ballot(own > 0.0 && front + upto >= border);
+    if (Row::lane() == 0) sh.words[Row::wave()] = past != 0;
+    __syncthreads();
+    int w = 0;
+    while (w + 1 < Row::WAVES && sh.words[w] == 0) ++w;
+    if (w == (int)Row::wave() && past && Row::lane() == (uint32_t)__ffsll((unsigned long long)past) - 1) {      // (top_p < 1: there is one)
+        double run = front + upto - own;
+        for (uint32_t e = 0; e < EACH; ++e) {
+            const uint32_t b = threadIdx.x * EACH + e;
+            if (sh.mass[b] == 0) continue;
+            sh.pick = b;
+            sh.room = border - run;
+            sh.own = sh.mass[b];
+            run += mass(b);
+            if (run >= border) break;
+        }
+    }
+    __syncthreads();
+    const uint32_t at_bin = same(sh.pick);
+    const double room = fmax(same(sh.room), DBL_MIN);
+    const unsigned long long in = same((uint64_t)sh.own);
+    __syncthreads();
+    // (half a bin to spare on either side: the exact answer is steps.of()'s)
+    const float step = 1.0f / steps.per, most = steps.high - ((float)at_bin - 0.5f) * step;
+    const float least = at_bin + 1 < BINS ? steps.high - ((float)at_bin + 1.5f) * step : -FLT_MAX;
     // (where the border of an earlier cut is in the step too, not all that are equal to it are in)
-    if ((old.r != 0 && bin(old.t) == at_bin) || !row.collect(least, most, [&](float l) { return bin(l) == at_bin; })) return radix_cut<Row, T, THREADS, true>(row, border, old);
-    return cut_of_list<Row, true>(row, (double)(border - above) * __longlong_as_double((long long)(1023 - row.s) << 52));
+    if ((old.r != 0 && steps.of(old.t) == at_bin) || !row.collect(least, most, [&](float l) { return steps.of(l) == at_bin; })) {
+        const double units = ceil(ldexp(room, row.s + steps.down(at_bin)));
+        return radix_cut<Row, T, THREADS, true>(row, min(max((unsigned long long)fmin(units, 0x1p62), 1ull), in), old, steps, at_bin);
+    }
+    return cut_of_list<Row, true>(row, room);
 }
 
 template <class T, int THREADS>
@@ -1569,10 +1626,10 @@ __global__ void __launch_bounds__(THREADS) k_sample_block(const SampleArgs a)
                         done = true;
                     }
                 }
-                if (!done) c = radix_cut<Row, T, THREADS, false>(row, p.top_k, c);
+                if (!done) c = radix_cut<Row, T, THREADS, false>(row, p.top_k, c, Steps(), 0);
             }
             if (!done) {
-                if (p.top_p < 1.0f) c = mass_cut<Row, T, THREADS>(row, p.top_p, p.reach(a.V), c);
+                if (p.top_p < 1.0f) c = mass_cut<Row, T, THREADS>(row, p.top_p, p.reach(a.V), p.octaves(a.V), c);
                 const uint32_t last_equal = c.last == UNKNOWN ? nth_equal(row, c.t, c.r) : c.last;
                 // scores this far below the maximum miss min_p whatever the rounding
                 const double least = p.min_p > 0.0f ? (double)fminf(p.min_p, 1.0f) : 0.0;
