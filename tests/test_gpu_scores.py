@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from vq_amd import Context, _lib
+from vq_amd import Context, VqhipError, _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -138,6 +138,32 @@ def test_a_model_costs_a_copy_until_scores_are_asked_for(ctx):
         return min(t)
 
     assert best(lambda: ctx.set_prototypes(W)) <= 4 * best(lambda: torch.from_numpy(W.copy()).cuda())
+
+
+# ---------------------------------------------------------------------------------------------- no room for the layout
+def test_a_layout_that_finds_no_memory_leaves_nothing_behind():
+    """The first scores call of a model needs 6 bytes a prototype value.  Where the card has none left it says so, and neither the next
+    operation nor the call itself, once there is room, sees that error again."""
+    g = gen(8)
+    W, X = torch.rand(1 << 19, 512, generator=g), torch.rand(5, 512, generator=g).cuda()
+    out = torch.empty(5, 1 << 19, device="cuda")
+    with Context(0) as c:
+        c.set_prototypes(W.numpy())
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        free, _ = torch.cuda.mem_get_info()
+        held = torch.empty(free - (96 << 20), dtype=torch.uint8, device="cuda")          # (the layout is 1.6 GB)
+        try:
+            with pytest.raises(VqhipError) as e:
+                c.scores(X, out=out)
+            assert e.value.code == _lib.ERR_NOMEM
+            assert out.fill_(3.0).eq(3.0).all().item()
+        finally:
+            del held
+            torch.cuda.empty_cache()
+        c.scores(X, out=out)
+        want = exact(X.cpu(), W[:50])
+        assert (np.abs(wide(out[:, :50]) - want) <= 1e-5 * np.abs(want)).all()
 
 
 # ---------------------------------------------------------------------------------------------- more than a launch holds

@@ -136,6 +136,7 @@ struct vqhip_ctx {
     }
     int fail_hip(hipError_t e, const char *what)
     {
+        (void)hipGetLastError();           // reported here: not once more by the thread's next launch, ours or the caller's
         err = std::string(what) + ": " + hipGetErrorString(e);
         return e == hipErrorOutOfMemory ? VQHIP_ERR_NOMEM : VQHIP_ERR_HIP;
     }
