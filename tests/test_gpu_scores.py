@@ -111,6 +111,76 @@ def test_assign_sampled_is_scores_and_sample_in_every_workspace(ctx, D):
             assert rc == 0 and torch.equal(i, idx) and torch.equal(p, prob), (how, rows)
 
 
+# ---------------------------------------------------------------------------------------------- the widest tile
+@pytest.mark.parametrize("N,K,D", [(262144 + 3, 256, 20), (140000, 509, 17), (262144 - 128 + 1, 250, 36)])
+@pytest.mark.parametrize("kind", ["spread", "few", "groups"])
+def test_scores_of_so_many_samples_that_tiles_are_widest(ctx, N, K, D, kind):
+    """2048 tiles of 128 x 256 or more.  Spread samples, ones with a close prototype each, and groups that fill whole tiles; the rows at
+    both ends, the columns at both ends and every 61st row against 64 bits."""
+    if kind == "groups":
+        X, W = groups(N, K, D, 2, N)
+    else:
+        g = gen(N)
+        W = torch.rand(K, D, generator=g) * 2 - 1
+        X = torch.rand(N, D, generator=g) * 2 - 1
+        if kind == "few":
+            X = W[torch.randint(K, (N,), generator=g)] + 0.02 * X
+    ctx.set_prototypes(W.numpy())
+    buf = torch.full((N, K + 3), 7.0, device="cuda")
+    S = ctx.scores(X.cuda(), out=buf[:, 1:K + 1])
+    assert (buf[:, 0] == 7).all() and (buf[:, K + 1:] == 7).all()
+    pick = torch.cat([torch.arange(0, N, 61), torch.arange(200), torch.arange(N - 200, N)])
+    want = exact(X[pick], W)
+    assert (np.abs(wide(S[pick.cuda()]) - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want)).all()
+    for cols in ([0, 1, 63, 64, 65, 127, 128, 129, 191, 192, K - 2, K - 1],):
+        want = exact(X, W[cols])
+        assert (np.abs(wide(S[:, cols]) - want) <= 8 * (2 * D + 6) * 2.0 ** -24 * np.abs(want)).all()
+    small = ctx.scores(X[1000:1700].cuda())
+    assert torch.equal(small, S[1000:1700])
+
+
+# ---------------------------------------------------------------------------------------------- all six products
+@pytest.mark.parametrize("D", [17, 33, 100, 784, 1000])
+def test_every_piece_of_every_value_counts(ctx, D):
+    """Samples and prototypes with one value each, +-a, of three full bf16 pieces: a product of two such values is a single term, so its
+    rounding errors do not grow with D.  The prototypes come in pairs +a, -a: their mean is exactly 0.  With e = 2^-24 and B = x^2 + w^2
+    (twice |x w| where both are in the same place and of about one size): the norms e B, the sum of six exact products at most 5 e |x w|, doubled,
+    what they leave out (below 2^-26 |x w|, doubled) e |x w|, B itself e B, the last addition e |s| <= 2 e B: 4 e B + 11 e |x w| <= 10 e B.
+    A product left out or taken twice, or a piece from another place, is off by 2^-17 |x w| and more, six times as much."""
+    g = gen(D)
+    a = 1.0 + 0.2 * torch.rand(8192, generator=g)
+    p1 = a.bfloat16().float()
+    p2 = (a - p1).bfloat16().float()
+    p3 = a - p1 - p2
+    a = a[(p2.abs() > 0.6 * 2.0 ** -8) & (p3.abs() > 0.6 * 2.0 ** -17)]
+    assert len(a) > 50
+    W, X = torch.zeros(2 * D, D), torch.zeros(D, D)
+    at = torch.arange(D)
+    W[2 * at, at] = a[at % len(a)]
+    W[2 * at + 1, at] = -a[at % len(a)]
+    X[at, at] = a[(at * 7 + 3) % len(a)]
+    ctx.set_prototypes(W.numpy())
+    S = wide(ctx.scores(X.cuda()))
+    want = exact(X, W)
+    B = wide(X.double().square().sum(1))[:, None] + wide(W.double().square().sum(1))[None]
+    close = np.abs(want) < B / 15                                          # measured directly
+    assert (np.abs(S - want)[~close] <= 10 * 2.0 ** -24 * B[~close]).all()
+    assert (np.abs(S - want)[close] <= (D + 3) * 2.0 ** -24 * np.abs(want)[close]).all()
+    assert close[at, 2 * at].all() and not close[at, 2 * at + 1].any()
+
+
+@pytest.mark.parametrize("N,D,K", [(300, 128, 256), (70, 784, 100), (130, 1000, 70)])
+@pytest.mark.parametrize("offset", [0.0, 100.0])
+def test_scores_are_within_the_library_s_bar(ctx, N, D, K, offset):
+    """1e-5 of the distance, whatever the length."""
+    g = gen(D)
+    W = torch.rand(K, D, generator=g) * 2 - 1 + offset
+    X = W[torch.randint(K, (N,), generator=g)] + 0.5 * (torch.rand(N, D, generator=g) * 2 - 1)
+    ctx.set_prototypes(W.numpy())
+    want = exact(X, W)
+    assert (np.abs(wide(ctx.scores(X.cuda())) - want) <= 1e-5 * np.abs(want)).all()
+
+
 # ---------------------------------------------------------------------------------------------- models
 def test_scores_follow_the_model(ctx):
     """A model after another, of other sizes, larger and smaller, with few prototypes and many."""
