@@ -360,6 +360,7 @@ class Context:
             K, D, ldt, code, dtype, src = self.K, self.D, self.D, _lib.F32, torch.float32, None
         else:
             K, D, ldt, code = self._check_rows(table, "table")
+            self._check_table(K)
             dtype, src = table.dtype, table.data_ptr()
         if out is None:
             out, ldy = torch.empty(*idx.shape, D, dtype=dtype, device=idx.device), D
@@ -384,6 +385,7 @@ class Context:
         rows = self._rows_of(grad, "grad", idx, D)
         _, _, ldg, code = self._check_rows(rows, "grad")
         K = self.K if K is None else int(K)
+        self._check_table(K)
         if K < 1 or D < 1:
             raise ValueError("the table must have at least one row and one column")
         if out is None:
@@ -472,10 +474,18 @@ class Context:
         if code is None:
             raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
         n, width = t.shape
+        if width >> 32:
+            raise ValueError(f"{name} must have rows of fewer than 2^32 elements")
         ld, step = t.stride()
         if (width > 1 and step != 1) or (n > 1 and ld < width):
             raise ValueError(f"{name} must have contiguous rows that do not overlap")
         return n, width, ld if n > 1 else width, code
+
+    @staticmethod
+    def _check_table(K):
+        """What the library takes as 32 bits (and refuses from 2^31 on)."""
+        if K >> 32:
+            raise ValueError("the table must have fewer than 2^32 rows")
 
     @staticmethod
     def _check_out(t, n, width, dtypes):
