@@ -1,4 +1,4 @@
-"""CPU: sizes that do not fit the 32 bits in which the library takes them are refused before it is called."""
+"""CPU: sizes that do not fit the 32 bits in which the library takes them, and shapes at their ends, are refused before it is called."""
 import pytest
 import torch
 
@@ -34,3 +34,13 @@ def test_tables_and_rows_beyond_32_bits_are_refused(size):
 def test_negative_tables_are_refused():
     with pytest.raises(ValueError):
         handle().lookup_gradient(empty(2, 4), empty(2, dtype=torch.int32), K=-1)
+
+
+def test_results_without_dimensions_are_refused():
+    """One index has no dimension; its result has one."""
+    c, one = handle(), empty(dtype=torch.int32)
+    for out in (empty(), empty(5), empty(1, 4)):
+        with pytest.raises(ValueError):
+            c.lookup(one, table=empty(3, 4), out=out)
+    with pytest.raises(ValueError):
+        c.lookup_gradient(empty(), one, K=3)

@@ -450,7 +450,7 @@ class Context:
     @staticmethod
     def _rows_of(t, name, idx, D):
         """A tensor of shape idx.shape + (D,) as N rows."""
-        if not _is_torch(t) or t.shape[:-1] != idx.shape or t.shape[-1] != D:
+        if not _is_torch(t) or t.dim() == 0 or t.shape[:-1] != idx.shape or t.shape[-1] != D:
             raise ValueError(f"{name} must be of shape {(*idx.shape, D)}")
         if t.dim() == 2:
             return t
