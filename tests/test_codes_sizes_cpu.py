@@ -13,7 +13,7 @@ def handle():
 
 
 def empty(*shape, dtype=torch.float32):
-    return torch.empty(*shape, dtype=dtype, device="meta")
+    return torch.empty(shape, dtype=dtype, device="meta")
 
 
 @pytest.mark.parametrize("size", [1 << 32, (1 << 32) + 5, (1 << 33) + 1])
