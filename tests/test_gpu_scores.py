@@ -221,15 +221,20 @@ def test_a_layout_that_finds_no_memory_leaves_nothing_behind():
         c.set_prototypes(W.numpy())
         torch.cuda.synchronize()
         torch.cuda.empty_cache()
-        free, _ = torch.cuda.mem_get_info()
-        held = torch.empty(free - (96 << 20), dtype=torch.uint8, device="cuda")          # (the layout is 1.6 GB)
+        held = []
         try:
+            for size in (16 << 30, 1 << 30, 128 << 20):                                      # (the layout is 1.6 GB)
+                try:
+                    while True:
+                        held.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+                except torch.OutOfMemoryError:
+                    pass
             with pytest.raises(VqhipError) as e:
                 c.scores(X, out=out)
             assert e.value.code == _lib.ERR_NOMEM
             assert out.fill_(3.0).eq(3.0).all().item()
         finally:
-            del held
+            held.clear()
             torch.cuda.empty_cache()
         c.scores(X, out=out)
         want = exact(X.cpu(), W[:50])
