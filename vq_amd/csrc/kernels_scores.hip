@@ -717,7 +717,7 @@ hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *d
         const uint64_t wide = c256 * 40, middle = c128 * 22, slim = c64 * 15;
         if (rows * c256 >= 2048 && wide <= middle && wide <= slim) return run_mfma<2, 4, 2, 2, 2>(a, s);
         if (rows * c128 >= 512 && middle <= slim) return run_mfma<2, 2, 2, 2, 2>(a, s);
-        return run_mfma<1, 1, 2, 2, 4>(a, s);
+        return run_mfma<1, 1, 2, 2, 5>(a, s);
     }
     // (the narrowest tile that pads the prototypes least)
     if (K <= 32) return run_direct<4>(a, s);
