@@ -273,7 +273,8 @@ typedef enum { VQHIP_F32 = 0, VQHIP_BF16 = 1, VQHIP_F16 = 2 } vqhip_dtype;
  * without the root), N x K, rows lds apart.  Euclidean models only (VQHIP_ERR_UNSUPPORTED with an Omega).  A softmax of
  * S / T is the distribution over codes that vqhip_assign_sampled_device draws from.  f32, in the direct form or, for rows of
  * more than 16 values, on the matrix cores as |x - c|^2 + |w - c|^2 - 2 (x - c).(w - c) with c the mean prototype; distances
- * small beside those norms are measured in the direct form there too, so a sample equal to a prototype scores 0 exactly. */
+ * small beside those norms are measured in the direct form there too, so a sample equal to a prototype scores 0 exactly.  A score
+ * depends on its sample and the model alone: the same bits whatever other rows the call has. */
 int vqhip_scores_device(vqhip_ctx *ctx, const float *dX, uint64_t N, float *dS, uint64_t lds, void *stream);
 
 /* How to draw: one value for all rows, or, where the pointer is not NULL, one per row (N values on the device).
@@ -305,7 +306,7 @@ int vqhip_sample_device(vqhip_ctx *ctx, const void *dS, int dtype, uint64_t N, u
 
 /* vqhip_assign_device with the winner drawn instead of nearest: vqhip_scores_device and vqhip_sample_device, a chunk of rows at a
  * time through dwork (at least K floats, 4-byte aligned; vqhip_assign_sampled_workspace gives the size that keeps the card
- * busy and the chunk in the last-level cache).  Results are those of the two calls. */
+ * busy and the chunk in the last-level cache).  Results are those of the two calls, bit for bit, whatever the workspace's size. */
 int vqhip_assign_sampled_workspace(vqhip_ctx *ctx, uint64_t N, size_t *bytes);
 int vqhip_assign_sampled_device(vqhip_ctx *ctx, const float *dX, uint64_t N, const vqhip_sampling *how, const float *du, uint32_t *didx_out,
                                 float *dprob_out, void *dwork, size_t work_bytes, void *stream);

@@ -335,7 +335,7 @@ class Context:
 
     def assign_sampled(self, X, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """vqhip_assign_sampled_device: assign with the winner drawn from softmax(-||x - w||^2 / temperature) instead of nearest
-        (temperature 0: the nearest) -> (idx int32, prob float32).  Equals sample(scores(X), u, ...)."""
+        (temperature 0: the nearest) -> (idx int32, prob float32).  The same bits as sample(scores(X), u, ...)."""
         self._check_torch(X)
         N = X.shape[0]
         how = self._sampling(N, u, temperature, top_k, top_p, min_p)
@@ -350,7 +350,8 @@ class Context:
     def lookup(self, idx, table=None, scale=1.0, out=None):
         """vqhip_lookup_device: scale * table[idx] for a CUDA int32 tensor of any shape -> idx.shape + (D,) in the table's type.
         table: K x D float32, bfloat16 or float16 (rows may be strided); None: the context's prototypes.  An index outside
-        [0, K), -1 for padding, gives zeros."""
+        [0, K), -1 for padding, gives zeros.  The result is not part of torch's autograd, also where the table is: lookup_gradient
+        is the way back.  (torch's own indices are int64: idx.int().)"""
         import torch
 
         N = self._check_index(idx)
@@ -375,7 +376,8 @@ class Context:
         """vqhip_lookup_gradient_device: the gradient of lookup(idx, table, scale) with respect to the table, given that of its
         result (idx.shape + (D,), float32, bfloat16 or float16) -> K x D (default K: the context's prototypes) in float32 or
         grad's type (out_dtype or out's; default float32).  accumulate adds to `out`.  want_counts: also how many indices name
-        each row (int32).  The sums are float32 in an order that depends on the inputs alone."""
+        each row (int32).  The sums are float32 in an order that depends on the inputs alone.  torch's autograd does not call
+        it by itself."""
         import torch
 
         N = self._check_index(idx)

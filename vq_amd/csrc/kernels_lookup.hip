@@ -18,7 +18,7 @@
 //              chunk borders go to the workspace in f32
 //     join     k_grad_join: adds up the parts of those runs in order, writes the rows no index names, and the counts
 //
-// What bounds them: memory.  Lookup of 2000000 rows of 128 out of 256, f32: 179 us, stores at 5.7 TB/s (a fill of this card: 6.8).
+// What bounds them: memory.  Lookup of 2000000 rows of 128 out of 256, f32: 177 us, stores at 5.8 TB/s (a fill of this card: 6.8).
 // Gradient of 2000000 rows of 128 over 256, f32: 242 us, of which the sums are 195 at 5.2 TB/s, read in the order of the indices, and
 // the sort 36.  16384 rows of 4096 over 65536, bf16 to f32: 266 us, of which clearing the rows nobody names is about 165 at
 // 5.6 TB/s, the sums 50 at 6 TB/s.

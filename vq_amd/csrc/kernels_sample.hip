@@ -18,11 +18,10 @@
 // hundred scores the filters are decided among and hands those to the same code as a wave's row; it reads the row three or
 // four times, all but the first from the caches.
 //
-// What bounds them: the vector units, not memory.  A weight in f64 is 23 instructions and there is no shorter exact way.  400000 x
-// 256 f32 with top_p 0.9: 236 us, 356 vector instructions a row, the units busy all the time (reading the scores once is 103 us
-// at the rate of a large copy).  256 x 131072 bf16 with top_p 0.9: 100 us, of which the weights and their histogram are about
-// 40, the four passes over memory and caches the rest.  1 x 131072 bf16 with top_k 50 and top_p 0.9: 19 us, one workgroup's
-// latency.
+// What bounds them: the vector units, not memory.  A weight in f64 is 23 instructions.  400000 x 256 f32 with top_p 0.9: 233 us, 356 vector
+// instructions a row, 92 of them the weights, the units busy all the time (reading the scores once is 89 us at the rate of a large copy).
+// 256 x 131072 bf16 with top_p 0.9: 98 us, the units busy 71 %, 74 instructions a score over the four passes, 46 of them its two
+// weights.  1 x 131072 bf16 with top_k 50 and top_p 0.9: 19 us, one workgroup's latency.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -1693,8 +1692,8 @@ hipError_t run_sample(const SampleArgs &a, uint64_t rows, hipStream_t s)
     if (a.V <= 512) return run_wave<T, 8>(a, s);
     if (a.V <= 1024) return run_wave<T, 16>(a, s);
     // A small workgroup wastes less at its barriers, a large one is done sooner where there are fewer rows than CUs, or long ones.  us at
-    // 256 / 512 / 1024 lanes, top_p 0.9: 8192 x 4096 150 / - / 461; 256 x 16384 32 / 25 / 27, 1024 x 16384 59 / 64 / 100; 256 x 50000
-    // 79 / 58 / 55, 512 x 50000 101 / 87 / 103; bf16 256 x 131072 187 / 118 / 105, 512 x 131072 224 / 225 / 193
+    // 256 / 512 / 1024 lanes, top_p 0.9: 8192 x 4096 151 / 241 / 481; 256 x 16384 31 / 24 / 26, 1024 x 16384 60 / 62 / 99; 256 x 50000
+    // 76 / 58 / 54, 512 x 50000 98 / 84 / 102; bf16 256 x 131072 177 / 114 / 98, 512 x 131072 219 / 220 / 188
     if (a.V <= 8192) return run_block<T, 256>(a, s);
     if (a.V <= 32768 || (a.V <= 65536 && rows > 256)) return run_block<T, 512>(a, s);
     return run_block<T, 1024>(a, s);

@@ -11,11 +11,12 @@
 // of the two norms, so the pairs whose distance is small beside them (below CLOSE of their sum: a sample and the few
 // prototypes next to it) are measured again in the direct form, by 4 lanes a pair, or a square of pairs where they are many.  Which
 // form a pair takes and the order of its sums depend on the pair alone, not on the tile or the pairs beside it: a score has the same
-// bits whatever other rows a call has.  500000 x 128 against 256, us: samples with a close prototype each 369, half of all pairs close 1240.
+// bits whatever other rows a call has.  500000 x 128 against 256, us: no pair close 261, a close prototype for each sample 318, half of
+// all pairs close 1250.
 //
-// What bounds them: the matrix cores where rows are long (20011 x 784 against 1000 178 us, 1060 TFLOP/s over the six products; a
+// What bounds them: the matrix cores where rows are long (20011 x 784 against 1000 179 us, 1050 TFLOP/s over the six products; a
 // library's bf16 product reaches 1195 here), staging, products and the stores of a tile in turn where they are short (500000 x 128 against
-// 256 246 us, 3.1 TB/s, the matrix pipe busy 39 %), the scores' stores where the prototypes are few (500000 x 4 against 256 92 us, 5.6 TB/s).
+// 256 245 us, 3.1 TB/s, the matrix pipe busy 40 %), the scores' stores where the prototypes are few (500000 x 4 against 256 92 us, 5.6 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -221,17 +222,17 @@ __global__ void __launch_bounds__(SC_THREADS) k_scores_few(const ScoreArgs a)
 
 // ---------------------------------------------------------------------------------------------- matrix cores
 // Which kernel.  us for 500000 samples (a lane per sample / direct tiles of 32, 64 or 128 prototypes / matrix cores):
-//     16 values: 3 prototypes 7.4 / 53 / 25, 16 prototypes 23 / 25 / 27, 32 prototypes 51 / 27 / 28, 64 prototypes 115 / 35 / 28,
-//                256 prototypes 438 / 137 / 116
-//      8 values: 16 prototypes 17 / 21 / 27, 64 prototypes 126 / 30 / 28, 256 prototypes 363 / 95 / 116
-//     32 values: 16 prototypes 35 / 96 / 31, 256 prototypes 524 / 203 / 133
-// The lanes of k_scores_few store K apart, which is what it costs: K^2 D up to 4096.  The direct form is kept to 16 values although
-// the matrix cores are as fast from 9 on: it has the smaller error.
+//     16 values: 3 prototypes 7.2 / 24 / 28, 16 prototypes 23 / 26 / 34, 32 prototypes 51 / 28 / 35, 64 prototypes 119 / 36 / 35,
+//                256 prototypes 438 / 137 / 120
+//      8 values: 16 prototypes 16 / 19 / 35, 64 prototypes 122 / 30 / 36, 256 prototypes 361 / 100 / 124
+//     32 values: 16 prototypes 36 / 44 / 35, 256 prototypes 524 / 224 / 135
+// The lanes of k_scores_few store K apart, which is what it costs: K^2 D up to 4096.  The direct form is kept to 16 values, where the
+// matrix cores are ahead against many prototypes: it has the smaller error.
 constexpr uint32_t FEW_D = 32, FEW_K = 32;      // k_scores_few
 constexpr uint32_t DIRECT_D = 16;               // k_scores_direct
 // Of |x - c|^2 + |w - c|^2; distances below it are measured directly.  The products' error is a few 2^-24 of the norms, so at 1/16
 // a distance is within a few 1e-6 of itself (the bar of this library is 1e-5); at 1/8 the samples of a codebook would take
-// their own prototype's way through the direct form too, 45 us more on 500k x 128 against 256.
+// their own prototype's way through the direct form too, 55 us more on 500k x 128 against 256.
 constexpr float CLOSE = 0.0625f;
 constexpr int MF_K = 16;
 // Norms above this become NaN, and with them every score made from them, so that such pairs are measured directly: the sum of two norms up
@@ -709,8 +710,8 @@ hipError_t launch_scores(const float *dX, uint64_t N, uint32_t D, const float *d
     }
     if (D > DIRECT_D) {
         // Larger tiles read both operands less often, smaller ones leave fewer of the 512 places (two workgroups a CU) empty in the last
-        // round.  us, 128 x 256 / 128 x 128 / 64 x 64 tiles: 500k x 128 against 256 (3907 wide tiles) 270 / 295 / 399, 20011 x 784
-        // against 1000 (628) 209 / 203 / 278
+        // round.  us, 128 x 256 / 128 x 128 / 64 x 64 tiles: 500k x 128 against 256 (3907 wide tiles) 256 / 274 / 342, 500k x 64 187 / 191 /
+        // 242, 20011 x 784 against 1000 (628) 194 / 176 / 237
         // Where prototypes would leave a large part of a wide tile empty, a narrower one is taken: what a tile of each kind costs per
         // column is 1 / 1.1 / 1.5.
         const uint64_t rows = (N + 127) / 128, c64 = ((uint64_t)K + 63) / 64, c128 = (c64 + 1) / 2, c256 = (c64 + 3) / 4;
