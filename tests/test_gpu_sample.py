@@ -171,3 +171,23 @@ def test_temperatures_of_any_size(ctx, V, t):
             j, p, margin = ref.sample_row(rows[i].numpy(), u[i].item(), temperature=t, **how)
             if margin > 1e-12:
                 assert idx[i].item() == j and abs(prob[i].item() - p) <= (2.0 ** -24 + 1e-9) * p, (i, how, idx[i].item(), j, margin)
+
+
+@pytest.mark.parametrize("V", [40, 700, 1500, 9001])
+@pytest.mark.parametrize("t", [1e-44, 1.0, 1e37, 1e38, 3e38])
+def test_infinite_scores_at_temperatures_of_any_size(ctx, V, t):
+    """A row's infinite scores share it, however small the others are beside the temperature; where they are many, a nucleus ends among them."""
+    g = gen(V)
+    rows = torch.randn(5, V, generator=g)
+    rows[0, V // 2] = INF
+    rows[1, ::3] = INF
+    rows[2, 5:] = INF
+    rows[3, [0, V - 1]] = INF
+    rows[4, ::2], rows[4, 1::4] = -INF, INF
+    u = torch.tensor([0.5, 0.999, 0.3, 0.75, 0.9])
+    for how in (dict(), dict(top_p=0.9), dict(top_p=0.3), dict(top_p=0.999, min_p=0.01), dict(top_k=V // 2, top_p=0.5), dict(top_k=3)):
+        idx, prob = ctx.sample(rows.cuda(), u.cuda(), temperature=t, **how)
+        for i in range(len(rows)):
+            j, p, margin = ref.sample_row(rows[i].numpy(), u[i].item(), temperature=t, **how)
+            if margin > 1e-12:
+                assert idx[i].item() == j and abs(prob[i].item() - p) <= (2.0 ** -24 + 1e-9) * p, (i, how, idx[i].item(), j, margin)

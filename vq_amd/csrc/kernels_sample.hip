@@ -1588,7 +1588,7 @@ __device__ __attribute__((noinline)) Cut mass_cut(const Row r0, float top_p, flo
     __syncthreads();
     // (half a bin to spare on either side: the exact answer is steps.of()'s)
     const float step = 1.0f / steps.per, most = steps.high - ((float)at_bin - 0.5f) * step;
-    const float least = at_bin + 1 < BINS ? steps.high - ((float)at_bin + 1.5f) * step : -FLT_MAX;
+    const float least = steps.high == INFINITY ? INFINITY : at_bin + 1 < BINS ? steps.high - ((float)at_bin + 1.5f) * step : -FLT_MAX;   // (inf - inf: no such bound)
     // (where the border of an earlier cut is in the step too, not all that are equal to it are in)
     if ((old.r != 0 && steps.of(old.t) == at_bin) || !row.collect(least, most, [&](float l) { return steps.of(l) == at_bin; })) {
         const double units = ceil(ldexp(room, row.s + steps.down(at_bin)));
