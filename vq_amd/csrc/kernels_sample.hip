@@ -925,7 +925,7 @@ struct Drawn {
 struct Steps {
     float high, per;                    // per: steps per unit of the score
     uint32_t fall;                      // powers of two that a weight falls by in a step, in units of 2^-20
-    __device__ Steps() {}
+    __device__ Steps() : high(0.0f), per(0.0f), fall(0) {}
     __device__ Steps(float maximum, float reach, float octaves) : high(maximum), per(fminf((float)BINS / reach, FLT_MAX)), fall((uint32_t)(octaves * (0x1p20f / (float)BINS))) {}
     __device__ __forceinline__ uint32_t of(float l) const { return (uint32_t)fminf(fmaxf((high - l) * per, 0.0f), (float)(BINS - 1)); }      // (inf - inf: the first)
     // Weights of step b are at most 2^-down(b), but for rounding: the step's largest or, where `per` was cut, less.
